@@ -25,6 +25,12 @@ PATH_AUTO = 0
 PATH_GEMV = 1
 PATH_GEMM = 2
 PEER_HANDLE_BYTES = 64
+DT_F32 = 0
+DT_BF16 = 1
+DT_F16 = 2
+KV_BLOCK = 32
+KV_MAX_REQUESTS = 8192
+TOPK_MAX = 32
 
 _vp = ctypes.c_void_p
 _sz = ctypes.c_size_t
@@ -79,6 +85,13 @@ SIGNATURES = {
     "mxq_decoder_embedding": [_vp, _sz, _sz, _vp],
     "mxq_decoder_set_trace": [_vp, _i],
     "mxq_decoder_get_trace": [_vp, _i, _vp, _sz],
+    "mxq_kv_plan": [_vp, _vp, _vp, _sz, _sz, _vp, _sz, _vp, _sz, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _vp],
+    "mxq_kv_release": [_vp, _vp, _vp, _sz, _sz, _vp, _sz, _vp, _sz, _vp],
+    "mxq_kv_append": [_vp, _vp, _i, _vp, _vp, _sz, _vp, _sz],
+    "mxq_kv_read": [_vp, _vp, _vp, _sz, _i, _vp, _vp],
+    "mxq_kv_attention": [_vp, _vp, _i, _vp, _sz, _sz, _sz, _vp, _sz, _vp, _vp, _sz, _sz, _f, _vp, _vp],
+    "mxq_token_logprobs": [_vp, _i, _vp, _sz, _sz, _sz, _vp, _sz, _vp, _vp, _vp, _vp, _vp],
+    "mxq_token_logprobs_grad": [_vp, _i, _vp, _sz, _sz, _sz, _vp, _vp, _vp, _vp, _vp, _vp, _sz],
     "mxq_weight_download": [_vp, _vp, _vp],
     "mxq_weight_save": [_vp, ctypes.c_char_p],
     "mxq_update_gaussian_moment": [_vp, _vp, _vp, _vp, _f],

@@ -72,6 +72,13 @@ struct mxq_context {
   static constexpr size_t kMaxHostGraphs = 64;
   std::vector<HostGraph> graphs;
   uint64_t graph_clock = 0;
+  // serving operators: one workspace for each stream they ran on
+  struct StreamWs {
+    cudaStream_t stream;
+    uint8_t* base;
+  };
+  std::vector<StreamWs> serve_ws;
+  int sms = 0;
 };
 
 struct mxq_weight_s {
@@ -637,6 +644,7 @@ int mxq_destroy(mxq_ctx c) {
     cudaFree(c->ws_out);
     cudaFree(c->ws_moe);
     cudaFree(c->ws_yr);
+    for (auto& w : c->serve_ws) cudaFree(w.base);
     for (auto& g : c->graphs)
       if (g.exec) cudaGraphExecDestroy(g.exec);
     if (c->pin_in) cudaFreeHost(c->pin_in);
@@ -2329,6 +2337,36 @@ int ctx_device(mxq_context* c) { return c->device; }
 void ctx_add_launches(mxq_context* c, uint64_t n) { c->launches += n; }
 uint64_t ctx_ws_gen(mxq_context* c) { return c->ws_gen; }
 uint64_t ctx_launches(mxq_context* c) { return c->launches; }
+
+int ctx_serve_ws(mxq_context* c, ServeWs* out) {
+  try {
+    uint8_t* base = nullptr;
+    for (auto& w : c->serve_ws)
+      if (w.stream == c->stream) base = w.base;
+    if (!base) {
+      if (c->sms == 0) {
+        const cudaError_t e = cudaDeviceGetAttribute(&c->sms, cudaDevAttrMultiProcessorCount, c->device);
+        if (e != cudaSuccess) return cuda_fail(c, e, "multiprocessor count");
+      }
+      c->serve_ws.reserve(c->serve_ws.size() + 1);
+      void* p = nullptr;
+      cudaError_t e = cudaMalloc(&p, kServeCounters * 4 + kServeScratch);
+      if (e == cudaSuccess) e = cudaMemsetAsync(p, 0, kServeCounters * 4, c->stream);
+      if (e != cudaSuccess) {
+        cudaFree(p);
+        return cuda_fail(c, e, "serving workspace");
+      }
+      base = static_cast<uint8_t*>(p);
+      c->serve_ws.push_back({c->stream, base});
+    }
+    out->counters = reinterpret_cast<uint32_t*>(base);
+    out->scratch = base + kServeCounters * 4;
+    out->sms = c->sms;
+    return MXQ_OK;
+  } catch (...) {
+    return fail(c, MXQ_ERR_OUT_OF_MEMORY, "host allocation failed");
+  }
+}
 void ctx_set_launches(mxq_context* c, uint64_t n) { c->launches = n; }
 const WeightView* weight_view(mxq_weight w) { return w ? &w->v : nullptr; }
 

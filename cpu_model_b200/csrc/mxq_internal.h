@@ -236,6 +236,22 @@ uint64_t ctx_launches(mxq_context* c);
 void ctx_set_launches(mxq_context* c, uint64_t n);
 const WeightView* weight_view(mxq_weight w);
 
+// Workspace of the serving operators (mxq_kv.cu, mxq_kvattn.cu), one for each
+// stream that a context has used them on, so that calls on two streams do not
+// meet in it: counters that every kernel leaves zero, then bytes that hold
+// nothing from one call to the next.
+constexpr size_t kServeCounters = 2048;                  // uint32
+constexpr size_t kServeScratch = 12u << 20;              // bytes
+struct ServeWs {
+  uint32_t* counters;
+  uint8_t* scratch;
+  int sms;
+};
+int ctx_serve_ws(mxq_context* c, ServeWs* out);
+
+// A row type of the serving operators (MXQ_DT_*): bytes an element, 0 unknown.
+inline size_t dtype_bytes(int dt) { return dt == MXQ_DT_F32 ? 4 : dt == MXQ_DT_BF16 || dt == MXQ_DT_F16 ? 2 : 0; }
+
 // Dense decoder steps (mxq_decoder_kernels.cu).
 cudaError_t dk_embed(const int32_t* tok, const float* table, int R, int d, int vocab, float* h, cudaStream_t s);
 cudaError_t dk_rmsnorm(const float* x, const float* g, int R, int d, float eps, float* y, cudaStream_t s);

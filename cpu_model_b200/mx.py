@@ -16,7 +16,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from ._lib import ACT_NONE, ACT_SILU, FMT_INT4, FMT_INT8, PATH_AUTO, PATH_GEMM, PATH_GEMV, check
+from ._lib import ACT_NONE, ACT_SILU, DT_BF16, DT_F16, DT_F32, FMT_INT4, FMT_INT8, PATH_AUTO, PATH_GEMM, PATH_GEMV, check
 
 __all__ = [
     "MXContext", "MXWeight", "MXActivation", "context",
@@ -25,6 +25,8 @@ __all__ = [
     "mx_rank16_dot_ptrs", "mx_block_dots", "mx_linear", "mx_linear_pair",
     "gated_mlp_step", "route_topk", "HashedRouter", "HaltingState", "halting_step", "mx_quantize_w",
     "fused_compute_gae", "fused_compute_gae_ring",
+    "KVCache", "KVPlan", "kv_plan", "kv_release", "kv_append", "kv_read", "kv_attention",
+    "TokenLogprobs", "token_logprobs", "token_logprobs_grad", "token_logp",
     "FMT_INT4", "FMT_INT8", "PATH_AUTO", "PATH_GEMV", "PATH_GEMM",
 ]
 
@@ -718,6 +720,291 @@ def ppo_rollout_forward(states, actions, w_proj, w_policy, w_value=None, ctx=Non
         values = mx_linear(latent, w_value, ctx)[:, 0]
     lp, alp, ent = policy_head(logits, actions, ctx)
     return lp, alp, ent, values
+
+
+# ------------------------------------------------------------------ serving ---
+_DTYPES = {torch.float32: DT_F32, torch.bfloat16: DT_BF16, torch.float16: DT_F16}
+KV_BLOCK = _lib.KV_BLOCK
+
+
+def _row_dtype(t, name):
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise ValueError("%s must be a CUDA tensor" % name)
+    if t.dtype not in _DTYPES:
+        raise ValueError("%s must be float32, bfloat16 or float16, got %s" % (name, t.dtype))
+    return _DTYPES[t.dtype]
+
+
+def _row_stride(t, name):
+    """Elements from one row to the next; the dimensions of a row lie side by side."""
+    inner = 1
+    for n, s in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
+        if n != 1 and s != inner:
+            raise ValueError("%s: only rows may have a stride, got %s" % (name, tuple(t.stride())))
+        inner *= n
+    return t.stride(0) if t.shape[0] > 1 else max(inner, t.stride(0))
+
+
+def _same_device(first, *others):
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise ValueError("tensors lie on %s and %s" % (first.device, t.device))
+    return first.device.index
+
+
+class _KVCacheC(ctypes.Structure):
+    """mxq_kv_cache (include/mxq.h)."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
+                ("v_scale", ctypes.c_void_p), ("n_pages", ctypes.c_int), ("page_size", ctypes.c_int),
+                ("n_kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int)]
+
+
+class KVCache:
+    """A paged 8-bit K/V cache (mxq_kv_cache): int8 values, one E8M0 scale for
+    each block of 32 tokens and head.  The four tensors are the caller's:
+    k int8 [n_pages][H][page/32][32][D], v int8 [n_pages][H][page/32][D/2][4][2][8],
+    k_scale and v_scale uint8 [n_pages][H][page/32]."""
+
+    def __init__(self, k, v, k_scale, v_scale):
+        _need_cuda(k, torch.int8, "k")
+        _need_cuda(v, torch.int8, "v")
+        _need_cuda(k_scale, torch.uint8, "k_scale")
+        _need_cuda(v_scale, torch.uint8, "v_scale")
+        if k.dim() != 5 or k.shape[3] != KV_BLOCK:
+            raise ValueError("k must be [n_pages][heads][blocks][32][head_dim], got %s" % (tuple(k.shape),))
+        n, h, nb, _, d = k.shape
+        if tuple(v.shape) != (n, h, nb, d // 2, 4, 2, 8):
+            raise ValueError("v must be [n_pages][heads][blocks][head_dim / 2][4][2][8], got %s" % (tuple(v.shape),))
+        if tuple(k_scale.shape) != (n, h, nb) or tuple(v_scale.shape) != (n, h, nb):
+            raise ValueError("k_scale and v_scale must be [n_pages][heads][blocks]")
+        self.device = _same_device(k, v, k_scale, v_scale)
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = n, h, nb * KV_BLOCK, d
+        self._c = _KVCacheC(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n, self.page_size, h, d)
+
+    @classmethod
+    def empty(cls, n_pages, page_size, n_kv_heads, head_dim, device="cuda"):
+        """A cache of n_pages pages; every block is written before it is read."""
+        if page_size <= 0 or page_size % KV_BLOCK:
+            raise ValueError("the page size is a multiple of 32, got %d" % page_size)
+        nb = page_size // KV_BLOCK
+        return cls(torch.zeros((n_pages, n_kv_heads, nb, KV_BLOCK, head_dim), dtype=torch.int8, device=device),
+                   torch.zeros((n_pages, n_kv_heads, nb, head_dim // 2, 4, 2, 8), dtype=torch.int8, device=device),
+                   torch.zeros((n_pages, n_kv_heads, nb), dtype=torch.uint8, device=device),
+                   torch.zeros((n_pages, n_kv_heads, nb), dtype=torch.uint8, device=device))
+
+
+@dataclass
+class KVPlan:
+    """One step's maps (mxq_kv_plan), all int32 on the device: ctx_len [R],
+    cu [R + 1], slots / positions / requests [n_tokens], free_count [1] and
+    short [1]."""
+    ctx_len: torch.Tensor
+    cu: torch.Tensor
+    slots: torch.Tensor
+    positions: torch.Tensor
+    requests: torch.Tensor
+    free_count: torch.Tensor
+    short: torch.Tensor
+
+
+def _table(table, rows):
+    _need_cuda(table, torch.int32, "table")
+    if table.dim() != 2 or table.shape[0] != rows:
+        raise ValueError("table must be [n_requests][max_pages], got %s" % (tuple(table.shape),))
+
+
+def kv_plan(past, new, page_size, table, free_pages, free_count, n_tokens, in_place=False, ctx=None):
+    """Block tables and slot maps of one step from the requests' lengths
+    (mxq_kv_plan): past and new int32 [R]; table int32 [R][max_pages] gets the
+    pages taken from the stack free_pages[:free_count]; n_tokens rows of maps
+    are written (the sum of new, or more: the rest are -1).  With in_place,
+    `past` becomes ctx_len and free_count is lowered.  Returns a KVPlan."""
+    for name, t in (("past", past), ("new", new), ("free_pages", free_pages), ("free_count", free_count)):
+        _need_cuda(t, torch.int32, name)
+    r = past.numel()
+    if new.numel() != r or free_count.numel() != 1:
+        raise ValueError("kv_plan: past and new must hold one length a request, free_count one number")
+    _table(table, r)
+    ctx = ctx or context(_same_device(past, new, table, free_pages, free_count))
+    n = int(n_tokens)
+    if n < 0:
+        raise ValueError("kv_plan: n_tokens is negative")
+    # one allocation for the maps and the two numbers
+    buf = torch.empty(3 * n + r + 1 + (2 if not in_place else 1) + (0 if in_place else r), dtype=torch.int32,
+                      device=past.device)
+    slots, pos, req = buf[:n], buf[n:2 * n], buf[2 * n:3 * n]
+    cu = buf[3 * n:3 * n + r + 1]
+    rest = buf[3 * n + r + 1:]
+    short, free_out = rest[:1], free_count if in_place else rest[1:2]
+    ctx_len = past if in_place else rest[2:]
+    ctx._bind()
+    check(ctx.lib.mxq_kv_plan(ctx.h, _ptr(past), _ptr(new), r, page_size, _ptr(table), table.shape[1], _ptr(free_pages),
+                              free_pages.numel(), _ptr(free_count), _ptr(ctx_len), _ptr(cu), _ptr(slots), _ptr(pos),
+                              _ptr(req), n, _ptr(free_out), _ptr(short)), ctx.h)
+    return KVPlan(ctx_len, cu, slots, pos, req, free_out, short)
+
+
+def kv_release(done, lengths, page_size, table, free_pages, free_count, ctx=None):
+    """Give the pages of ended requests back (mxq_kv_release): done uint8 or
+    bool [R]; lengths, table, free_pages and free_count are updated."""
+    if isinstance(done, torch.Tensor) and done.dtype == torch.bool:
+        done = done.view(torch.uint8)
+    _need_cuda(done, torch.uint8, "done")
+    for name, t in (("lengths", lengths), ("free_pages", free_pages), ("free_count", free_count)):
+        _need_cuda(t, torch.int32, name)
+    r = lengths.numel()
+    if done.numel() != r or free_count.numel() != 1:
+        raise ValueError("kv_release: done and lengths must hold one value a request, free_count one number")
+    _table(table, r)
+    ctx = ctx or context(_same_device(lengths, done, table, free_pages, free_count))
+    ctx._bind()
+    check(ctx.lib.mxq_kv_release(ctx.h, _ptr(done), _ptr(lengths), r, page_size, _ptr(table), table.shape[1],
+                                 _ptr(free_pages), free_pages.numel(), _ptr(free_count)), ctx.h)
+
+
+def kv_append(cache, k, v, slots, ctx=None):
+    """Quantise new K/V rows into the cache (mxq_kv_append): k, v [N][H][D]
+    (float32, bfloat16 or float16; rows may have a stride, as slices of fused
+    QKV rows do), slots int32 [N] (-1: not stored)."""
+    dt = _row_dtype(k, "k")
+    _need_cuda(slots, torch.int32, "slots")
+    if not isinstance(v, torch.Tensor) or v.dtype != k.dtype or v.shape != k.shape:
+        raise ValueError("kv_append: k and v must have one type and shape")
+    if k.dim() != 3 or tuple(k.shape[1:]) != (cache.n_kv_heads, cache.head_dim) or slots.numel() != k.shape[0]:
+        raise ValueError("kv_append: k and v must be [n][%d][%d] with one slot a row" % (cache.n_kv_heads, cache.head_dim))
+    stride = _row_stride(k, "k")
+    if _row_stride(v, "v") != stride:
+        raise ValueError("kv_append: k and v must have the same row stride")
+    ctx = ctx or context(_same_device(cache.k, k, v, slots))
+    ctx._bind()
+    check(ctx.lib.mxq_kv_append(ctx.h, ctypes.byref(cache._c), dt, _ptr(k), _ptr(v), stride, _ptr(slots), k.shape[0]),
+          ctx.h)
+
+
+def kv_read(cache, slots, dtype=torch.float32, ctx=None):
+    """Cached tokens as values (mxq_kv_read): (k, v) [N][H][D] of `dtype`."""
+    _need_cuda(slots, torch.int32, "slots")
+    if dtype not in _DTYPES:
+        raise ValueError("kv_read: float32, bfloat16 or float16, got %s" % dtype)
+    ctx = ctx or context(_same_device(cache.k, slots))
+    shape = (slots.numel(), cache.n_kv_heads, cache.head_dim)
+    k = torch.empty(shape, dtype=dtype, device=slots.device)
+    v = torch.empty(shape, dtype=dtype, device=slots.device)
+    ctx._bind()
+    check(ctx.lib.mxq_kv_read(ctx.h, ctypes.byref(cache._c), _ptr(slots), slots.numel(), _DTYPES[dtype], _ptr(k), _ptr(v)),
+          ctx.h)
+    return k, v
+
+
+def kv_attention(q, cache, table, ctx_len, cu, scale=None, max_new=None, want_lse=True, ctx=None):
+    """Causal attention of the new rows over the cache (mxq_kv_attention): q
+    [N][Hq][D] (float32, bfloat16 or float16; rows may have a stride); request
+    r's rows are cu[r] .. cu[r + 1] - 1, the last of its ctx_len[r] tokens.
+    scale defaults to 1 / sqrt(D); max_new bounds the new rows of a request.
+    Returns (out [N][Hq][D] of q's type, lse fp32 [N][Hq] or None)."""
+    dt = _row_dtype(q, "q")
+    _need_cuda(ctx_len, torch.int32, "ctx_len")
+    _need_cuda(cu, torch.int32, "cu")
+    r = ctx_len.numel()
+    _table(table, r)
+    if q.dim() != 3 or q.shape[2] != cache.head_dim or q.shape[1] % cache.n_kv_heads:
+        raise ValueError("kv_attention: q must be [n][heads][%d] with heads a multiple of %d, got %s"
+                         % (cache.head_dim, cache.n_kv_heads, tuple(q.shape)))
+    if cu.numel() != r + 1:
+        raise ValueError("kv_attention: cu must hold n_requests + 1 offsets")
+    n, hq, d = q.shape
+    if max_new is not None and max_new < 1:
+        raise ValueError("kv_attention: max_new must be positive")
+    ctx = ctx or context(_same_device(cache.k, q, table, ctx_len, cu))
+    out = torch.empty((n, hq, d), dtype=q.dtype, device=q.device)
+    lse = torch.empty((n, hq), dtype=torch.float32, device=q.device) if want_lse else None
+    ctx._bind()
+    check(ctx.lib.mxq_kv_attention(ctx.h, ctypes.byref(cache._c), dt, _ptr(q), _row_stride(q, "q"), n, hq, _ptr(table),
+                                   table.shape[1], _ptr(ctx_len), _ptr(cu), r, max(1, n if max_new is None else max_new),
+                                   float(d ** -0.5 if scale is None else scale), _ptr(out), _ptr(lse)), ctx.h)
+    return out, lse
+
+
+@dataclass
+class TokenLogprobs:
+    """mxq_token_logprobs's results, fp32 [N] (top_logp [N][top_k], top_ids
+    int32 [N][top_k]; None without alternatives)."""
+    logp: torch.Tensor
+    entropy: torch.Tensor
+    lse: torch.Tensor
+    top_logp: torch.Tensor = None
+    top_ids: torch.Tensor = None
+
+
+def _logits_rows(logits, targets):
+    dt = _row_dtype(logits, "logits")
+    _need_cuda(targets, torch.int32, "targets")
+    if logits.dim() != 2 or targets.numel() != logits.shape[0]:
+        raise ValueError("logits must be [rows][vocab] with one target a row")
+    return dt, _row_stride(logits, "logits")
+
+
+def token_logprobs(logits, targets, top_k=0, ctx=None):
+    """Log probabilities of given tokens with entropy and the top_k largest
+    alternatives (mxq_token_logprobs): logits [N][V] (float32, bfloat16 or
+    float16; rows may have a stride), targets int32 [N] (outside [0, V): 0).
+    Returns a TokenLogprobs; no autograd (see token_logp)."""
+    dt, stride = _logits_rows(logits, targets)
+    n, v = logits.shape
+    if not 0 <= top_k <= min(v, _lib.TOPK_MAX):
+        raise ValueError("token_logprobs: top_k (%d) must be in [0, min(32, vocab=%d)]" % (top_k, v))
+    ctx = ctx or context(_same_device(logits, targets))
+    res = torch.empty((3, n), dtype=torch.float32, device=logits.device)
+    top = torch.empty((n, top_k), dtype=torch.float32, device=logits.device) if top_k else None
+    ids = torch.empty((n, top_k), dtype=torch.int32, device=logits.device) if top_k else None
+    ctx._bind()
+    check(ctx.lib.mxq_token_logprobs(ctx.h, dt, _ptr(logits), stride, n, v, _ptr(targets), top_k, _ptr(res[0]),
+                                     _ptr(res[1]), _ptr(res[2]), _ptr(top), _ptr(ids)), ctx.h)
+    return TokenLogprobs(res[0], res[1], res[2], top, ids)
+
+
+def token_logprobs_grad(logits, targets, lse, entropy, dlogp=None, dentropy=None, out=None, ctx=None):
+    """The gradient of token_logprobs's logp and entropy to the logits
+    (mxq_token_logprobs_grad), of the logits' type; out may be logits."""
+    dt, stride = _logits_rows(logits, targets)
+    n, v = logits.shape
+    for name, t in (("lse", lse), ("entropy", entropy), ("dlogp", dlogp), ("dentropy", dentropy)):
+        if t is not None:
+            _need_cuda(t, torch.float32, name)
+            if t.numel() != n:
+                raise ValueError("token_logprobs_grad: %s must hold one value a row" % name)
+    if lse is None or (dentropy is not None and entropy is None):
+        raise ValueError("token_logprobs_grad: lse is needed, and entropy for dentropy")
+    if out is None:
+        out = torch.empty((n, v), dtype=logits.dtype, device=logits.device)
+    elif out.dtype != logits.dtype or out.shape != logits.shape:
+        raise ValueError("token_logprobs_grad: out must have the logits' type and shape")
+    ctx = ctx or context(_same_device(logits, targets, lse, entropy, dlogp, dentropy, out))
+    ctx._bind()
+    check(ctx.lib.mxq_token_logprobs_grad(ctx.h, dt, _ptr(logits), stride, n, v, _ptr(targets), _ptr(lse), _ptr(entropy),
+                                          _ptr(dlogp), _ptr(dentropy), _ptr(out), _row_stride(out, "out")), ctx.h)
+    return out
+
+
+class _TokenLogp(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, targets):
+        r = token_logprobs(logits, targets)
+        ctx.save_for_backward(logits, targets, r.lse, r.entropy)
+        return r.logp, r.entropy
+
+    @staticmethod
+    def backward(ctx, dlogp, dentropy):
+        logits, targets, lse, entropy = ctx.saved_tensors
+        flat = lambda g: None if g is None else g.contiguous()
+        return token_logprobs_grad(logits, targets, lse, entropy, flat(dlogp), flat(dentropy)), None
+
+
+def token_logp(logits, targets):
+    """(logp [N], entropy [N]) of given tokens, differentiable in the logits
+    (the policy-gradient and entropy terms of a rollout update)."""
+    return _TokenLogp.apply(logits, targets)
 
 
 # ------------------------------------------------------------------ decoder ---

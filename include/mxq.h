@@ -569,6 +569,142 @@ MXQ_API int mxq_decoder_set_trace(mxq_decoder dec, int layer);
 MXQ_API int mxq_decoder_get_trace(mxq_decoder dec, int id, float* out,
                                   size_t count);
 
+/* ------------------------------------------------------------ serving --- */
+/* Requests of different lengths served (or rolled out) together: block
+ * tables and slot maps built on the device, a paged K/V cache in 8 bits,
+ * attention over it, and the log probabilities of the chosen tokens.  No
+ * counterpart in the reference, whose sequences share one position; the
+ * cache's values are the MX activations of mx_quantize_x
+ * (nn/core/layers/ssm.cpp:164-177) with the block laid over 32 tokens of a
+ * head instead of 32 features of a token.
+ *
+ * Row types of the tensors below. */
+#define MXQ_DT_F32 0
+#define MXQ_DT_BF16 1
+#define MXQ_DT_F16 2
+
+#define MXQ_KV_BLOCK 32         /* tokens that share a scale */
+#define MXQ_KV_MAX_REQUESTS 8192
+#define MXQ_TOPK_MAX 32
+
+/* A paged K/V cache in caller-owned device memory.  Token slot s of the pool
+ * lives in page s / page_size; a block is 32 consecutive slots of a page, and
+ * every (block, head) of K and of V has one E8M0 scale:
+ *   k        int8 [n_pages][n_kv_heads][page_size / 32][32][head_dim]
+ *   v        int8 [n_pages][n_kv_heads][page_size / 32][head_dim / 2][4][2][8]
+ *            (token 8 j + 2 c + b of the block, dimension d, at
+ *             [d / 2][c][d % 2][2 j + b]: eight tokens of a dimension side by
+ *             side, the order in which the P.V product takes them)
+ *   k_scale, v_scale  u8 [n_pages][n_kv_heads][page_size / 32]
+ * value = q * 2^(scale - 127), scale 255 = NaN.  page_size is a multiple of
+ * 32 (at most 1024), head_dim 64 or 128, n_pages * page_size < 2^31.  k and v
+ * are 16-byte aligned. */
+typedef struct mxq_kv_cache {
+  void* k;
+  void* v;
+  uint8_t* k_scale;
+  uint8_t* v_scale;
+  int n_pages, page_size, n_kv_heads, head_dim;
+} mxq_kv_cache;
+
+/* One step's block tables and slot maps from the requests' lengths (device
+ * pointers, one launch).  Request r has past[r] cached tokens and add[r] new
+ * ones (a negative length counts as 0); table [n_req][max_pages] holds the
+ * pages of its past.  Pages for the new tokens are taken from the top of the
+ * stack free_pages[0 .. *free_count) (capacity n_pages), in request order,
+ * and written into table; then
+ *   ctx_len[r] = past[r] + add[r]
+ *   cu[0 .. n_req]   prefix sums of add: request r's new rows are
+ *                    cu[r] .. cu[r + 1] - 1
+ *   for new row i < n_tokens: request[i], position[i] (from 0), slot[i] =
+ *                    page * page_size + offset; all -1 for rows past cu[n_req]
+ *   *free_out        the pages left on the stack
+ *   *short_out       pages that were wanted but not there (the stack ran
+ *                    out or the table is too narrow; 0 when all were):
+ *                    the slots of their rows, and the entries of the table
+ *                    that it has for them, are -1
+ * ctx_len may be past and free_out may be free_count (in place).  n_req <=
+ * MXQ_KV_MAX_REQUESTS; lengths and their sums fit int32. */
+MXQ_API int mxq_kv_plan(mxq_ctx ctx, const int32_t* past, const int32_t* add,
+                        size_t n_req, size_t page_size, int32_t* table,
+                        size_t max_pages, const int32_t* free_pages,
+                        size_t n_pages, const int32_t* free_count,
+                        int32_t* ctx_len, int32_t* cu, int32_t* slot,
+                        int32_t* position, int32_t* request, size_t n_tokens,
+                        int32_t* free_out, int32_t* short_out);
+/* Requests that ended: for every r with done[r] != 0, the pages of its len[r]
+ * tokens go back on the stack (in request and page order), their table
+ * entries become -1 and len[r] 0. */
+MXQ_API int mxq_kv_release(mxq_ctx ctx, const uint8_t* done, int32_t* len,
+                           size_t n_req, size_t page_size, int32_t* table,
+                           size_t max_pages, int32_t* free_pages,
+                           size_t n_pages, int32_t* free_count);
+
+/* New rows into the cache: k, v [n][n_kv_heads][head_dim] of type dtype, row
+ * i starting at i * row_stride elements (16-byte aligned rows; a slice of the
+ * fused QKV rows will do), into slots slot[i] (outside the pool: skipped).
+ * Consecutive rows of one block form a run, rows of a block must be
+ * consecutive; o = the run's first offset in the block.  o = 0 starts the
+ * block: its exponent is the run's (smallest e with max|x| <= 127 * 2^e over
+ * the run's rows of the head, as in mxq_quantize_x; NaN or inf: scale 255 and
+ * zeros), the rest of the block is unspecified.  o > 0 extends it: the
+ * exponent is the larger of the block's and the run's, and where it grew the
+ * values already there are re-rounded, half to even (255 stays 255). */
+MXQ_API int mxq_kv_append(mxq_ctx ctx, const mxq_kv_cache* cache, int dtype,
+                          const void* k, const void* v, size_t row_stride,
+                          const int32_t* slot, size_t n);
+/* Cached tokens back as values: k_out, v_out [n][n_kv_heads][head_dim] of type
+ * dtype (exact in fp32 and bf16; a slot outside the pool gives zeros). */
+MXQ_API int mxq_kv_read(mxq_ctx ctx, const mxq_kv_cache* cache,
+                        const int32_t* slot, size_t n, int dtype, void* k_out,
+                        void* v_out);
+
+/* Causal attention of the new rows over the cache.  Rows cu[r] .. cu[r+1]-1 of
+ * q [n][n_heads][head_dim] (row stride q_stride elements, 16-byte aligned) are
+ * the last tokens of request r's ctx_len[r]: row t sees the keys at
+ * positions <= ctx_len[r] - (cu[r+1] - cu[r]) + t.  Head h reads K/V head
+ * h / (n_heads / n_kv_heads).  out [n][n_heads][head_dim] of q's type =
+ * softmax(scale * q k^T) v; lse [n][n_heads] fp32 (may be null) the natural
+ * logarithm of the softmax's denominator.  A row that sees no key, or that
+ * belongs to no request (rows from cu[n_req] on), gets 0 and -inf.  Pages
+ * outside the pool hold no keys.  max_new >= every request's number of new rows (more is safe; it only
+ * chooses the kernel).  The call works in a workspace that the context
+ * keeps for each stream (made by the first call there, which therefore must
+ * not be one that is being captured). */
+MXQ_API int mxq_kv_attention(mxq_ctx ctx, const mxq_kv_cache* cache, int dtype,
+                             const void* q, size_t q_stride, size_t n,
+                             size_t n_heads, const int32_t* table,
+                             size_t max_pages, const int32_t* ctx_len,
+                             const int32_t* cu, size_t n_req, size_t max_new,
+                             float scale, void* out, float* lse);
+
+/* Log probabilities of given tokens: logits [rows][vocab] of type dtype, row
+ * stride row_stride elements; per row, in fp32,
+ *   lse = log sum_j exp(x_j), logp = x_target - lse,
+ *   entropy = -sum_j p_j log p_j,
+ *   the top_k (0 .. MXQ_TOPK_MAX, <= vocab) largest logits: their ids
+ *   (descending, ties to the lower id, NaN first) and log probabilities.
+ * A target outside [0, vocab) gives logp 0; a banned token is a logit of -inf;
+ * a row with nothing but -inf gives lse, logp and top_logp -inf, entropy 0.
+ * logp, entropy, lse may be null. */
+MXQ_API int mxq_token_logprobs(mxq_ctx ctx, int dtype, const void* logits,
+                               size_t row_stride, size_t rows, size_t vocab,
+                               const int32_t* target, size_t top_k,
+                               float* logp, float* entropy, float* lse,
+                               float* top_logp, int32_t* top_ids);
+/* Its gradient: dlogits [rows][vocab] (dlogits' row stride grad_stride) =
+ *   dlogp (1[j = target] - p_j) - dentropy p_j (log p_j + entropy)
+ * from the forward pass's lse and entropy; dlogp or dentropy may be null (0),
+ * entropy too where dentropy is.  Rows whose lse is below -1e30 (every token
+ * banned, by -inf or by the lowest value of fp32 or bf16) get 0.  dlogits may
+ * be logits itself. */
+MXQ_API int mxq_token_logprobs_grad(mxq_ctx ctx, int dtype, const void* logits,
+                                    size_t row_stride, size_t rows,
+                                    size_t vocab, const int32_t* target,
+                                    const float* lse, const float* entropy,
+                                    const float* dlogp, const float* dentropy,
+                                    void* dlogits, size_t grad_stride);
+
 /* The MX bytes of a dense weight back in the MXINT8Tensor layout: data int8
  * [N][K] or packed int4 [N][K/2], scales [N][K/32] (host memory).  The
  * inverse of mxq_weight_create (for serialisation and checking). */
