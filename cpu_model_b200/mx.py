@@ -44,6 +44,15 @@ def _need_cuda(t, dtype, name):
         raise ValueError("%s must be contiguous" % name)
 
 
+def _current_stream(device):
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+# the current stream's handle without a Stream object in between (several
+# microseconds of a call that takes the GPU three), where this torch has it
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _current_stream)
+
+
 class MXContext:
     """One library context per device; work goes to torch's current stream."""
 
@@ -55,8 +64,9 @@ class MXContext:
         self.h = h
 
     def _bind(self):
-        s = torch.cuda.current_stream(self.device).cuda_stream
-        check(self.lib.mxq_set_stream(self.h, ctypes.c_void_p(s)), self.h)
+        rc = self.lib.mxq_set_stream(self.h, _raw_stream(self.device))
+        if rc:
+            check(rc, self.h)
 
     def set_path(self, path):
         check(self.lib.mxq_set_path(self.h, path), self.h)
@@ -727,29 +737,55 @@ _DTYPES = {torch.float32: DT_F32, torch.bfloat16: DT_BF16, torch.float16: DT_F16
 KV_BLOCK = _lib.KV_BLOCK
 
 
+# These calls take the GPU a few microseconds, so the checks before them are
+# written to cost less: pointers go to the library as integers, and the words of a
+# refusal are put together only where there is one.
+def _want(t, dtype, name):
+    try:
+        if t.dtype is dtype and t.is_cuda and t.is_contiguous():
+            return
+    except AttributeError:
+        pass
+    _need_cuda(t, dtype, name)
+
+
 def _row_dtype(t, name):
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError("%s must be a CUDA tensor" % name)
-    if t.dtype not in _DTYPES:
+    dt = _DTYPES.get(t.dtype)
+    if dt is None:
         raise ValueError("%s must be float32, bfloat16 or float16, got %s" % (name, t.dtype))
-    return _DTYPES[t.dtype]
+    return dt
 
 
 def _row_stride(t, name):
     """Elements from one row to the next; the dimensions of a row lie side by side."""
+    shape, stride = t.shape, t.stride()
+    if t.is_contiguous():
+        inner = t.numel() // shape[0] if shape[0] else 1
+        return max(inner, stride[0])
     inner = 1
-    for n, s in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
+    for n, s in zip(reversed(shape[1:]), reversed(stride[1:])):
         if n != 1 and s != inner:
-            raise ValueError("%s: only rows may have a stride, got %s" % (name, tuple(t.stride())))
+            raise ValueError("%s: only rows may have a stride, got %s" % (name, stride))
         inner *= n
-    return t.stride(0) if t.shape[0] > 1 else max(inner, t.stride(0))
+    return stride[0] if shape[0] > 1 else max(inner, stride[0])
 
 
-def _same_device(first, *others):
+def _serve_ctx(ctx, first, *others):
+    """The context of the call, bound to the current stream."""
+    dev = first.get_device()
     for t in others:
-        if t is not None and t.device != first.device:
+        if t is not None and t.get_device() != dev:
             raise ValueError("tensors lie on %s and %s" % (first.device, t.device))
-    return first.device.index
+    if ctx is None:
+        ctx = _contexts.get(dev) or context(dev)
+    ctx._bind()
+    return ctx
+
+
+def _at(t):
+    return 0 if t is None else t.data_ptr()
 
 
 class _KVCacheC(ctypes.Structure):
@@ -766,18 +802,19 @@ class KVCache:
     k_scale and v_scale uint8 [n_pages][H][page/32]."""
 
     def __init__(self, k, v, k_scale, v_scale):
-        _need_cuda(k, torch.int8, "k")
-        _need_cuda(v, torch.int8, "v")
-        _need_cuda(k_scale, torch.uint8, "k_scale")
-        _need_cuda(v_scale, torch.uint8, "v_scale")
+        _want(k, torch.int8, "k")
+        _want(v, torch.int8, "v")
+        _want(k_scale, torch.uint8, "k_scale")
+        _want(v_scale, torch.uint8, "v_scale")
         if k.dim() != 5 or k.shape[3] != KV_BLOCK:
             raise ValueError("k must be [n_pages][heads][blocks][32][head_dim], got %s" % (tuple(k.shape),))
         n, h, nb, _, d = k.shape
-        if tuple(v.shape) != (n, h, nb, d // 2, 4, 2, 8):
+        if v.shape != (n, h, nb, d // 2, 4, 2, 8):
             raise ValueError("v must be [n_pages][heads][blocks][head_dim / 2][4][2][8], got %s" % (tuple(v.shape),))
-        if tuple(k_scale.shape) != (n, h, nb) or tuple(v_scale.shape) != (n, h, nb):
+        if k_scale.shape != (n, h, nb) or v_scale.shape != (n, h, nb):
             raise ValueError("k_scale and v_scale must be [n_pages][heads][blocks]")
-        self.device = _same_device(k, v, k_scale, v_scale)
+        if not k.get_device() == v.get_device() == k_scale.get_device() == v_scale.get_device():
+            raise ValueError("the cache's tensors lie on different devices")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = n, h, nb * KV_BLOCK, d
         self._c = _KVCacheC(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n, self.page_size, h, d)
@@ -809,7 +846,7 @@ class KVPlan:
 
 
 def _table(table, rows):
-    _need_cuda(table, torch.int32, "table")
+    _want(table, torch.int32, "table")
     if table.dim() != 2 or table.shape[0] != rows:
         raise ValueError("table must be [n_requests][max_pages], got %s" % (tuple(table.shape),))
 
@@ -820,28 +857,30 @@ def kv_plan(past, new, page_size, table, free_pages, free_count, n_tokens, in_pl
     pages taken from the stack free_pages[:free_count]; n_tokens rows of maps
     are written (the sum of new, or more: the rest are -1).  With in_place,
     `past` becomes ctx_len and free_count is lowered.  Returns a KVPlan."""
-    for name, t in (("past", past), ("new", new), ("free_pages", free_pages), ("free_count", free_count)):
-        _need_cuda(t, torch.int32, name)
+    _want(past, torch.int32, "past")
+    _want(new, torch.int32, "new")
+    _want(free_pages, torch.int32, "free_pages")
+    _want(free_count, torch.int32, "free_count")
     r = past.numel()
     if new.numel() != r or free_count.numel() != 1:
         raise ValueError("kv_plan: past and new must hold one length a request, free_count one number")
     _table(table, r)
-    ctx = ctx or context(_same_device(past, new, table, free_pages, free_count))
     n = int(n_tokens)
     if n < 0:
         raise ValueError("kv_plan: n_tokens is negative")
+    ctx = _serve_ctx(ctx, past, new, table, free_pages, free_count)
     # one allocation for the maps and the two numbers
-    buf = torch.empty(3 * n + r + 1 + (2 if not in_place else 1) + (0 if in_place else r), dtype=torch.int32,
-                      device=past.device)
-    slots, pos, req = buf[:n], buf[n:2 * n], buf[2 * n:3 * n]
-    cu = buf[3 * n:3 * n + r + 1]
-    rest = buf[3 * n + r + 1:]
-    short, free_out = rest[:1], free_count if in_place else rest[1:2]
-    ctx_len = past if in_place else rest[2:]
-    ctx._bind()
-    check(ctx.lib.mxq_kv_plan(ctx.h, _ptr(past), _ptr(new), r, page_size, _ptr(table), table.shape[1], _ptr(free_pages),
-                              free_pages.numel(), _ptr(free_count), _ptr(ctx_len), _ptr(cu), _ptr(slots), _ptr(pos),
-                              _ptr(req), n, _ptr(free_out), _ptr(short)), ctx.h)
+    sizes = [n, n, n, r + 1, 1] if in_place else [n, n, n, r + 1, 1, 1, r]
+    views = torch.empty(3 * n + r + 2 + (0 if in_place else 1 + r), dtype=torch.int32, device=past.device).split(sizes)
+    slots, pos, req, cu, short = views[:5]
+    free_out, ctx_len = (free_count, past) if in_place else views[5:]
+    cu_at = cu.data_ptr()
+    at = cu_at - 12 * n
+    rc = ctx.lib.mxq_kv_plan(ctx.h, past.data_ptr(), new.data_ptr(), r, page_size, table.data_ptr(), table.shape[1],
+                             free_pages.data_ptr(), free_pages.numel(), free_count.data_ptr(), ctx_len.data_ptr(), cu_at, at,
+                             at + 4 * n, at + 8 * n, n, free_out.data_ptr(), cu_at + 4 * (r + 1))
+    if rc:
+        check(rc, ctx.h)
     return KVPlan(ctx_len, cu, slots, pos, req, free_out, short)
 
 
@@ -850,17 +889,16 @@ def kv_release(done, lengths, page_size, table, free_pages, free_count, ctx=None
     bool [R]; lengths, table, free_pages and free_count are updated."""
     if isinstance(done, torch.Tensor) and done.dtype == torch.bool:
         done = done.view(torch.uint8)
-    _need_cuda(done, torch.uint8, "done")
+    _want(done, torch.uint8, "done")
     for name, t in (("lengths", lengths), ("free_pages", free_pages), ("free_count", free_count)):
-        _need_cuda(t, torch.int32, name)
+        _want(t, torch.int32, name)
     r = lengths.numel()
     if done.numel() != r or free_count.numel() != 1:
         raise ValueError("kv_release: done and lengths must hold one value a request, free_count one number")
     _table(table, r)
-    ctx = ctx or context(_same_device(lengths, done, table, free_pages, free_count))
-    ctx._bind()
-    check(ctx.lib.mxq_kv_release(ctx.h, _ptr(done), _ptr(lengths), r, page_size, _ptr(table), table.shape[1],
-                                 _ptr(free_pages), free_pages.numel(), _ptr(free_count)), ctx.h)
+    ctx = _serve_ctx(ctx, lengths, done, table, free_pages, free_count)
+    check(ctx.lib.mxq_kv_release(ctx.h, _at(done), _at(lengths), r, page_size, _at(table), table.shape[1],
+                                 _at(free_pages), free_pages.numel(), _at(free_count)), ctx.h)
 
 
 def kv_append(cache, k, v, slots, ctx=None):
@@ -868,32 +906,34 @@ def kv_append(cache, k, v, slots, ctx=None):
     (float32, bfloat16 or float16; rows may have a stride, as slices of fused
     QKV rows do), slots int32 [N] (-1: not stored)."""
     dt = _row_dtype(k, "k")
-    _need_cuda(slots, torch.int32, "slots")
+    _want(slots, torch.int32, "slots")
     if not isinstance(v, torch.Tensor) or v.dtype != k.dtype or v.shape != k.shape:
         raise ValueError("kv_append: k and v must have one type and shape")
-    if k.dim() != 3 or tuple(k.shape[1:]) != (cache.n_kv_heads, cache.head_dim) or slots.numel() != k.shape[0]:
+    n = slots.numel()
+    if k.shape != (n, cache.n_kv_heads, cache.head_dim):
         raise ValueError("kv_append: k and v must be [n][%d][%d] with one slot a row" % (cache.n_kv_heads, cache.head_dim))
     stride = _row_stride(k, "k")
     if _row_stride(v, "v") != stride:
         raise ValueError("kv_append: k and v must have the same row stride")
-    ctx = ctx or context(_same_device(cache.k, k, v, slots))
-    ctx._bind()
-    check(ctx.lib.mxq_kv_append(ctx.h, ctypes.byref(cache._c), dt, _ptr(k), _ptr(v), stride, _ptr(slots), k.shape[0]),
-          ctx.h)
+    ctx = _serve_ctx(ctx, cache.k, k, v, slots)
+    rc = ctx.lib.mxq_kv_append(ctx.h, ctypes.byref(cache._c), dt, k.data_ptr(), v.data_ptr(), stride, slots.data_ptr(), n)
+    if rc:
+        check(rc, ctx.h)
 
 
 def kv_read(cache, slots, dtype=torch.float32, ctx=None):
     """Cached tokens as values (mxq_kv_read): (k, v) [N][H][D] of `dtype`."""
-    _need_cuda(slots, torch.int32, "slots")
+    _want(slots, torch.int32, "slots")
     if dtype not in _DTYPES:
         raise ValueError("kv_read: float32, bfloat16 or float16, got %s" % dtype)
-    ctx = ctx or context(_same_device(cache.k, slots))
-    shape = (slots.numel(), cache.n_kv_heads, cache.head_dim)
+    ctx = _serve_ctx(ctx, cache.k, slots)
+    n = slots.numel()
+    shape = (n, cache.n_kv_heads, cache.head_dim)
     k = torch.empty(shape, dtype=dtype, device=slots.device)
     v = torch.empty(shape, dtype=dtype, device=slots.device)
-    ctx._bind()
-    check(ctx.lib.mxq_kv_read(ctx.h, ctypes.byref(cache._c), _ptr(slots), slots.numel(), _DTYPES[dtype], _ptr(k), _ptr(v)),
-          ctx.h)
+    rc = ctx.lib.mxq_kv_read(ctx.h, ctypes.byref(cache._c), slots.data_ptr(), n, _DTYPES[dtype], k.data_ptr(), v.data_ptr())
+    if rc:
+        check(rc, ctx.h)
     return k, v
 
 
@@ -904,8 +944,8 @@ def kv_attention(q, cache, table, ctx_len, cu, scale=None, max_new=None, want_ls
     scale defaults to 1 / sqrt(D); max_new bounds the new rows of a request.
     Returns (out [N][Hq][D] of q's type, lse fp32 [N][Hq] or None)."""
     dt = _row_dtype(q, "q")
-    _need_cuda(ctx_len, torch.int32, "ctx_len")
-    _need_cuda(cu, torch.int32, "cu")
+    _want(ctx_len, torch.int32, "ctx_len")
+    _want(cu, torch.int32, "cu")
     r = ctx_len.numel()
     _table(table, r)
     if q.dim() != 3 or q.shape[2] != cache.head_dim or q.shape[1] % cache.n_kv_heads:
@@ -916,13 +956,16 @@ def kv_attention(q, cache, table, ctx_len, cu, scale=None, max_new=None, want_ls
     n, hq, d = q.shape
     if max_new is not None and max_new < 1:
         raise ValueError("kv_attention: max_new must be positive")
-    ctx = ctx or context(_same_device(cache.k, q, table, ctx_len, cu))
-    out = torch.empty((n, hq, d), dtype=q.dtype, device=q.device)
-    lse = torch.empty((n, hq), dtype=torch.float32, device=q.device) if want_lse else None
-    ctx._bind()
-    check(ctx.lib.mxq_kv_attention(ctx.h, ctypes.byref(cache._c), dt, _ptr(q), _row_stride(q, "q"), n, hq, _ptr(table),
-                                   table.shape[1], _ptr(ctx_len), _ptr(cu), r, max(1, n if max_new is None else max_new),
-                                   float(d ** -0.5 if scale is None else scale), _ptr(out), _ptr(lse)), ctx.h)
+    ctx = _serve_ctx(ctx, cache.k, q, table, ctx_len, cu)
+    device = q.device
+    out = torch.empty((n, hq, d), dtype=q.dtype, device=device)
+    lse = torch.empty((n, hq), dtype=torch.float32, device=device) if want_lse else None
+    rc = ctx.lib.mxq_kv_attention(ctx.h, ctypes.byref(cache._c), dt, q.data_ptr(), _row_stride(q, "q"), n, hq,
+                                  table.data_ptr(), table.shape[1], ctx_len.data_ptr(), cu.data_ptr(), r,
+                                  max(1, n if max_new is None else max_new), d ** -0.5 if scale is None else scale,
+                                  out.data_ptr(), _at(lse))
+    if rc:
+        check(rc, ctx.h)
     return out, lse
 
 
@@ -939,7 +982,7 @@ class TokenLogprobs:
 
 def _logits_rows(logits, targets):
     dt = _row_dtype(logits, "logits")
-    _need_cuda(targets, torch.int32, "targets")
+    _want(targets, torch.int32, "targets")
     if logits.dim() != 2 or targets.numel() != logits.shape[0]:
         raise ValueError("logits must be [rows][vocab] with one target a row")
     return dt, _row_stride(logits, "logits")
@@ -954,14 +997,16 @@ def token_logprobs(logits, targets, top_k=0, ctx=None):
     n, v = logits.shape
     if not 0 <= top_k <= min(v, _lib.TOPK_MAX):
         raise ValueError("token_logprobs: top_k (%d) must be in [0, min(32, vocab=%d)]" % (top_k, v))
-    ctx = ctx or context(_same_device(logits, targets))
-    res = torch.empty((3, n), dtype=torch.float32, device=logits.device)
-    top = torch.empty((n, top_k), dtype=torch.float32, device=logits.device) if top_k else None
-    ids = torch.empty((n, top_k), dtype=torch.int32, device=logits.device) if top_k else None
-    ctx._bind()
-    check(ctx.lib.mxq_token_logprobs(ctx.h, dt, _ptr(logits), stride, n, v, _ptr(targets), top_k, _ptr(res[0]),
-                                     _ptr(res[1]), _ptr(res[2]), _ptr(top), _ptr(ids)), ctx.h)
-    return TokenLogprobs(res[0], res[1], res[2], top, ids)
+    ctx = _serve_ctx(ctx, logits, targets)
+    device = logits.device
+    logp, entropy, lse = torch.empty((3, n), dtype=torch.float32, device=device).unbind(0)
+    top = torch.empty((n, top_k), dtype=torch.float32, device=device) if top_k else None
+    ids = torch.empty((n, top_k), dtype=torch.int32, device=device) if top_k else None
+    rc = ctx.lib.mxq_token_logprobs(ctx.h, dt, logits.data_ptr(), stride, n, v, targets.data_ptr(), top_k, logp.data_ptr(),
+                                    entropy.data_ptr(), lse.data_ptr(), _at(top), _at(ids))
+    if rc:
+        check(rc, ctx.h)
+    return TokenLogprobs(logp, entropy, lse, top, ids)
 
 
 def token_logprobs_grad(logits, targets, lse, entropy, dlogp=None, dentropy=None, out=None, ctx=None):
@@ -971,7 +1016,7 @@ def token_logprobs_grad(logits, targets, lse, entropy, dlogp=None, dentropy=None
     n, v = logits.shape
     for name, t in (("lse", lse), ("entropy", entropy), ("dlogp", dlogp), ("dentropy", dentropy)):
         if t is not None:
-            _need_cuda(t, torch.float32, name)
+            _want(t, torch.float32, name)
             if t.numel() != n:
                 raise ValueError("token_logprobs_grad: %s must hold one value a row" % name)
     if lse is None or (dentropy is not None and entropy is None):
@@ -980,10 +1025,13 @@ def token_logprobs_grad(logits, targets, lse, entropy, dlogp=None, dentropy=None
         out = torch.empty((n, v), dtype=logits.dtype, device=logits.device)
     elif out.dtype != logits.dtype or out.shape != logits.shape:
         raise ValueError("token_logprobs_grad: out must have the logits' type and shape")
-    ctx = ctx or context(_same_device(logits, targets, lse, entropy, dlogp, dentropy, out))
-    ctx._bind()
-    check(ctx.lib.mxq_token_logprobs_grad(ctx.h, dt, _ptr(logits), stride, n, v, _ptr(targets), _ptr(lse), _ptr(entropy),
-                                          _ptr(dlogp), _ptr(dentropy), _ptr(out), _row_stride(out, "out")), ctx.h)
+    elif not out.is_cuda:
+        raise ValueError("token_logprobs_grad: out must be a CUDA tensor")
+    ctx = _serve_ctx(ctx, logits, targets, lse, entropy, dlogp, dentropy, out)
+    rc = ctx.lib.mxq_token_logprobs_grad(ctx.h, dt, logits.data_ptr(), stride, n, v, targets.data_ptr(), lse.data_ptr(),
+                                         _at(entropy), _at(dlogp), _at(dentropy), out.data_ptr(), _row_stride(out, "out"))
+    if rc:
+        check(rc, ctx.h)
     return out
 
 
