@@ -241,7 +241,7 @@ const WeightView* weight_view(mxq_weight w);
 // meet in it: counters that every kernel leaves zero, then bytes that hold
 // nothing from one call to the next.
 constexpr size_t kServeCounters = 2048;                  // uint32
-constexpr size_t kServeScratch = 16u << 20;              // bytes
+constexpr size_t kServeScratch = 24u << 20;              // bytes
 struct ServeWs {
   uint32_t* counters;
   uint8_t* scratch;

@@ -37,9 +37,9 @@ namespace mxq {
 
 namespace {
 
-constexpr int kWarps = 8;
-constexpr int kThreads = kWarps * 32;
+constexpr int kMaxWarps = 12;
 constexpr int kMaxRows = 16;             // query rows a unit
+constexpr int kStages = 2;               // blocks a warp has in its ring
 constexpr int kStart = 1;                // places a unit's start takes
 constexpr int kMinPiece = 2;             // places a piece at least
 constexpr float kLn2 = 0.693147180559945f;
@@ -54,7 +54,7 @@ struct AttnArgs {
   int dtype, R, n, Hq, G, max_pages;
   float scale2;                          // scale * log2(e)
   uint32_t* counters;                    // [CTAs], zero
-  float* warp_part;                      // [CTAs * kWarps][rows][D + 2]
+  float* warp_part;                      // [CTAs * warps][rows][D + 2]
   float* cta_part;                       // [CTAs][2][rows][D + 2]
 };
 
@@ -82,15 +82,6 @@ template <int N> __device__ __forceinline__ void cp_wait() {
 // Start of request r's rows (r = R: their end), inside q whatever is given.
 __device__ __forceinline__ int row_start(const AttnArgs& a, int r) { return min(max(a.cu[r], 0), a.n); }
 
-// A piece's share of a unit that other pieces share too.
-struct Part {
-  long unit0;                            // the unit's place in the line
-  float* at;                             // [rows][D], maxima [rows], sums [rows]
-  int row0, tile, head, nrows;           // rows: tile * kRows + 0 .. nrows - 1 of the request that starts at row0
-  int g_first, g_last;                   // the pieces that share it
-  int valid;
-};
-
 // Rows [0, nrows) of a tile: row i is query head head * G + (tile's row) % G of
 // token row0 + (tile's row) / G.
 template <int D>
@@ -104,6 +95,436 @@ __device__ __forceinline__ void write_row(const AttnArgs& a, int row0, int first
   if (a.lse && d == 0) a.lse[at] = l == 0.0f ? neg_inf() : m * kLn2 + logf(l);
 }
 
+// ------------------------------------------------------------------ tiles --
+// A tile is a warp's query rows of one unit: its digits, running maxima and sums,
+// and O.  start() takes the rows, keys() a block's K (leaving the
+// probabilities), values() its V, park() puts (O, maxima, sums) where another may
+// join them, write() the finished rows where they belong.
+
+// Digits of four fixed-point numbers, a byte of a word each; digit 0 is the uppermost.
+__device__ __forceinline__ void digits3(const float (&x)[4], float inv, bool finite, uint32_t (&dig)[3]) {
+  dig[0] = dig[1] = dig[2] = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    int q = finite ? __float2int_rn(x[e] * inv) : 0;
+#pragma unroll
+    for (int p = 2; p >= 0; --p) {
+      dig[p] |= (uint32_t)(q & 0xFF) << (8 * e);
+      q = (q + 128) >> 8;
+    }
+  }
+}
+
+// The step 2^ex of a row whose largest element has the bits `top`: |q| <=
+// 127 * 256^2; tiny rows keep a step that is a normal number.
+struct Step {
+  bool finite;
+  float inv, scale;                      // 2^-ex, 2^ex scale log2(e)
+  __device__ __forceinline__ Step(uint32_t top, float scale2) {
+    finite = top < 0x7f800000u;
+    const int ex = max(e8m0_exponent<127>(__uint_as_float(top)) - 16, -126);
+    inv = finite ? __int_as_float((127 - ex) << 23) : 0.0f;
+    scale = finite ? __int_as_float((ex + 127) << 23) * scale2 : __int_as_float(0x7fc00000);
+  }
+};
+
+// A block's maximum joined to a row's running one: what O and the sum are
+// to be multiplied with (alpha), the block's weight (beta), and what to
+// subtract from the block's scores.
+struct Rise {
+  float alpha, beta, base;
+  bool none;                             // no key of the block is seen
+  __device__ __forceinline__ Rise(float& mx, float bm) {
+    none = bm == neg_inf();
+    const float mn = fmaxf(mx, bm), ms = mn == neg_inf() ? 0.0f : mn;
+    beta = none ? 0.0f : ex2(bm - ms);
+    alpha = ex2(mx - ms);
+    base = none ? 0.0f : bm;
+    mx = mn;
+  }
+};
+
+template <int NP>
+struct Top {                             // what probability 1 is in fixed point, 127 * 256^(NP-1)
+  static constexpr float k = NP == 2 ? 32512.0f : 8323072.0f;
+};
+
+// Rows of a unit in the MMA's layout: 8 or 16 of them.
+template <int D_, int MT, int NP>
+struct MmaTile {
+  static constexpr int D = D_;
+  static constexpr int kRows = 8 * MT;
+  static constexpr int kWarps = MT == 1 ? 12 : 8;
+  static constexpr int kJ = D / 64;                       // 64-dimension halves
+  static constexpr int kU = D / 16;                       // V words of 16 dimensions
+  static constexpr int kTiles = MT == 1 ? 2 : 3;          // MMA row tiles of S: upper digits of 8 rows each, then the lowest
+  static constexpr int kTilesP = NP == 2 ? MT : kTiles;   // of O
+
+  uint32_t qa[MT][3][kJ][4];
+  float qs[MT];
+  int last[MT];
+  float o[MT][kU][4];
+  float mx[MT], sum[MT];
+  uint32_t pa[MT][NP][2];                // probabilities' digits, slots 0-3 and 4-7
+  float fac[MT];
+
+  // Place of a 16-byte piece of K / V in the ring: K rows of 128 bytes have
+  // every other row's halves exchanged, so that a quarter warp's two rows lie in
+  // different banks.
+  static __device__ __forceinline__ int k_place(int ch) { return D == 128 ? ch ^ ((ch >> 3 & 1) << 2) : ch; }
+  static __device__ __forceinline__ int v_place(int ch) { return ch; }
+
+  // A fragments: 64 dimensions are two k-steps; lane (r8, c4) has 16 values of
+  // row r8: words 0, 1 of step 0 and 2, 3 of step 1.
+  __device__ __forceinline__ void start(const AttnArgs& a, int row0, int tile, int head, int nrows, int past) {
+    const int lane = threadIdx.x & 31, c4 = lane & 3, r8 = lane >> 2;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const int row = m * 8 + r8, gr = tile * kRows + row, t = gr / a.G, h = head * a.G + (gr - t * a.G);
+      float x[kJ][4][4];
+      uint32_t top = 0;
+#pragma unroll
+      for (int j = 0; j < kJ; ++j)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[j][w][e] = 0.0f;
+          if (row < nrows)
+            load4_dt(a.dtype, a.q, (long)(row0 + t) * a.q_stride + (long)h * D + j * 64 + c4 * 16 + w * 4, x[j][w]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(x[j][w][e]) & 0x7fffffffu);
+        }
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const Step st(top, a.scale2);
+#pragma unroll
+      for (int j = 0; j < kJ; ++j)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          uint32_t dig[3];
+          digits3(x[j][w], st.inv, st.finite, dig);
+#pragma unroll
+          for (int p = 0; p < 3; ++p) qa[m][p][j][w] = dig[p];
+        }
+      qs[m] = st.scale;
+      last[m] = row < nrows ? past + t : -1;
+      mx[m] = neg_inf();
+      sum[m] = 0.0f;
+#pragma unroll
+      for (int u = 0; u < kU; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[m][u][e] = 0.0f;
+    }
+  }
+
+  __device__ __forceinline__ void keys(const uint8_t* k, int key0, float ks, float vs, uint8_t*) {
+    const int lane = threadIdx.x & 31, c4 = lane & 3, r8 = lane >> 2;
+    int acc[kTiles][4][4];
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[t][n][e] = 0;
+#pragma unroll
+    for (int j = 0; j < kJ; ++j)
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const int row = 8 * n + r8;
+        const int ch = D == 128 ? row * 8 + ((j * 4 + c4) ^ ((row & 1) << 2)) : row * 4 + c4;
+        const uint4 b = *reinterpret_cast<const uint4*>(k + ch * 16);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          mma_s8(acc[m][n], qa[m][0][j][0], qa[m][1][j][0], qa[m][0][j][1], qa[m][1][j][1], b.x, b.y);
+          mma_s8(acc[m][n], qa[m][0][j][2], qa[m][1][j][2], qa[m][0][j][3], qa[m][1][j][3], b.z, b.w);
+        }
+        mma_s8(acc[kTiles - 1][n], qa[0][2][j][0], MT == 2 ? qa[MT - 1][2][j][0] : 0u, qa[0][2][j][1],
+               MT == 2 ? qa[MT - 1][2][j][1] : 0u, b.x, b.y);
+        mma_s8(acc[kTiles - 1][n], qa[0][2][j][2], MT == 2 ? qa[MT - 1][2][j][2] : 0u, qa[0][2][j][3],
+               MT == 2 ? qa[MT - 1][2][j][3] : 0u, b.z, b.w);
+      }
+    float alpha[MT];
+    bool same = true;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      float x[8];
+      float bm = neg_inf();
+      const float f = qs[m] * ks;
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int hl = acc[m][n][e] * 256 + acc[m][n][2 + e];
+          const float s = fmaf((float)hl, 256.0f, (float)acc[kTiles - 1][n][2 * m + e]);
+          x[2 * n + e] = key0 + 2 * c4 + 8 * n + e <= last[m] ? s * f : neg_inf();
+          bm = fmaxf(bm, x[2 * n + e]);
+        }
+      bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, 1));
+      bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, 2));
+      const float was = mx[m];
+      const Rise r(mx[m], bm);
+      alpha[m] = r.alpha;
+      same = same && was == mx[m];
+      float ps = 0.0f;
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float p = ex2(x[4 * g + e] - r.base);
+          ps += p;
+          // the sum with 2^23 leaves the nearest integer in the low bits
+          w[e] = __float_as_uint(fmaf(p, Top<NP>::k, 8388608.0f));
+        }
+#pragma unroll
+        for (int p = NP - 1; p >= 0; --p) {
+          pa[m][p][g] = __byte_perm(__byte_perm(w[0], w[1], 0x0040), __byte_perm(w[2], w[3], 0x0040), 0x5410);
+          if (p) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = (w[e] + 128) >> 8;
+          }
+        }
+      }
+      sum[m] = sum[m] * r.alpha + ps * r.beta;
+      fac[m] = r.none ? 0.0f : r.beta * vs * (1.0f / Top<NP>::k);
+    }
+    if (!__all_sync(0xffffffffu, same)) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int u = 0; u < kU; ++u)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[m][u][e] *= alpha[m];
+    }
+  }
+
+  __device__ __forceinline__ void values(const uint8_t* v, const uint8_t*) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const uint4 b = *reinterpret_cast<const uint4*>(v + (u * 32 + lane) * 16);
+#pragma unroll
+      for (int d = 0; d < 2; ++d) {
+        const uint32_t b_lo = d ? b.z : b.x, b_hi = d ? b.w : b.y;
+        int pv[kTilesP][4];
+#pragma unroll
+        for (int t = 0; t < kTilesP; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) pv[t][e] = 0;
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+          mma_s8(pv[m], pa[m][0][0], pa[m][1][0], pa[m][0][1], pa[m][1][1], b_lo, b_hi);
+        if (NP == 3)
+          mma_s8(pv[kTilesP - 1], pa[0][NP - 1][0], MT == 2 ? pa[MT - 1][NP - 1][0] : 0u, pa[0][NP - 1][1],
+                 MT == 2 ? pa[MT - 1][NP - 1][1] : 0u, b_lo, b_hi);
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float s = (float)(pv[m][e] * 256 + pv[m][2 + e]);
+            if (NP == 3) s = fmaf(s, 256.0f, (float)pv[kTilesP - 1][2 * m + e]);
+            o[m][u][2 * e + d] = fmaf(s, fac[m], o[m][u][2 * e + d]);
+          }
+      }
+    }
+  }
+
+  __device__ __forceinline__ void finish() {
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      sum[m] += __shfl_xor_sync(0xffffffffu, sum[m], 1);
+      sum[m] += __shfl_xor_sync(0xffffffffu, sum[m], 2);
+    }
+  }
+  // lane (r8, c4) has dimensions 16 u + 4 c4 .. + 3 of its rows
+  __device__ __forceinline__ void write(const AttnArgs& a, int row0, int tile, int head, int nrows) const {
+    const int lane = threadIdx.x & 31, c4 = lane & 3, r8 = lane >> 2;
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+      if (m * 8 + r8 < nrows)
+#pragma unroll
+        for (int u = 0; u < kU; ++u)
+          write_row<D>(a, row0, tile * kRows, m * 8 + r8, head, u * 16 + c4 * 4, o[m][u], mx[m], sum[m]);
+  }
+  __device__ __forceinline__ void park(float* at, int nrows) const {
+    const int lane = threadIdx.x & 31, c4 = lane & 3, r8 = lane >> 2;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const int row = m * 8 + r8;
+      if (row >= nrows) continue;
+#pragma unroll
+      for (int u = 0; u < kU; ++u)
+        *reinterpret_cast<float4*>(at + row * D + u * 16 + c4 * 4) = make_float4(o[m][u][0], o[m][u][1], o[m][u][2], o[m][u][3]);
+      if (c4 == 0) {
+        at[kRows * D + row] = mx[m];
+        at[kRows * (D + 1) + row] = sum[m];
+      }
+    }
+  }
+};
+
+// One query row a unit (a token of a head of its own).  The MMA would leave
+// seven of its eight rows empty; dp4a takes the same digits with a lane for each
+// token (S, no sums across lanes) and a lane for every D / 32 dimensions (O): under half
+// the instructions.
+template <int D_, int NP>
+struct DotTile {
+  static constexpr int D = D_;
+  static constexpr int kRows = 1;
+  static constexpr int kWarps = 12;
+  static constexpr int kW = D / 4;                        // words of a K row
+  static constexpr int kPairs = D / 64;                   // dimension pairs a lane: lane, lane + 32
+
+  uint32_t q[3][kW];                     // the row's digits, the same in every lane
+  float qs;
+  int last;
+  float o[kPairs][2];
+  float mx, sum, fac;
+
+  // a quarter warp reads 8 rows, or 8 dimension pairs: their pieces are
+  // rotated so that they lie in different banks
+  static __device__ __forceinline__ int k_place(int ch) {
+    return D == 128 ? ch ^ (ch >> 3 & 7) : ch ^ (ch >> 3 & 3);
+  }
+  static __device__ __forceinline__ int v_place(int ch) { return ch ^ (ch >> 3 & 3); }
+
+  __device__ __forceinline__ void start(const AttnArgs& a, int row0, int tile, int head, int, int past) {
+    const int lane = threadIdx.x & 31;
+    const int t = tile / a.G, h = head * a.G + (tile - t * a.G);
+    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    uint32_t top = 0;
+    if (lane < D / 4) {
+      load4_dt(a.dtype, a.q, (long)(row0 + t) * a.q_stride + (long)h * D + lane * 4, x);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+    }
+    const Step st(__reduce_max_sync(0xffffffffu, top), a.scale2);
+    uint32_t dig[3];
+    digits3(x, st.inv, st.finite, dig);
+#pragma unroll
+    for (int p = 0; p < 3; ++p)
+#pragma unroll
+      for (int w = 0; w < kW; ++w) q[p][w] = __shfl_sync(0xffffffffu, dig[p], w);
+    qs = st.scale;
+    last = past + t;
+    mx = neg_inf();
+    sum = 0.0f;
+#pragma unroll
+    for (int u = 0; u < kPairs; ++u) o[u][0] = o[u][1] = 0.0f;
+  }
+
+  __device__ __forceinline__ void keys(const uint8_t* k, int key0, float ks, float vs, uint8_t* scratch) {
+    const int lane = threadIdx.x & 31;
+    int s[3] = {0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) {
+      const uint4 b = *reinterpret_cast<const uint4*>(k + k_place(lane * (D / 16) + j) * 16);
+      const uint32_t w[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int p = 0; p < 3; ++p) s[p] = __dp4a((int)w[e], (int)q[p][j * 4 + e], s[p]);
+    }
+    float x = fmaf((float)(s[0] * 256 + s[1]), 256.0f, (float)s[2]) * (qs * ks);
+    if (key0 + lane > last) x = neg_inf();
+    // the block's maximum as an integer with the floats' order
+    int key = __float_as_int(x);
+    key ^= (key >> 31) & 0x7fffffff;
+    key = __reduce_max_sync(0xffffffffu, key);
+    const Rise r(mx, __int_as_float(key ^ ((key >> 31) & 0x7fffffff)));
+    const float p = ex2(x - r.base);
+    sum = sum * r.alpha + p * r.beta;
+    fac = r.none ? 0.0f : r.beta * vs * (1.0f / Top<NP>::k);
+#pragma unroll
+    for (int u = 0; u < kPairs; ++u) {
+      o[u][0] *= r.alpha;
+      o[u][1] *= r.alpha;
+    }
+    // the token's digits where V's words have its byte: token 8 j + 2 c + b is byte 2 (j % 2) + b of word 2 c + j / 2
+    uint32_t v = __float_as_uint(fmaf(p, Top<NP>::k, 8388608.0f));
+    const int at = ((lane >> 1) & 3) * 8 + (lane >> 4) * 4 + ((lane >> 3) & 1) * 2 + (lane & 1);
+#pragma unroll
+    for (int d = NP - 1; d >= 0; --d) {
+      scratch[d * 32 + at] = (uint8_t)v;
+      v = (v + 128) >> 8;
+    }
+    __syncwarp();
+  }
+
+  __device__ __forceinline__ void values(const uint8_t* v, const uint8_t* scratch) {
+    const int lane = threadIdx.x & 31;
+    int s[kPairs][2][NP];
+#pragma unroll
+    for (int u = 0; u < kPairs; ++u)
+#pragma unroll
+      for (int d = 0; d < 2; ++d)
+#pragma unroll
+        for (int p = 0; p < NP; ++p) s[u][d][p] = 0;
+#pragma unroll
+    for (int c = 0; c < 4; c += 2) {
+      uint32_t pw[NP][4];                // words of eight-token groups c and c + 1
+#pragma unroll
+      for (int p = 0; p < NP; ++p) {
+        const uint4 w = *reinterpret_cast<const uint4*>(scratch + p * 32 + c * 8);
+        pw[p][0] = w.x; pw[p][1] = w.y; pw[p][2] = w.z; pw[p][3] = w.w;
+      }
+#pragma unroll
+      for (int u = 0; u < kPairs; ++u)
+#pragma unroll
+        for (int cc = 0; cc < 2; ++cc) {
+          const uint4 b = *reinterpret_cast<const uint4*>(v + v_place((lane + 32 * u) * 4 + c + cc) * 16);
+#pragma unroll
+          for (int p = 0; p < NP; ++p) {
+            s[u][0][p] = __dp4a((int)b.x, (int)pw[p][2 * cc], s[u][0][p]);
+            s[u][0][p] = __dp4a((int)b.y, (int)pw[p][2 * cc + 1], s[u][0][p]);
+            s[u][1][p] = __dp4a((int)b.z, (int)pw[p][2 * cc], s[u][1][p]);
+            s[u][1][p] = __dp4a((int)b.w, (int)pw[p][2 * cc + 1], s[u][1][p]);
+          }
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < kPairs; ++u)
+#pragma unroll
+      for (int d = 0; d < 2; ++d) {
+        float y = (float)(s[u][d][0] * 256 + s[u][d][1]);
+        if (NP == 3) y = fmaf(y, 256.0f, (float)s[u][d][NP - 1]);
+        o[u][d] = fmaf(y, fac, o[u][d]);
+      }
+  }
+
+  __device__ __forceinline__ void finish() {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  }
+  __device__ __forceinline__ void write(const AttnArgs& a, int row0, int tile, int head, int) const {
+    const int lane = threadIdx.x & 31;
+    const int t = tile / a.G, h = head * a.G + (tile - t * a.G);
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const long at = (long)(row0 + t) * a.Hq + h;
+#pragma unroll
+    for (int u = 0; u < kPairs; ++u) store2_dt(a.dtype, a.out, at * D + 64 * u + 2 * lane, o[u][0] * inv, o[u][1] * inv);
+    if (a.lse && lane == 0) a.lse[at] = sum == 0.0f ? neg_inf() : mx * kLn2 + logf(sum);
+  }
+  __device__ __forceinline__ void park(float* at, int) const {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int u = 0; u < kPairs; ++u) *reinterpret_cast<float2*>(at + 64 * u + 2 * lane) = make_float2(o[u][0], o[u][1]);
+    if (lane == 0) {
+      at[D] = mx;
+      at[D + 1] = sum;
+    }
+  }
+};
+
+// A piece's share of a unit that other pieces share too.
+struct Part {
+  long unit0;                            // the unit's place in the line
+  float* at;                             // [rows][D], maxima [rows], sums [rows]
+  int row0, tile, head, nrows;           // rows: tile * kRows + 0 .. nrows - 1 of the request that starts at row0
+  int g_first, g_last;                   // the pieces that share it
+  int valid;
+};
+
 // A running softmax (m, l, y) joined with another.
 __device__ __forceinline__ void join(float& m, float& l, float (&y)[4], float pm, float pl, const float4& v) {
   const float mn = fmaxf(m, pm), ms = mn == neg_inf() ? 0.0f : mn;
@@ -116,23 +537,19 @@ __device__ __forceinline__ void join(float& m, float& l, float (&y)[4], float pm
   m = mn;
 }
 
-template <int D, int MT, int NP, int ST>
-__global__ void __launch_bounds__(kThreads, 1) kv_attn_kernel(AttnArgs a) {
-  constexpr int kRows = 8 * MT;
-  constexpr int kPart = kRows * (D + 2);           // floats of a part
+template <typename Tile>
+__global__ void __launch_bounds__(Tile::kWarps * 32, 1) kv_attn_kernel(AttnArgs a) {
+  constexpr int D = Tile::D, kRows = Tile::kRows, kWarps = Tile::kWarps, kThreads = kWarps * 32;
+  constexpr int kPart = (kRows * (D + 2) + 3) / 4 * 4;   // floats of a part, whole 16-byte pieces
   constexpr int kStage = 64 * D;                   // one block's K and V
-  constexpr int kJ = D / 64;                       // 64-dimension halves
-  constexpr int kU = D / 16;                       // V words of 16 dimensions
-  constexpr int kTiles = MT == 1 ? 2 : 3;          // MMA row tiles of S: upper digits of 8 rows each, then the lowest
-  constexpr int kTilesP = NP == 2 ? MT : kTiles;   // of O
-  static_assert(kPart * 4 <= ST * kStage, "a part takes its warp's ring");
+  static_assert(kPart * 4 <= kStages * kStage, "a part takes its warp's ring");
   extern __shared__ __align__(16) uint8_t sm[];
-  long* s_sum = reinterpret_cast<long*>(sm + kWarps * ST * kStage);   // [R + 1]
+  uint8_t* scratch = sm + kWarps * kStages * kStage + (threadIdx.x >> 5) * 128;   // a tile's own
+  long* s_sum = reinterpret_cast<long*>(sm + kWarps * (kStages * kStage + 128));  // [R + 1]
   __shared__ long s_warp[kWarps];
   __shared__ Part s_part[kWarps * 2];
   __shared__ int s_flag;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int c4 = lane & 3, r8 = lane >> 2;
   const int Hkv = a.c.heads, G = a.G, nb = a.c.nb;
 
   // ---- the line of work: units * places of every request, summed
@@ -172,7 +589,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attn_kernel(AttnArgs a) {
   const int piece = blockIdx.x * kWarps + warp;
   const long lo = piece * len, hi = min(lo + len, total);
 
-  uint8_t* ring = sm + warp * (ST * kStage);
+  uint8_t* ring = sm + warp * (kStages * kStage);
   const uint32_t ring_s = smem_u32(ring);
 
   auto request_of = [&](long pos) {      // the request with work at a place of the line
@@ -212,35 +629,32 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attn_kernel(AttnArgs a) {
       }
     }
   };
-  auto fetch = [&](int i) {              // place i of this piece into its stage
+  const int mine = lo < hi ? (int)(hi - lo) : 0;
+  // place i of this piece into its stage: K and V are groups of their own, so
+  // that K's part is refilled while V's is still in use
+  auto fetch = [&](int i, bool is_v) {
     const long at = __shfl_sync(0xffffffffu, place, i & 31);
-    if (at >= 0) {
-      const uint32_t st = ring_s + (i % ST) * kStage;
-      const int8_t* k = a.c.k + at * (32 * D);
-      const int8_t* v = a.c.v + at * (32 * D);
+    if (i < mine && at >= 0) {
+      const uint32_t st = ring_s + (i % kStages) * kStage + (is_v ? 32 * D : 0);
+      const int8_t* src = (is_v ? a.c.v : a.c.k) + at * (32 * D);
 #pragma unroll
       for (int u = 0; u < 2 * D / 32; ++u) {
         const int ch = u * 32 + lane;
-        // rows of 128 bytes: every other row's halves change places, so that a
-        // quarter warp's two rows lie in different banks
-        const int sw = D == 128 ? ch ^ ((ch >> 3 & 1) << 2) : ch;
-        cp16(st + sw * 16, k + ch * 16);
-        cp16(st + 32 * D + ch * 16, v + ch * 16);
+        cp16(st + (is_v ? Tile::v_place(ch) : Tile::k_place(ch)) * 16, src + ch * 16);
       }
     }
     cp_commit();
   };
   long pl_now = -1;                      // the 32 places that hold the current one
   uint32_t sc_now = 0;
-  const int mine = lo < hi ? (int)(hi - lo) : 0;
   if (mine) {
     look_up(lo);
     pl_now = place;
     sc_now = place_sc;
 #pragma unroll
-    for (int i = 0; i < ST - 1; ++i) {
-      if (i < mine) fetch(i);
-      else cp_commit();
+    for (int i = 0; i < kStages; ++i) {
+      fetch(i, false);
+      fetch(i, true);
     }
   }
 
@@ -263,214 +677,36 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attn_kernel(AttnArgs a) {
     const bool has = blocks ? skip < kStart + blocks && skip + (end - i) > kStart
                             : skip <= kStart && skip + (end - i) > kStart;   // a unit without keys: whoever has its first place
 
-    // ---- A fragments of the query's digits: 64 dimensions are two k-steps;
-    // lane (r8, c4) has 16 values of row r8: words 0, 1 of step 0 and 2, 3 of step 1
-    uint32_t qa[MT][3][kJ][4];
-    float qs[MT];
-    int last[MT];
-    float o[MT][kU][4];
-    float mx[MT], sum[MT];
-    if (has) {
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        const int row = m * 8 + r8, gr = tile * kRows + row, t = gr / G, h = head * G + (gr - t * G);
-        float x[kJ][16];
-        uint32_t top = 0;
-#pragma unroll
-        for (int j = 0; j < kJ; ++j)
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (row < nrows)
-              load4_dt(a.dtype, a.q, (long)(row0 + t) * a.q_stride + (long)h * D + j * 64 + c4 * 16 + w * 4, y);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              x[j][w * 4 + e] = y[e];
-              top = max(top, __float_as_uint(y[e]) & 0x7fffffffu);
-            }
-          }
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const bool finite = top < 0x7f800000u;
-        // |q| <= 127 * 256^2; tiny rows keep a step that is a normal number
-        const int ex = max(e8m0_exponent<127>(__uint_as_float(top)) - 16, -126);
-        const float inv = finite ? __int_as_float((127 - ex) << 23) : 0.0f;
-#pragma unroll
-        for (int j = 0; j < kJ; ++j)
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            uint32_t dig[3] = {0, 0, 0};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              int q = finite ? __float2int_rn(x[j][w * 4 + e] * inv) : 0;
-#pragma unroll
-              for (int p = 2; p >= 0; --p) {       // digit 0 is the uppermost
-                dig[p] |= (uint32_t)(q & 0xFF) << (8 * e);
-                q = (q + 128) >> 8;
-              }
-            }
-#pragma unroll
-            for (int p = 0; p < 3; ++p) qa[m][p][j][w] = dig[p];
-          }
-        qs[m] = finite ? __int_as_float((ex + 127) << 23) * a.scale2 : __int_as_float(0x7fc00000);
-        last[m] = row < nrows ? past + t : -1;
-        mx[m] = neg_inf();
-        sum[m] = 0.0f;
-#pragma unroll
-        for (int u = 0; u < kU; ++u)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[m][u][e] = 0.0f;
-      }
-    }
-
+    Tile t;
+    if (has) t.start(a, row0, tile, head, nrows, past);
     for (; i < end; ++i) {
-      const int nx = i + ST - 1;
+      const int nx = i + kStages;
       // place / place_sc: the 32 places that hold nx
       if ((i & 31) == 0 && i) {
         pl_now = place;
         sc_now = place_sc;
       }
       if ((nx & 31) == 0) look_up(lo + nx);
-      cp_wait<ST - 2>();
-      __syncwarp();
-      const uint8_t* st = ring + (i % ST) * kStage;
+      uint8_t* st = ring + (i % kStages) * kStage;
       const long at = __shfl_sync(0xffffffffu, pl_now, i & 31);
       const uint32_t sc = __shfl_sync(0xffffffffu, sc_now, i & 31);
-      if (at >= 0) {
-        const float ks = e8m0_to_float(sc & 0xFF), vs = e8m0_to_float(sc >> 8);
-        const int key0 = ((int)(lo + i - unit0) - kStart) * 32 + 2 * c4;
-        int acc[kTiles][4][4];
-#pragma unroll
-        for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-          for (int n = 0; n < 4; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[t][n][e] = 0;
-#pragma unroll
-        for (int n = 0; n < 4; ++n)
-#pragma unroll
-          for (int j = 0; j < kJ; ++j) {
-            const int row = 8 * n + r8;
-            const int ch = D == 128 ? row * 8 + ((j * 4 + c4) ^ ((row & 1) << 2)) : row * 4 + c4;
-            const uint4 b = *reinterpret_cast<const uint4*>(st + ch * 16);
-#pragma unroll
-            for (int m = 0; m < MT; ++m) {
-              mma_s8(acc[m][n], qa[m][0][j][0], qa[m][1][j][0], qa[m][0][j][1], qa[m][1][j][1], b.x, b.y);
-              mma_s8(acc[m][n], qa[m][0][j][2], qa[m][1][j][2], qa[m][0][j][3], qa[m][1][j][3], b.z, b.w);
-            }
-            mma_s8(acc[kTiles - 1][n], qa[0][2][j][0], MT == 2 ? qa[MT - 1][2][j][0] : 0u, qa[0][2][j][1],
-                   MT == 2 ? qa[MT - 1][2][j][1] : 0u, b.x, b.y);
-            mma_s8(acc[kTiles - 1][n], qa[0][2][j][2], MT == 2 ? qa[MT - 1][2][j][2] : 0u, qa[0][2][j][3],
-                   MT == 2 ? qa[MT - 1][2][j][3] : 0u, b.z, b.w);
-          }
-        uint32_t pa[MT][NP][2];          // probabilities' digits, slots 0-3 and 4-7
-        float fac[MT], alpha[MT];
-        bool same = true;
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          float x[8];
-          float bm = neg_inf();
-          const float f = qs[m] * ks;
-#pragma unroll
-          for (int n = 0; n < 4; ++n)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int hl = acc[m][n][e] * 256 + acc[m][n][2 + e];
-              float s = fmaf((float)hl, 256.0f, (float)acc[kTiles - 1][n][2 * m + e]);
-              s = key0 + 8 * n + e <= last[m] ? s * f : neg_inf();
-              x[2 * n + e] = s;
-              bm = fmaxf(bm, s);
-            }
-          bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, 1));
-          bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, 2));
-          const bool none = bm == neg_inf();
-          const float mn = fmaxf(mx[m], bm), ms = mn == neg_inf() ? 0.0f : mn;
-          const float beta = none ? 0.0f : ex2(bm - ms);
-          alpha[m] = ex2(mx[m] - ms);
-          same = same && mn == mx[m];
-          const float bs = none ? 0.0f : bm;
-          float ps = 0.0f;
-          constexpr float kTop = NP == 2 ? 32512.0f : 8323072.0f;       // 127 * 256^(NP-1)
-#pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            uint32_t w[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float p = ex2(x[4 * g + e] - bs);
-              ps += p;
-              // the sum with 2^23 leaves the nearest integer in the low bits
-              w[e] = __float_as_uint(fmaf(p, kTop, 8388608.0f));
-            }
-#pragma unroll
-            for (int p = NP - 1; p >= 0; --p) {
-              pa[m][p][g] = __byte_perm(__byte_perm(w[0], w[1], 0x0040), __byte_perm(w[2], w[3], 0x0040), 0x5410);
-              if (p) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) w[e] = (w[e] + 128) >> 8;
-              }
-            }
-          }
-          sum[m] = sum[m] * alpha[m] + ps * beta;
-          mx[m] = mn;
-          fac[m] = none ? 0.0f : beta * vs * (1.0f / kTop);
-        }
-        same = __all_sync(0xffffffffu, same);
-        if (!same) {
-#pragma unroll
-          for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int u = 0; u < kU; ++u)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) o[m][u][e] *= alpha[m];
-        }
-        const uint8_t* sv = st + 32 * D;
-#pragma unroll
-        for (int u = 0; u < kU; ++u) {
-          const uint4 b = *reinterpret_cast<const uint4*>(sv + ((8 * u + r8) * 4 + c4) * 16);
-#pragma unroll
-          for (int d = 0; d < 2; ++d) {
-            const uint32_t b_lo = d ? b.z : b.x, b_hi = d ? b.w : b.y;
-            int pv[kTilesP][4];
-#pragma unroll
-            for (int t = 0; t < kTilesP; ++t)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) pv[t][e] = 0;
-#pragma unroll
-            for (int m = 0; m < MT; ++m)
-              mma_s8(pv[m], pa[m][0][0], pa[m][1][0], pa[m][0][1], pa[m][1][1], b_lo, b_hi);
-            if (NP == 3)
-              mma_s8(pv[kTilesP - 1], pa[0][NP - 1][0], MT == 2 ? pa[MT - 1][NP - 1][0] : 0u, pa[0][NP - 1][1],
-                     MT == 2 ? pa[MT - 1][NP - 1][1] : 0u, b_lo, b_hi);
-#pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                float s = (float)(pv[m][e] * 256 + pv[m][2 + e]);
-                if (NP == 3) s = fmaf(s, 256.0f, (float)pv[kTilesP - 1][2 * m + e]);
-                o[m][u][2 * e + d] = fmaf(s, fac[m], o[m][u][2 * e + d]);
-              }
-          }
-        }
-      }
-      __syncwarp();                      // every lane has read stage i before it is refilled
-      if (nx < mine) fetch(nx);
-      else cp_commit();
+      cp_wait<2 * kStages - 1>();        // K of place i is there; V of it and what follows may be on the way
+      __syncwarp();
+      if (at >= 0)
+        t.keys(st, ((int)(lo + i - unit0) - kStart) * 32, e8m0_to_float(sc & 0xFF), e8m0_to_float(sc >> 8), scratch);
+      __syncwarp();                      // every lane has read it before it is refilled
+      fetch(nx, false);
+      cp_wait<2 * kStages - 1>();        // V of place i
+      __syncwarp();
+      if (at >= 0) t.values(st + 32 * D, scratch);
+      __syncwarp();
+      fetch(nx, true);
     }
     if (!has) continue;
 
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      sum[m] += __shfl_xor_sync(0xffffffffu, sum[m], 1);
-      sum[m] += __shfl_xor_sync(0xffffffffu, sum[m], 2);
-    }
-    // lane (r8, c4) has dimensions 16 u + 4 c4 .. + 3 of its rows
+    t.finish();
     if (g_first == g_last) {
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-        if (m * 8 + r8 < nrows)
-#pragma unroll
-          for (int u = 0; u < kU; ++u)
-            write_row<D>(a, row0, tile * kRows, m * 8 + r8, head, u * 16 + c4 * 4, o[m][u], mx[m], sum[m]);
+      t.write(a, row0, tile, head, nrows);
     } else {
       // the piece's last unit may take the ring's place, an earlier one goes to workspace
       const bool final = i >= mine;
@@ -479,19 +715,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attn_kernel(AttnArgs a) {
         __syncwarp();
       }
       float* at = final ? reinterpret_cast<float*>(ring) : a.warp_part + (long)piece * kPart;
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        const int row = m * 8 + r8;
-        if (row < nrows) {
-#pragma unroll
-          for (int u = 0; u < kU; ++u)
-            *reinterpret_cast<float4*>(at + row * D + u * 16 + c4 * 4) = make_float4(o[m][u][0], o[m][u][1], o[m][u][2], o[m][u][3]);
-          if (c4 == 0) {
-            at[kRows * D + row] = mx[m];
-            at[kRows * (D + 1) + row] = sum[m];
-          }
-        }
-      }
+      t.park(at, nrows);
       if (lane == 0) s_part[warp * 2 + (piece == g_first ? 1 : 0)] = Part{unit0, at, row0, tile, head, nrows, g_first, g_last, 1};
     }
   }
@@ -599,27 +823,23 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attn_kernel(AttnArgs a) {
   }
 }
 
-SmemAttr g_attn_attr[2][2][2][2];
-
-template <int D, int MT, int NP, int ST>
+template <typename Tile>
 cudaError_t launch(const AttnArgs& a, int ctas, cudaStream_t st) {
-  const size_t smem = (size_t)kWarps * ST * 64 * D + ((size_t)a.R + 1) * 8;
-  const cudaError_t e = g_attn_attr[D == 128][MT - 1][NP - 2][ST - 2].ensure(kv_attn_kernel<D, MT, NP, ST>, smem);
+  static SmemAttr attr;
+  const size_t smem = (size_t)Tile::kWarps * (kStages * 64 * Tile::D + 128) + ((size_t)a.R + 1) * 8;
+  const cudaError_t e = attr.ensure(kv_attn_kernel<Tile>, smem);
   if (e != cudaSuccess) return e;
-  kv_attn_kernel<D, MT, NP, ST><<<(unsigned)ctas, kThreads, smem, st>>>(a);
+  kv_attn_kernel<Tile><<<(unsigned)ctas, Tile::kWarps * 32, smem, st>>>(a);
   return cudaGetLastError();
 }
 
-// Three stages a warp where the lengths' sums leave the room (228 KB an SM).
-template <int D, int MT, int NP>
-cudaError_t launch_st(const AttnArgs& a, int ctas, cudaStream_t st) {
-  return a.R <= 3000 || D == 64 ? launch<D, MT, NP, 3>(a, ctas, st) : launch<D, MT, NP, 2>(a, ctas, st);
-}
-
+// One row a unit, eight while no request has more (16-row tiles spend twice the
+// registers on them), else sixteen.
 template <int D>
-cudaError_t launch_d(const AttnArgs& a, bool two, bool f32, int ctas, cudaStream_t st) {
-  if (two) return f32 ? launch_st<D, 2, 3>(a, ctas, st) : launch_st<D, 2, 2>(a, ctas, st);
-  return f32 ? launch_st<D, 1, 3>(a, ctas, st) : launch_st<D, 1, 2>(a, ctas, st);
+cudaError_t launch_rows(const AttnArgs& a, size_t rows, bool f32, int ctas, cudaStream_t st) {
+  if (rows == 1) return f32 ? launch<DotTile<D, 3>>(a, ctas, st) : launch<DotTile<D, 2>>(a, ctas, st);
+  if (rows <= 8) return f32 ? launch<MmaTile<D, 1, 3>>(a, ctas, st) : launch<MmaTile<D, 1, 2>>(a, ctas, st);
+  return f32 ? launch<MmaTile<D, 2, 3>>(a, ctas, st) : launch<MmaTile<D, 2, 2>>(a, ctas, st);
 }
 
 int bad(mxq_context* c, const char* msg) { return ctx_fail(c, MXQ_ERR_INVALID_ARGUMENT, msg); }
@@ -673,17 +893,15 @@ int mxq_kv_attention(mxq_ctx c, const mxq_kv_cache* cache, int dtype, const void
   // a part for each warp and two for each CTA
   const size_t per = kMaxRows * (size_t)(kv.dim + 2) * 4;
   int ctas = ws.sms;
-  const int fit = (int)(kServeScratch / ((kWarps + 2) * per));
+  const int fit = (int)(kServeScratch / ((kMaxWarps + 2) * per));
   if (ctas > fit) ctas = fit;
   if (ctas > (int)kServeCounters - 1) ctas = (int)kServeCounters - 1;
   a.warp_part = reinterpret_cast<float*>(ws.scratch);
-  a.cta_part = reinterpret_cast<float*>(ws.scratch + (size_t)ctas * kWarps * per);
-  // eight rows a tile while no request has more (16-row tiles spend twice the
-  // registers and, below nine rows, the same MMAs)
-  const bool two = max_new * (size_t)a.G > 8;
+  a.cta_part = reinterpret_cast<float*>(ws.scratch + (size_t)ctas * kMaxWarps * per);
+  const size_t rows = max_new * (size_t)a.G;
   const cudaStream_t st = ctx_stream(c);
   const bool f32 = dtype == MXQ_DT_F32;
-  const cudaError_t e = kv.dim == 64 ? launch_d<64>(a, two, f32, ctas, st) : launch_d<128>(a, two, f32, ctas, st);
+  const cudaError_t e = kv.dim == 64 ? launch_rows<64>(a, rows, f32, ctas, st) : launch_rows<128>(a, rows, f32, ctas, st);
   return serve_launched(c, e, "kv attention");
 }
 

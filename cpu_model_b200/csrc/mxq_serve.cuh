@@ -82,6 +82,13 @@ __device__ __forceinline__ void store4_dt(int dt, void* p, long at, const float 
   else store4(static_cast<__half*>(p) + at, v);
 }
 
+__device__ __forceinline__ void store2_dt(int dt, void* p, long at, float x, float y) {
+  if (dt == MXQ_DT_F32) *reinterpret_cast<float2*>(static_cast<float*>(p) + at) = make_float2(x, y);
+  else if (dt == MXQ_DT_BF16)
+    *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(p) + at) = __floats2bfloat162_rn(x, y);
+  else *reinterpret_cast<__half2*>(static_cast<__half*>(p) + at) = __floats2half2_rn(x, y);
+}
+
 // ------------------------------------------------------------------ host --
 struct ServeDevice {
   int prev = -1;
