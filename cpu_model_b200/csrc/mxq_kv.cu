@@ -190,8 +190,8 @@ __global__ void __launch_bounds__(1024) kv_release_kernel(const uint8_t* done, i
 
 // ---------------------------------------------------------------- append --
 
-constexpr int kAppendThreads = 256;
-constexpr int kCtaRun = 8;         // runs of at least this many rows take the whole CTA, shorter ones a warp
+constexpr int kCopyWarps = 4;      // warps a CTA, each on its own
+constexpr int kLongRun = 8;        // runs of at least this many rows are built in registers
 
 // Four int8 of a word re-rounded to a step 2^d times as large.
 __device__ __forceinline__ uint32_t reround4(uint32_t w, float down) {
@@ -211,238 +211,331 @@ __device__ __forceinline__ uint4 reround16(uint4 w, float down) {
 __device__ __forceinline__ int scale_byte(uint32_t top) {
   return top >= 0x7f800000u ? 255 : e8m0_exponent<127>(__uint_as_float(top)) + 127;
 }
-__device__ __forceinline__ int quant_byte(float x, int byte) {
-  return byte == 255 ? 0 : quant_value(x, byte - 127);
-}
 // 2^(from - to), 0 once every int8 rounds to 0
 __device__ __forceinline__ float step_down(int from, int to) {
   const int d = to - from;
   return d > 30 ? 0.0f : __int_as_float((127 - d) << 23);
 }
+// rint(x * inv) in the low byte: x * inv is exact (a power of two), the sum with 1.5 * 2^23 rounds it half to even
+__device__ __forceinline__ uint32_t quant_bits(float x, float inv) {
+  return __float_as_uint(fmaf(x, inv, 12582912.0f));
+}
 
-// One CTA: the runs that start in `chunk` consecutive rows, of one head, of K
-// (z = 0) or V (z = 1).  A run of a prompt fills up to 32 rows: 256 threads
-// hold it in registers, agree on the exponent, and write 16 bytes each (V by
-// way of shared memory, which turns it).  A decode step's runs are one row
-// each: a warp a run.
+// A lane's V consecutive values of a row, as loaded.
+template <typename T, int V> struct Raw {
+  uint32_t w[V * sizeof(T) / 4];
+  __device__ __forceinline__ void load(const T* p) {
+    constexpr int kBytes = V * (int)sizeof(T);
+    if (kBytes == 16) {
+      const uint4 x = __ldg(reinterpret_cast<const uint4*>(p));
+      w[0] = x.x; w[1 % (kBytes / 4)] = x.y; w[2 % (kBytes / 4)] = x.z; w[3 % (kBytes / 4)] = x.w;
+    } else if (kBytes == 8) {
+      const uint2 x = __ldg(reinterpret_cast<const uint2*>(p));
+      w[0] = x.x; w[1 % (kBytes / 4)] = x.y;
+    } else {
+      w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+    }
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < V * (int)sizeof(T) / 4; ++i) w[i] = 0;
+  }
+  __device__ __forceinline__ float get(int i) const;
+};
+template <> __device__ __forceinline__ float Raw<float, 4>::get(int i) const { return __uint_as_float(w[i]); }
+template <> __device__ __forceinline__ float Raw<float, 2>::get(int i) const { return __uint_as_float(w[i]); }
+__device__ __forceinline__ float bf16_at(uint32_t w, int i) { return __uint_as_float(i & 1 ? w & 0xFFFF0000u : w << 16); }
+template <> __device__ __forceinline__ float Raw<__nv_bfloat16, 4>::get(int i) const { return bf16_at(w[i >> 1], i); }
+template <> __device__ __forceinline__ float Raw<__nv_bfloat16, 2>::get(int i) const { return bf16_at(w[0], i); }
+__device__ __forceinline__ float f16_at(uint32_t w, int i) {
+  return __half2float(__ushort_as_half((unsigned short)(i & 1 ? w >> 16 : w & 0xFFFFu)));
+}
+template <> __device__ __forceinline__ float Raw<__half, 4>::get(int i) const { return f16_at(w[i >> 1], i); }
+template <> __device__ __forceinline__ float Raw<__half, 2>::get(int i) const { return f16_at(w[0], i); }
+
+// The byte mask of the V word with tokens 16 w + 2 c + {0, 1, 8, 9}, from a mask of the block's tokens.
+__device__ __forceinline__ uint32_t v_word_mask(uint32_t tokens, int c, int w) {
+  const uint32_t t = tokens >> (16 * w + 2 * c);
+  return (t & 1 ? 0xFFu : 0u) | (t & 2 ? 0xFF00u : 0u) | (t & 0x100 ? 0xFF0000u : 0u) | (t & 0x200 ? 0xFF000000u : 0u);
+}
+
+// Runs among 32 consecutive entries base .. of a slot list (of which `chunk`
+// may start one): entries whose slots follow one another in a block.
+struct Runs {
+  int s0, s1;                      // slot of entry base + lane, base + 32 + lane; -1: outside the pool or the list
+  uint32_t starts;                 // entries that start a run
+  __device__ __forceinline__ Runs(const int32_t* slot, int n, int slots, int base, int chunk) {
+    const int lane = threadIdx.x & 31;
+    auto at = [&](int i) {
+      const int s = i >= 0 && i < n ? slot[i] : -1;
+      return s < slots ? s : -1;
+    };
+    s0 = at(base + lane);
+    s1 = at(base + 32 + lane);
+    const int first_before = lane == 0 ? at(base - 1) : 0;
+    const int up = __shfl_up_sync(0xffffffffu, s0, 1);
+    const int before = lane == 0 ? first_before : up;
+    starts = __ballot_sync(0xffffffffu, lane < chunk && s0 >= 0 && !(before >= 0 && s0 == before + 1 && (s0 & 31)));
+  }
+  // The run that starts at entry `first`: its slot and length.
+  __device__ __forceinline__ int run(int first, int* len) const {
+    const int lane = threadIdx.x & 31;
+    const int s = __shfl_sync(0xffffffffu, s0, first);
+    const uint32_t e0 = __ballot_sync(0xffffffffu, s0 == s + (lane - first) && (s0 >> 5) == (s >> 5));
+    const uint32_t e1 = __ballot_sync(0xffffffffu, s1 == s + (lane + 32 - first) && (s1 >> 5) == (s >> 5));
+    const uint64_t e = ((uint64_t)e1 << 32 | e0) >> first;
+    *len = min(__ffsll((long long)~e) - 1, 32);
+    return s;
+  }
+};
+
+// A warp: the runs that start in `chunk` consecutive rows, of one head, of K
+// (z = 0) or V (z = 1).  A lane has D / 32 dimensions of every row.  A long
+// run is read once into registers, all rows in flight; a K row leaves as 4
+// bytes a lane, and V needs no exchange between lanes, since the 16-byte pieces of
+// its layout (two dimensions, eight tokens) each lie with one lane.  A decode step's runs
+// are one row each: V's bytes go out one by one, less than a block's way in and out.
 template <typename T, int D>
-__global__ void __launch_bounds__(kAppendThreads)
+__global__ void __launch_bounds__(kCopyWarps * 32)
     kv_append_kernel(KvView c, const T* __restrict__ k, const T* __restrict__ v, long stride,
                      const int32_t* __restrict__ slot, int n, int chunk) {
-  constexpr int kPad = 4;
-  __shared__ int s_slot[32 + 33];
-  __shared__ int s_first[32], s_len[32];
-  __shared__ int s_runs;
-  __shared__ uint32_t s_top[kAppendThreads / 32];
-  __shared__ uint8_t s_q[32][D + kPad];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int base = blockIdx.x * chunk, head = blockIdx.y;
+  constexpr int V = D / 32;        // dimensions a lane
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int base = (blockIdx.x * kCopyWarps + warp) * chunk, head = blockIdx.y;
+  if (base >= n) return;
   const bool is_v = blockIdx.z != 0;
-  const T* src = (is_v ? v : k) + (long)head * D;
+  const T* src = (is_v ? v : k) + (long)head * D + lane * V;
   int8_t* data = is_v ? c.v : c.k;
   uint8_t* scales = is_v ? c.vs : c.ks;
-  const int slots = c.n_pages * c.page;
+  const Runs runs(slot, n, c.n_pages * c.page, base, chunk);
 
-  // slots of the rows base - 1 .. base + chunk + 30
-  for (int i = tid; i < chunk + 32; i += kAppendThreads) {
-    const int row = base - 1 + i;
-    const int s = row >= 0 && row < n ? slot[row] : -1;
-    s_slot[i] = s >= 0 && s < slots ? s : -1;
-  }
-  __syncthreads();
-  if (warp == 0) {
-    bool lead = false;
-    int len = 0;
-    if (lane < chunk) {
-      const int s = s_slot[lane + 1], before = s_slot[lane];
-      lead = s >= 0 && (before < 0 || (before >> 5) != (s >> 5));
-      if (lead)
-        for (len = 1; len < 32; ++len) {
-          const int u = s_slot[lane + 1 + len];
-          if (u < 0 || (u >> 5) != (s >> 5)) break;
-        }
-    }
-    const uint32_t all = __ballot_sync(0xffffffffu, lead);
-    if (lead) {
-      const int at = __popc(all & ((1u << lane) - 1));
-      s_first[at] = lane;
-      s_len[at] = len;
-    }
-    if (lane == 0) s_runs = __popc(all);
-  }
-  __syncthreads();
-  const int runs = s_runs;
-
-  for (int i = 0; i < runs; ++i) {           // long runs: the whole CTA
-    const int first = s_first[i], len = s_len[i];
-    if (len < kCtaRun) continue;
-    const int s0 = s_slot[first + 1];
+  for (uint32_t left = runs.starts; left; left &= left - 1) {
+    int len;
+    const int first = __ffs((int)left) - 1, s0 = runs.run(first, &len), o = s0 & 31;
     const long blk = kv_block(c, s0 / c.page, head, (s0 % c.page) >> 5);
     uint8_t* dst = reinterpret_cast<uint8_t*>(data) + blk * (32 * D);
-    constexpr int kVals = D / 8;             // values a thread: row tid / 8, an eighth of it
-    const int row = tid >> 3, seg = tid & 7;
-    float x[kVals];
-    uint32_t top = 0;
-    if (row < len) {
-#pragma unroll
-      for (int u = 0; u < kVals; u += 4) {
-        float y[4];
-        load4(src + (long)(base + first + row) * stride + seg * kVals + u, y);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          x[u + e] = y[e];
-          top = max(top, __float_as_uint(y[e]) & 0x7fffffffu);
-        }
-      }
-    }
-    const bool extends = (s0 & 31) != 0;
-    const int was = extends ? scales[blk] : 0;
-    top = __reduce_max_sync(0xffffffffu, top);
-    if (lane == 0) s_top[warp] = top;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kAppendThreads / 32; ++w) top = max(top, s_top[w]);
-    const int byte = max(scale_byte(top), was);
-    const bool grew = extends && byte > was && byte != 255;
-    const float down = grew ? step_down(was, byte) : 1.0f;
-    uint32_t in_run = 0;
-    for (int r = 0; r < len; ++r) in_run |= 1u << (s_slot[first + 1 + r] & 31);
-    uint32_t q[kVals / 4];
-    if (row < len) {
-#pragma unroll
-      for (int u = 0; u < kVals; ++u) {
-        if ((u & 3) == 0) q[u / 4] = 0;
-        q[u / 4] |= (uint32_t)(quant_byte(x[u], byte) & 0xFF) << (8 * (u & 3));
-      }
-      const int t = s_slot[first + 1 + row] & 31;
-      uint8_t* to = is_v ? &s_q[t][seg * kVals] : dst + t * D + seg * kVals;
-#pragma unroll
-      for (int u = 0; u < kVals / 4; ++u) reinterpret_cast<uint32_t*>(to)[u] = q[u];
-    }
-    if (!is_v) {
-      if (grew && !(in_run >> row & 1)) {
-        uint32_t* old = reinterpret_cast<uint32_t*>(dst + row * D + seg * kVals);
-#pragma unroll
-        for (int u = 0; u < kVals / 4; ++u) old[u] = reround4(old[u], down);
-      }
-    } else {
-      __syncthreads();
-      for (int ch = tid; ch < 2 * D; ch += kAppendThreads) {   // 16 bytes: two dimensions, eight tokens
-        const int pair = ch >> 2, cc = ch & 3;
-        uint4* to = reinterpret_cast<uint4*>(dst) + ch;
-        uint4 w = make_uint4(0, 0, 0, 0);
-        if (extends) {
-          w = *to;
-          if (grew) w = reround16(w, down);
-        }
-        uint32_t out[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int dd = e >> 3, t = ((e & 7) >> 1) * 8 + 2 * cc + (e & 1);
-          if (in_run >> t & 1) {
-            const uint32_t b = s_q[t][2 * pair + dd];
-            out[e >> 2] = (out[e >> 2] & ~(0xFFu << (8 * (e & 3)))) | b << (8 * (e & 3));
-          }
-        }
-        *to = make_uint4(out[0], out[1], out[2], out[3]);
-      }
-    }
-    if (tid == 0) scales[blk] = (uint8_t)byte;
-    __syncthreads();
-  }
-
-  for (int i = warp; i < runs; i += kAppendThreads / 32) {   // short runs: a warp each
-    const int first = s_first[i], len = s_len[i];
-    if (len >= kCtaRun) continue;
-    const int s0 = s_slot[first + 1];
-    const long blk = kv_block(c, s0 / c.page, head, (s0 % c.page) >> 5);
-    uint8_t* dst = reinterpret_cast<uint8_t*>(data) + blk * (32 * D);
-    const bool extends = (s0 & 31) != 0, mine = lane < D / 4;
-    const int was = extends ? scales[blk] : 0;
-    uint32_t top = 0;
-    if (mine)
+    const int was = o ? scales[blk] : 0;
+    const T* rows = src + (long)(base + first) * stride;
+    if (len < kLongRun) {
+      uint32_t top = 0;
+      Raw<T, V> x;
       for (int r = 0; r < len; ++r) {
-        float y[4];
-        load4(src + (long)(base + first + r) * stride + lane * 4, y);
+        x.load(rows + (long)r * stride);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(y[e]) & 0x7fffffffu);
+        for (int e = 0; e < V; ++e) top = max(top, __float_as_uint(x.get(e)) & 0x7fffffffu);
       }
-    top = __reduce_max_sync(0xffffffffu, top);
-    const int byte = max(scale_byte(top), was);
-    if (extends && byte > was && byte != 255) {
-      const float down = step_down(was, byte);
+      top = __reduce_max_sync(0xffffffffu, top);
+      const int byte = max(scale_byte(top), was);
+      if (o && byte > was && byte != 255) {
+        const float down = step_down(was, byte);
 #pragma unroll
-      for (int u = 0; u < 2 * D / 32; ++u) {
-        uint4* w = reinterpret_cast<uint4*>(dst) + u * 32 + lane;
-        *w = reround16(*w, down);
+        for (int u = 0; u < 2 * D / 32; ++u) {
+          uint4* w = reinterpret_cast<uint4*>(dst) + u * 32 + lane;
+          *w = reround16(*w, down);
+        }
+        __syncwarp();
       }
-      __syncwarp();
-    }
-    if (mine)
+      const float inv = byte == 255 ? 0.0f : __int_as_float((254 - byte) << 23);
       for (int r = 0; r < len; ++r) {
-        float y[4];
-        load4(src + (long)(base + first + r) * stride + lane * 4, y);
-        const int t = s_slot[first + 1 + r] & 31;
+        if (len > 1) x.load(rows + (long)r * stride);
         uint32_t w = 0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t q = (uint32_t)quant_byte(y[e], byte) & 0xFF;
-          if (is_v) dst[v_offset(t, lane * 4 + e)] = (uint8_t)q;
+        for (int e = 0; e < V; ++e) {
+          const uint32_t q = byte == 255 ? 0u : quant_bits(x.get(e), inv) & 0xFF;
+          if (is_v) dst[v_offset(o + r, lane * V + e)] = (uint8_t)q;
           w |= q << (8 * e);
         }
-        if (!is_v) *reinterpret_cast<uint32_t*>(dst + t * D + lane * 4) = w;
+        if (!is_v) {
+          if (V == 4) *reinterpret_cast<uint32_t*>(dst + (o + r) * D + lane * 4) = w;
+          else *reinterpret_cast<uint16_t*>(dst + (o + r) * D + lane * 2) = (uint16_t)w;
+        }
       }
+      if (lane == 0) scales[blk] = (uint8_t)byte;
+      continue;
+    }
+
+    // x[t]: the row of the block's token t
+    Raw<T, V> x[32];
+#pragma unroll
+    for (int t = 0; t < 32; ++t) {
+      if (t >= o && t < o + len) x[t].load(rows + (long)(t - o) * stride);
+      else x[t].clear();
+    }
+    uint32_t top = 0;
+#pragma unroll
+    for (int t = 0; t < 32; ++t)
+#pragma unroll
+      for (int e = 0; e < V; ++e) top = max(top, __float_as_uint(x[t].get(e)) & 0x7fffffffu);
+    top = __reduce_max_sync(0xffffffffu, top);
+    const int byte = max(scale_byte(top), was);
+    const bool grew = o && byte > was && byte != 255;
+    const float down = grew ? step_down(was, byte) : 1.0f;
+    const float inv = byte == 255 ? 0.0f : __int_as_float((254 - byte) << 23);
+    const uint32_t tokens = (len == 32 ? 0xffffffffu : (1u << len) - 1) << o;
+    if (byte == 255) {
+#pragma unroll
+      for (int t = 0; t < 32; ++t) x[t].clear();
+    }
+    if (!is_v) {
+#pragma unroll
+      for (int t = 0; t < 32; ++t) {
+        uint32_t w = 0;
+        if (V == 4) {
+          const uint32_t lo = __byte_perm(quant_bits(x[t].get(0), inv), quant_bits(x[t].get(1), inv), 0x0040);
+          const uint32_t hi = __byte_perm(quant_bits(x[t].get(2 % V), inv), quant_bits(x[t].get(3 % V), inv), 0x0040);
+          w = __byte_perm(lo, hi, 0x5410);
+          uint32_t* to = reinterpret_cast<uint32_t*>(dst + t * D + lane * 4);
+          if (tokens >> t & 1) *to = w;
+          else if (grew) *to = reround4(*to, down);
+        } else {
+          w = __byte_perm(quant_bits(x[t].get(0), inv), quant_bits(x[t].get(1), inv), 0x0040);
+          uint16_t* to = reinterpret_cast<uint16_t*>(dst + t * D + lane * 2);
+          if (tokens >> t & 1) *to = (uint16_t)w;
+          else if (grew) *to = (uint16_t)reround4(*to, down);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int pr = 0; pr < V / 2; ++pr)
+#pragma unroll
+        for (int cc = 0; cc < 4; ++cc) {
+          uint32_t w[4];           // dimension 2 pr: tokens of words 0, 1; then 2 pr + 1
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int t0 = 16 * (e & 1) + 2 * cc, d = 2 * pr + (e >> 1);
+            const uint32_t lo = __byte_perm(quant_bits(x[t0].get(d), inv), quant_bits(x[t0 + 1].get(d), inv), 0x0040);
+            const uint32_t hi = __byte_perm(quant_bits(x[t0 + 8].get(d), inv), quant_bits(x[t0 + 9].get(d), inv), 0x0040);
+            w[e] = __byte_perm(lo, hi, 0x5410);
+          }
+          uint4* to = reinterpret_cast<uint4*>(dst) + (lane * (V / 2) + pr) * 4 + cc;
+          if (o) {                 // the block's other tokens stay
+            uint4 old = *to;
+            if (grew) old = reround16(old, down);
+            const uint32_t m0 = v_word_mask(tokens, cc, 0), m1 = v_word_mask(tokens, cc, 1);
+            w[0] = (w[0] & m0) | (old.x & ~m0);
+            w[1] = (w[1] & m1) | (old.y & ~m1);
+            w[2] = (w[2] & m0) | (old.z & ~m0);
+            w[3] = (w[3] & m1) | (old.w & ~m1);
+          }
+          *to = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
     if (lane == 0) scales[blk] = (uint8_t)byte;
   }
 }
 
 // ------------------------------------------------------------------ read --
 
+// N consecutive values, N * sizeof(T) bytes aligned.
+__device__ __forceinline__ void put2(float* p, float a, float b) { *reinterpret_cast<float2*>(p) = make_float2(a, b); }
+__device__ __forceinline__ void put2(__nv_bfloat16* p, float a, float b) {
+  *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(a, b);
+}
+__device__ __forceinline__ void put2(__half* p, float a, float b) {
+  *reinterpret_cast<__half2*>(p) = __floats2half2_rn(a, b);
+}
+
+// A warp: `chunk` consecutive entries, of one head, of K or V.  K rows are read
+// four at a time.  V is read a run at a time, whole blocks in 16-byte pieces: a
+// lane has two dimensions of eight tokens, and four lanes' stores reach
+// four rows in whole sectors.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) kv_read_kernel(KvView c, const int32_t* __restrict__ slot, int n,
-                                                      T* __restrict__ k_out, T* __restrict__ v_out) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, head = blockIdx.y;
+__global__ void __launch_bounds__(kCopyWarps * 32)
+    kv_read_kernel(KvView c, const int32_t* __restrict__ slot, int n, int chunk, T* __restrict__ k_out,
+                   T* __restrict__ v_out) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int base = (blockIdx.x * kCopyWarps + warp) * chunk, head = blockIdx.y;
+  if (base >= n) return;
   const bool is_v = blockIdx.z != 0;
-  if (lane >= D / 4) return;
-  for (int i = blockIdx.x * 32 + warp; i < min(n, (int)(blockIdx.x + 1) * 32); i += 8) {
-    const int s = slot[i];
-    float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (s >= 0 && s < c.n_pages * c.page) {
+  const Runs runs(slot, n, c.n_pages * c.page, base, chunk);
+  const int count = min(chunk, n - base);
+  const long row = (long)c.heads * D;
+  T* out = (is_v ? v_out : k_out) + (long)base * row + (long)head * D;
+  // entries outside the pool
+  for (uint32_t z = __ballot_sync(0xffffffffu, lane < count && runs.s0 < 0); z; z &= z - 1) {
+    T* to = out + (long)(__ffs((int)z) - 1) * row;
+    for (int d = 2 * lane; d < D; d += 64) put2(to + d, 0.0f, 0.0f);
+  }
+  if (!is_v) {
+    constexpr int kLanes = D / 16, kRows = 32 / kLanes;    // 16 dimensions a lane
+    for (int i0 = 0; i0 < count; i0 += kRows) {
+      const int i = i0 + lane / kLanes;
+      const int s = __shfl_sync(0xffffffffu, runs.s0, i & 31);
+      if (i >= count || s < 0) continue;
       const long blk = kv_block(c, s / c.page, head, (s % c.page) >> 5);
-      const int8_t* at = (is_v ? c.v : c.k) + blk * (32 * D);
-      const float sc = e8m0_to_float((is_v ? c.vs : c.ks)[blk]);
+      const uint4 w = __ldg(reinterpret_cast<const uint4*>(c.k + blk * (32 * D) + (s & 31) * D) + lane % kLanes);
+      const float sc = e8m0_to_float(c.ks[blk]);
+      const uint32_t q[4] = {w.x, w.y, w.z, w.w};
+      T* to = out + (long)i * row + (lane % kLanes) * 16;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int d = lane * 4 + e;
-        y[e] = (float)at[is_v ? v_offset(s & 31, d) : (s & 31) * D + d] * sc;
+        float y[4];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) y[b] = (float)(int8_t)(q[e] >> (8 * b)) * sc;
+        store4(to + 4 * e, y);
       }
     }
-    store4((is_v ? v_out : k_out) + ((long)i * c.heads + head) * D + lane * 4, y);
+    return;
   }
+  // a run may have started before this warp's entries: its first entry here counts as a start
+  const int s_first = __shfl_sync(0xffffffffu, runs.s0, 0);
+  uint32_t left = runs.starts | (s_first >= 0 ? 1u : 0u);
+  for (; left; left &= left - 1) {
+    int len;
+    const int first = __ffs((int)left) - 1, s0 = runs.run(first, &len), o = s0 & 31;
+    len = min(len, count - first);
+    const long blk = kv_block(c, s0 / c.page, head, (s0 % c.page) >> 5);
+    const uint4* src = reinterpret_cast<const uint4*>(c.v + blk * (32 * D));
+    const float sc = e8m0_to_float(c.vs[blk]);
+    const int cc = lane & 3;
+    uint4 w[D / 16];
+#pragma unroll
+    for (int u = 0; u < D / 16; ++u) w[u] = __ldg(src + u * 32 + lane);
+#pragma unroll
+    for (int jb = 0; jb < 8; ++jb) {
+      const int r = (jb >> 1) * 8 + 2 * cc + (jb & 1) - o;   // the token's entry in the run
+      if (r < 0 || r >= len) continue;
+      T* to = out + (long)(first + r) * row + 2 * (lane >> 2);
+#pragma unroll
+      for (int u = 0; u < D / 16; ++u) {
+        const uint32_t a = jb < 4 ? w[u].x : w[u].y, b = jb < 4 ? w[u].z : w[u].w;
+        put2(to + u * 16, (float)(int8_t)(a >> (8 * (jb & 3))) * sc, (float)(int8_t)(b >> (8 * (jb & 3))) * sc);
+      }
+    }
+  }
+}
+
+// Rows a warp looks for runs in: 32 (a prompt's warp then has a block or two),
+// fewer while that many warps would leave the SMs without 16 each: a decode step's runs
+// are one row, and a warp takes its runs one after another (32 rows x 32
+// heads: 9.0 us with 8 rows a warp, 5.0 with one).
+int rows_a_warp(const KvView& c, int n) {
+  const long units = 2l * n * c.heads, enough = 148l * 16;
+  return units / 32 >= enough ? 32 : units / 8 >= enough ? 8 : 1;
 }
 
 template <typename T>
 cudaError_t launch_append(const KvView& c, const void* k, const void* v, long stride, const int32_t* slot, int n,
                           cudaStream_t st) {
-  // 8 rows a CTA while that leaves the GPU with few of them, 32 beyond
-  const int chunk = (long)n * c.heads <= 8l * 148 * 8 ? 8 : 32;
-  const dim3 grid((unsigned)((n + chunk - 1) / chunk), (unsigned)c.heads, 2);
+  const int chunk = rows_a_warp(c, n), per = chunk * kCopyWarps;
+  const dim3 grid((unsigned)((n + per - 1) / per), (unsigned)c.heads, 2);
   if (c.dim == 64)
-    kv_append_kernel<T, 64><<<grid, kAppendThreads, 0, st>>>(c, static_cast<const T*>(k), static_cast<const T*>(v),
-                                                             stride, slot, n, chunk);
-  else
-    kv_append_kernel<T, 128><<<grid, kAppendThreads, 0, st>>>(c, static_cast<const T*>(k), static_cast<const T*>(v),
+    kv_append_kernel<T, 64><<<grid, kCopyWarps * 32, 0, st>>>(c, static_cast<const T*>(k), static_cast<const T*>(v),
                                                               stride, slot, n, chunk);
+  else
+    kv_append_kernel<T, 128><<<grid, kCopyWarps * 32, 0, st>>>(c, static_cast<const T*>(k), static_cast<const T*>(v),
+                                                               stride, slot, n, chunk);
   return cudaGetLastError();
 }
 
 template <typename T>
 cudaError_t launch_read(const KvView& c, const int32_t* slot, int n, void* k, void* v, cudaStream_t st) {
-  const dim3 grid((unsigned)((n + 31) / 32), (unsigned)c.heads, 2);
+  const int chunk = rows_a_warp(c, n), per = chunk * kCopyWarps;
+  const dim3 grid((unsigned)((n + per - 1) / per), (unsigned)c.heads, 2);
   if (c.dim == 64)
-    kv_read_kernel<T, 64><<<grid, 256, 0, st>>>(c, slot, n, static_cast<T*>(k), static_cast<T*>(v));
+    kv_read_kernel<T, 64><<<grid, kCopyWarps * 32, 0, st>>>(c, slot, n, chunk, static_cast<T*>(k), static_cast<T*>(v));
   else
-    kv_read_kernel<T, 128><<<grid, 256, 0, st>>>(c, slot, n, static_cast<T*>(k), static_cast<T*>(v));
+    kv_read_kernel<T, 128><<<grid, kCopyWarps * 32, 0, st>>>(c, slot, n, chunk, static_cast<T*>(k), static_cast<T*>(v));
   return cudaGetLastError();
 }
 

@@ -871,7 +871,7 @@ def kv_plan(past, new, page_size, table, free_pages, free_count, n_tokens, in_pl
     ctx = _serve_ctx(ctx, past, new, table, free_pages, free_count)
     # one allocation for the maps and the two numbers
     sizes = [n, n, n, r + 1, 1] if in_place else [n, n, n, r + 1, 1, 1, r]
-    views = torch.empty(3 * n + r + 2 + (0 if in_place else 1 + r), dtype=torch.int32, device=past.device).split(sizes)
+    views = past.new_empty(3 * n + r + 2 + (0 if in_place else 1 + r)).split_with_sizes(sizes)
     slots, pos, req, cu, short = views[:5]
     free_out, ctx_len = (free_count, past) if in_place else views[5:]
     cu_at = cu.data_ptr()
@@ -929,8 +929,8 @@ def kv_read(cache, slots, dtype=torch.float32, ctx=None):
     ctx = _serve_ctx(ctx, cache.k, slots)
     n = slots.numel()
     shape = (n, cache.n_kv_heads, cache.head_dim)
-    k = torch.empty(shape, dtype=dtype, device=slots.device)
-    v = torch.empty(shape, dtype=dtype, device=slots.device)
+    k = slots.new_empty(shape, dtype=dtype)
+    v = torch.empty_like(k)
     rc = ctx.lib.mxq_kv_read(ctx.h, ctypes.byref(cache._c), slots.data_ptr(), n, _DTYPES[dtype], k.data_ptr(), v.data_ptr())
     if rc:
         check(rc, ctx.h)
@@ -957,9 +957,8 @@ def kv_attention(q, cache, table, ctx_len, cu, scale=None, max_new=None, want_ls
     if max_new is not None and max_new < 1:
         raise ValueError("kv_attention: max_new must be positive")
     ctx = _serve_ctx(ctx, cache.k, q, table, ctx_len, cu)
-    device = q.device
-    out = torch.empty((n, hq, d), dtype=q.dtype, device=device)
-    lse = torch.empty((n, hq), dtype=torch.float32, device=device) if want_lse else None
+    out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((n, hq, d))
+    lse = q.new_empty((n, hq), dtype=torch.float32) if want_lse else None
     rc = ctx.lib.mxq_kv_attention(ctx.h, ctypes.byref(cache._c), dt, q.data_ptr(), _row_stride(q, "q"), n, hq,
                                   table.data_ptr(), table.shape[1], ctx_len.data_ptr(), cu.data_ptr(), r,
                                   max(1, n if max_new is None else max_new), d ** -0.5 if scale is None else scale,
@@ -998,10 +997,9 @@ def token_logprobs(logits, targets, top_k=0, ctx=None):
     if not 0 <= top_k <= min(v, _lib.TOPK_MAX):
         raise ValueError("token_logprobs: top_k (%d) must be in [0, min(32, vocab=%d)]" % (top_k, v))
     ctx = _serve_ctx(ctx, logits, targets)
-    device = logits.device
-    logp, entropy, lse = torch.empty((3, n), dtype=torch.float32, device=device).unbind(0)
-    top = torch.empty((n, top_k), dtype=torch.float32, device=device) if top_k else None
-    ids = torch.empty((n, top_k), dtype=torch.int32, device=device) if top_k else None
+    logp, entropy, lse = logits.new_empty((3, n), dtype=torch.float32).unbind(0)
+    top = logits.new_empty((n, top_k), dtype=torch.float32) if top_k else None
+    ids = targets.new_empty((n, top_k)) if top_k else None
     rc = ctx.lib.mxq_token_logprobs(ctx.h, dt, logits.data_ptr(), stride, n, v, targets.data_ptr(), top_k, logp.data_ptr(),
                                     entropy.data_ptr(), lse.data_ptr(), _at(top), _at(ids))
     if rc:

@@ -643,8 +643,8 @@ MXQ_API int mxq_kv_release(mxq_ctx ctx, const uint8_t* done, int32_t* len,
 /* New rows into the cache: k, v [n][n_kv_heads][head_dim] of type dtype, row
  * i starting at i * row_stride elements (16-byte aligned rows; a slice of the
  * fused QKV rows will do), into slots slot[i] (outside the pool: skipped).
- * Consecutive rows of one block form a run, rows of a block must be
- * consecutive; o = the run's first offset in the block.  o = 0 starts the
+ * Consecutive rows whose slots follow one another in a block form a run; a
+ * call has one run for a block at most; o = the run's first offset in it.  o = 0 starts the
  * block: its exponent is the run's (smallest e with max|x| <= 127 * 2^e over
  * the run's rows of the head, as in mxq_quantize_x; NaN or inf: scale 255 and
  * zeros), the rest of the block is unspecified.  o > 0 extends it: the
