@@ -33,89 +33,97 @@ __device__ __forceinline__ int last_not_above(const int* a, int n, int x) {
   return lo;
 }
 
-// Inclusive sum over the block of one value a thread; every thread calls it.
-__device__ __forceinline__ int block_scan(int v, int* warp_sums, int* total) {
+// Inclusive sums over the block of a pair of values a thread; every thread calls it.
+__device__ __forceinline__ int2 block_scan(int2 v, int2* warp_sums, int2* total) {
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, nw = blockDim.x >> 5;
+#pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int u = __shfl_up_sync(0xffffffffu, v, o);
-    if (lane >= o) v += u;
+    const int a = __shfl_up_sync(0xffffffffu, v.x, o), b = __shfl_up_sync(0xffffffffu, v.y, o);
+    if (lane >= o) v.x += a, v.y += b;
   }
   __syncthreads();                 // the sums of the last call have been read
   if (lane == 31) warp_sums[w] = v;
   __syncthreads();
-  int before = 0, all = 0;
-  for (int i = 0; i < nw; ++i) {
-    if (i < w) before += warp_sums[i];
-    all += warp_sums[i];
+  int2 s = lane < nw ? warp_sums[lane] : make_int2(0, 0);
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int a = __shfl_up_sync(0xffffffffu, s.x, o), b = __shfl_up_sync(0xffffffffu, s.y, o);
+    if (lane >= o) s.x += a, s.y += b;
   }
-  *total = all;
-  return v + before;
+  const int before = w > 0 ? w - 1 : 0;
+  const int bx = __shfl_sync(0xffffffffu, s.x, before), by = __shfl_sync(0xffffffffu, s.y, before);
+  if (w > 0) v.x += bx, v.y += by;
+  *total = make_int2(__shfl_sync(0xffffffffu, s.x, 31), __shfl_sync(0xffffffffu, s.y, 31));
+  return v;
 }
 
 // Every CTA sums the lengths itself (R ints from L2; a scan shared through
-// memory would cost a second launch or a wait on another CTA) and then writes
-// its share of the rows and of the new table entries.  What may be updated in
-// place (the lengths, the stack's height) is written by the last CTA to
-// finish, when the others have read it.
+// memory would cost a second launch or a wait on another CTA), one scan over the
+// threads with a few requests each, and then writes its share of the rows and
+// of the new table entries.  What may be updated in place (the lengths, the
+// stack's height) is written by the last CTA to finish, when the others have
+// read it.
 __global__ void __launch_bounds__(1024) kv_plan_kernel(PlanArgs a) {
   extern __shared__ int sh[];
   int* cu = sh;                    // [R + 1] first new row of a request
-  int* pf = sh + a.R + 1;          // [R + 1] pages taken before it
-  __shared__ int sums[32], sums2[32];
+  int* pf = cu + a.R + 1;          // [R + 1] pages taken before it
+  int* len = pf + a.R + 1;         // [R] its past
+  __shared__ int2 sums[32];
   __shared__ int missing;
   __shared__ int last;
   const int tid = threadIdx.x, nt = blockDim.x;
+  const int height = min(at_least_0(*a.free_count), a.n_pages);
   if (tid == 0) missing = 0;
-  int base_n = 0, base_p = 0, over = 0;
-  for (int r0 = 0; r0 < a.R; r0 += nt) {
-    const int r = r0 + tid;
-    int n = 0, w = 0;
-    if (r < a.R) {
-      const int p = at_least_0(a.past[r]);
-      n = at_least_0(a.add[r]);
-      const int have = (p + a.P - 1) / a.P, full = (p + n + a.P - 1) / a.P;
-      w = min(full, a.max_pages) - min(have, a.max_pages);
-      over += full - have - w;     // pages beyond the table's width
-    }
-    int tn, tp;
-    const int sn = block_scan(n, sums, &tn), sp = block_scan(w, sums2, &tp);
-    if (r < a.R) {
-      cu[r] = base_n + sn - n;
-      pf[r] = base_p + sp - w;
-    }
-    base_n += tn;
-    base_p += tp;
-  }
-  if (tid == 0) {
-    cu[a.R] = base_n;
-    pf[a.R] = base_p;
+  for (int r = tid; r < a.R; r += nt) {
+    len[r] = at_least_0(a.past[r]);
+    cu[r] = at_least_0(a.add[r]);
   }
   __syncthreads();
+  const int own = (a.R + nt - 1) / nt, r0 = min(tid * own, a.R), r1 = min(r0 + own, a.R);
+  int over = 0;
+  int2 mine = make_int2(0, 0);
+  for (int r = r0; r < r1; ++r) {
+    const int have = (len[r] + a.P - 1) / a.P, full = (len[r] + cu[r] + a.P - 1) / a.P;
+    const int w = min(full, a.max_pages) - min(have, a.max_pages);
+    over += full - have - w;       // pages beyond the table's width
+    pf[r] = w;
+    mine.x += cu[r];
+    mine.y += w;
+  }
+  int2 all;
+  const int2 upto = block_scan(mine, sums, &all);
+  int2 at = make_int2(upto.x - mine.x, upto.y - mine.y);
+  for (int r = r0; r < r1; ++r) {
+    const int n = cu[r], w = pf[r];
+    cu[r] = at.x;
+    pf[r] = at.y;
+    at.x += n;
+    at.y += w;
+  }
+  if (tid == 0) {
+    cu[a.R] = all.x;
+    pf[a.R] = all.y;
+  }
   if (over) atomicAdd(&missing, over);
-  const int height = min(at_least_0(*a.free_count), a.n_pages);
-  const int taken = min(base_p, height);
+  __syncthreads();
+  const int rows = all.x, wanted = all.y, taken = min(wanted, height);
   const int t0 = blockIdx.x * nt + tid, step = gridDim.x * nt;
 
-  for (int j = t0; j < base_p; j += step) {
+  for (int j = t0; j < wanted; j += step) {
     const int r = last_not_above(pf, a.R, j);
-    const int have = (at_least_0(a.past[r]) + a.P - 1) / a.P;
-    const int at = height - 1 - j;
-    a.table[(long)r * a.max_pages + have + (j - pf[r])] = at >= 0 ? a.free_pages[at] : -1;
+    const int have = (len[r] + a.P - 1) / a.P, from = height - 1 - j;
+    a.table[(long)r * a.max_pages + have + (j - pf[r])] = from >= 0 ? a.free_pages[from] : -1;
   }
   for (int i = t0; i < a.N; i += step) {
     int slot = -1, pos = -1, req = -1;
-    if (i < base_n) {
+    if (i < rows) {
       req = last_not_above(cu, a.R, i);
-      const int p = at_least_0(a.past[req]);
+      const int p = len[req];
       pos = p + (i - cu[req]);
       const int have = (p + a.P - 1) / a.P, pi = pos / a.P;
       if (pi < a.max_pages) {
-        int page;
-        if (pi < have) page = a.table[(long)req * a.max_pages + pi];
-        else {
-          const int at = height - 1 - (pf[req] + pi - have);
-          page = at >= 0 ? a.free_pages[at] : -1;
-        }
+        const int from = height - 1 - (pf[req] + pi - have);
+        const int page = pi < have ? a.table[(long)req * a.max_pages + pi] : from >= 0 ? a.free_pages[from] : -1;
         if (page >= 0 && page < a.n_pages) slot = page * a.P + (pos - pi * a.P);
       }
     }
@@ -123,25 +131,22 @@ __global__ void __launch_bounds__(1024) kv_plan_kernel(PlanArgs a) {
     a.position[i] = pos;
     a.request[i] = req;
   }
-  if (blockIdx.x == 0)
-    for (int r = tid; r <= a.R; r += nt) a.cu[r] = cu[r];
+  for (int r = t0; r <= a.R; r += step) a.cu[r] = cu[r];
 
-  __syncthreads();
-  if (tid == 0) {
-    last = 1;
-    if (gridDim.x > 1) {
-      __threadfence();
+  if (gridDim.x > 1) {
+    __threadfence();
+    __syncthreads();
+    if (tid == 0) {
       last = atomicAdd(a.done, 1u) == gridDim.x - 1;
       if (last) *a.done = 0;
     }
+    __syncthreads();
+    if (!last) return;
   }
-  __syncthreads();
-  if (!last) return;
-  // lengths: past and its successor may be the same array, so each is read and written by one thread
-  for (int r = tid; r < a.R; r += nt) a.ctx_len[r] = at_least_0(a.past[r]) + (cu[r + 1] - cu[r]);
+  for (int r = tid; r < a.R; r += nt) a.ctx_len[r] = len[r] + (cu[r + 1] - cu[r]);
   if (tid == 0) {
     *a.free_out = height - taken;
-    *a.short_out = base_p - taken + missing;
+    *a.short_out = wanted - taken + missing;
   }
 }
 
@@ -153,16 +158,16 @@ __global__ void __launch_bounds__(1024) kv_release_kernel(const uint8_t* done, i
                                                           int32_t* table, int max_pages, int32_t* free_pages,
                                                           int n_pages, int32_t* free_count) {
   extern __shared__ int pf[];      // [R + 1] pages of ended requests before this one
-  __shared__ int sums[32];
+  __shared__ int2 sums[32];
   const int tid = threadIdx.x, nt = blockDim.x;
   int base = 0;
   for (int r0 = 0; r0 < R; r0 += nt) {
     const int r = r0 + tid;
     const int w = r < R && done[r] ? min((at_least_0(len[r]) + P - 1) / P, max_pages) : 0;
-    int total;
-    const int s = block_scan(w, sums, &total);
+    int2 total;
+    const int s = block_scan(make_int2(w, 0), sums, &total).x;
     if (r < R) pf[r] = base + s - w;
-    base += total;
+    base += total.x;
   }
   if (tid == 0) pf[R] = base;
   __syncthreads();
@@ -177,10 +182,10 @@ __global__ void __launch_bounds__(1024) kv_release_kernel(const uint8_t* done, i
       *e = -1;
       if (page >= n_pages) page = -1;
     }
-    int total;
-    const int s = block_scan(page >= 0, sums, &total);
+    int2 total;
+    const int s = block_scan(make_int2(page >= 0, 0), sums, &total).x;
     if (page >= 0 && height + s - 1 < n_pages) free_pages[height + s - 1] = page;
-    height = min(height + total, n_pages);
+    height = min(height + total.x, n_pages);
   }
   __syncthreads();
   if (tid == 0) *free_count = height;
@@ -574,7 +579,7 @@ int mxq_kv_plan(mxq_ctx c, const int32_t* past, const int32_t* add, size_t n_req
   const int threads = most <= 4096 ? 256 : 1024;
   size_t ctas = (most + threads - 1) / threads;
   if (ctas > (size_t)ws.sms) ctas = (size_t)ws.sms;
-  const size_t smem = 2 * (n_req + 1) * sizeof(int);
+  const size_t smem = (3 * n_req + 2) * sizeof(int);
   cudaError_t e = g_plan_attr.ensure(kv_plan_kernel, smem);
   if (e == cudaSuccess) {
     kv_plan_kernel<<<(unsigned)ctas, threads, smem, ctx_stream(c)>>>(a);

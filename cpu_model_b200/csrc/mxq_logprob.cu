@@ -31,7 +31,7 @@ __device__ __forceinline__ uint32_t order_key(float x) {
   const uint32_t b = __float_as_uint(x + 0.0f);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
-__device__ __forceinline__ float key_value(uint32_t k) {
+__device__ __forceinline__ float key_value(uint32_t k) {   // of an entry; of 0, a NaN
   if (k == 0xFFFFFFFFu) return __int_as_float(0x7fc00000);
   return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
 }
@@ -174,12 +174,12 @@ __device__ __forceinline__ void place_entries(const uint64_t* in, int n, int k, 
 // One row, `slices` CTAs (a cluster when there are several: few rows leave
 // SMs idle, and a row is long).  The top alternatives need no second pass
 // over the row: every group of THREADS / 32 threads knows its largest logit, so the
-// k-th largest of these 32 is a bound that at least k logits reach; only the threads
-// whose own maximum reaches it look through their part again.
+// k-th largest of these 32 is a bound that at least k logits reach; only the parts
+// of threads whose own maximum reaches it are looked through again.
 template <typename T, int THREADS>
 __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(LogprobArgs a) {
   __shared__ LogprobShared<THREADS> sh;
-  constexpr int kN = Vec<T>::kN, kUnroll = 4;
+  constexpr int kN = Vec<T>::kN, kAhead = 4;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int slices = a.slices, rank = slices > 1 ? (int)cluster_ctarank() : 0;
   const long row = blockIdx.x / slices;
@@ -194,26 +194,35 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(LogprobArgs a) 
       any = true;
     }
   }
+  // kAhead vectors on the way while the last ones are added, 8 values at a time
+  constexpr int kPair = 8 / kN;
   const int step = slices * THREADS;
+  uint4 w[kAhead];
   int i = rank * THREADS + tid;
-  for (; i + (kUnroll - 1) * step < rv.nv; i += kUnroll * step) {
-    uint4 w[kUnroll];
+  any = any || i < rv.nv;
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) w[u] = __ldg(rv.body + i + u * step);
-    any = true;
+  for (int u = 0; u < kAhead; ++u)
+    if (i + u * step < rv.nv) w[u] = __ldcs(rv.body + i + u * step);
+  for (; i + (kAhead - 1) * step < rv.nv; i += kAhead * step) {
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
+    for (int u = 0; u < kAhead; u += kPair) {
+      float v[8];
+#pragma unroll
+      for (int q = 0; q < kPair; ++q) {
+        unpack16<T>(w[u + q], v + q * kN);
+        const int nx = i + (kAhead + u + q) * step;
+        if (nx < rv.nv) w[u + q] = __ldcs(rv.body + nx);
+      }
+      add_values(t, v);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u)
+    if (i + u * step < rv.nv) {
       float v[kN];
       unpack16<T>(w[u], v);
       add_values(t, v);
     }
-  }
-  for (; i < rv.nv; i += step) {
-    float v[kN];
-    unpack16<T>(__ldg(rv.body + i), v);
-    add_values(t, v);
-    any = true;
-  }
   const uint32_t mine = any ? order_key(t.m) : 0u;
 
   // the slice's statistics
@@ -252,13 +261,26 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(LogprobArgs a) 
   if (a.k > 0) {
     const uint32_t least = sh.threshold;
     const bool odd = !(sh.all.s == sh.all.s);     // a NaN or +inf among them: the maxima are not to be trusted
-    if (!odd && any && mine >= least)
-      rv.template each<THREADS>(rank, slices, [&](float x, int id) {
-        if (order_key(x) >= least) {
+    if (!odd) {
+      // a warp looks through the part of each of its lanes in turn, a vector a lane
+      const float bound = key_value(least);       // least 0: a group without logits, every logit counts
+      auto test = [&](float x, int id) {
+        if (least == 0u || x >= bound) {
           const int at = atomicAdd(&sh.count, 1);
           if (at < kCandidates) sh.cand[at] = order_entry(x, id);
         }
-      });
+      };
+      for (uint32_t left = __ballot_sync(0xffffffffu, any && mine >= least); left; left &= left - 1) {
+        const int who = warp * 32 + __ffs((int)left) - 1;
+        if (rank == 0 && lane == 0 && who < rv.head + rv.tail) test(to_f32(rv.x[rv.end(who)]), rv.end(who));
+        for (int j = rank * THREADS + who + lane * step; j < rv.nv; j += 32 * step) {
+          float v[kN];
+          unpack16<T>(__ldg(rv.body + j), v);
+#pragma unroll
+          for (int e = 0; e < kN; ++e) test(v[e], rv.head + j * kN + e);
+        }
+      }
+    }
     __syncthreads();
     const int n = sh.count;
     if (!odd && n <= kCandidates) {
@@ -370,11 +392,14 @@ template <> __device__ __forceinline__ void store16(__half* p, const float* v) {
   *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-constexpr int kGradThreads = 256, kGradVecs = 4;
+constexpr int kGradThreads = 256;
+constexpr int kGradBatch = 4;      // vectors a thread has on the way
+constexpr int kGradLoops = 4;      // times that, a CTA
 
-// dx_j = dlogp (1[j = t] - p_j) - dentropy p_j (log p_j + H), element by
-// element: 16-byte stores at the gradient's alignment, the logits in 16 bytes
-// where they share it.
+// dx_j = dlogp (1[j = t] - p_j) - dentropy p_j (log p_j + H): 16-byte stores at
+// the gradient's alignment, the logits in 16 bytes where they share it.  The
+// target's element is the only one with a second term: the thread that has
+// it adds it there.
 template <typename T>
 __global__ void __launch_bounds__(kGradThreads) token_logprobs_grad_kernel(LogprobGradArgs a) {
   constexpr int kN = Vec<T>::kN;
@@ -382,6 +407,30 @@ __global__ void __launch_bounds__(kGradThreads) token_logprobs_grad_kernel(Logpr
   const int part = blockIdx.x % a.per_row, tid = threadIdx.x;
   const T* x = static_cast<const T*>(a.logits) + row * a.stride;
   T* g = static_cast<T*>(a.grad) + row * a.grad_stride;
+  const int mis = (int)((reinterpret_cast<uintptr_t>(g) & 15u) / sizeof(T));
+  const int head = min(mis ? kN - mis : 0, a.vocab);
+  const int nv = (a.vocab - head) / kN;
+  const bool same = (reinterpret_cast<uintptr_t>(x + head) & 15u) == 0;
+  const int per_cta = kGradThreads * kGradBatch * kGradLoops;
+  int first = part * per_cta + tid;
+  const int end = min(nv, (part + 1) * per_cta);
+  uint4 w[kGradBatch];
+  auto load_one = [&](int i, uint4& to) {
+    const T* from = x + head + (long)i * kN;
+    if (same) {
+      to = __ldcs(reinterpret_cast<const uint4*>(from));
+    } else if (sizeof(T) == 4) {
+      const uint32_t* p = reinterpret_cast<const uint32_t*>(from);
+      to = make_uint4(p[0], p[1], p[2], p[3]);
+    } else {
+      const uint16_t* p = reinterpret_cast<const uint16_t*>(from);
+      auto two = [&](int e) { return (uint32_t)p[e] | (uint32_t)p[e + 1] << 16; };
+      to = make_uint4(two(0), two(2), two(4 % kN), two(6 % kN));
+    }
+  };
+#pragma unroll
+  for (int u = 0; u < kGradBatch; ++u)
+    if (first + u * kGradThreads < end) load_one(first + u * kGradThreads, w[u]);
   const float lse = a.lse[row], h = a.entropy ? a.entropy[row] : 0.0f;
   // nothing but banned tokens, by -inf or by the lowest value of fp32 or bf16: log p
   // cannot be had from lse there, and no token is to be pushed anywhere
@@ -389,42 +438,41 @@ __global__ void __launch_bounds__(kGradThreads) token_logprobs_grad_kernel(Logpr
   const int tgt = a.target[row];
   const float dl = a.dlogp && tgt >= 0 && tgt < a.vocab && !empty ? a.dlogp[row] : 0.0f;
   const float de = a.dentropy && !empty ? a.dentropy[row] : 0.0f;
-  auto one = [&](float v, int id) {
-    const float lp = empty ? -1000.0f : v - lse;
-    const float p = exp2_approx(lp * kLog2e);
-    // -(dl + de (log p + H)) p, with a finite log p where p is 0
-    const float r = -p * fmaf(de, drop(lp) + h, dl);
-    return id == tgt ? dl + r : r;
+  const float c = -fmaf(de, h, dl);
+  auto one = [&](float y) {
+    const float lp = empty ? -1000.0f : y - lse;
+    // p (c - de log p), with a finite log p where p is 0
+    return exp2_approx(lp * kLog2e) * fmaf(-de, drop(lp), c);
   };
-  const int mis = (int)((reinterpret_cast<uintptr_t>(g) & 15u) / sizeof(T));
-  const int head = min(mis ? kN - mis : 0, a.vocab);
-  const int nv = (a.vocab - head) / kN;
-  const bool same = (reinterpret_cast<uintptr_t>(x + head) & 15u) == 0;
   if (part == 0) {
-    for (int i = tid; i < head; i += kGradThreads) g[i] = from_f32<T>(one(to_f32(x[i]), i));
-    for (int i = head + nv * kN + tid; i < a.vocab; i += kGradThreads) g[i] = from_f32<T>(one(to_f32(x[i]), i));
-  }
-  const int first = part * (kGradThreads * kGradVecs) + tid;
-  float v[kGradVecs][kN];
-#pragma unroll
-  for (int u = 0; u < kGradVecs; ++u) {
-    const int i = first + u * kGradThreads;
-    if (i < nv) {
-      if (same) {
-        unpack16<T>(*reinterpret_cast<const uint4*>(x + head + (long)i * kN), v[u]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < kN; ++e) v[u][e] = to_f32(x[head + (long)i * kN + e]);
-      }
+    for (int i = tid; i < head; i += kGradThreads) {
+      const float r = one(to_f32(x[i]));
+      g[i] = from_f32<T>(i == tgt ? dl + r : r);
+    }
+    for (int i = head + nv * kN + tid; i < a.vocab; i += kGradThreads) {
+      const float r = one(to_f32(x[i]));
+      g[i] = from_f32<T>(i == tgt ? dl + r : r);
     }
   }
+  const int tv = tgt >= head ? (tgt - head) / kN : -1;   // the target's vector, and its element
+  const int te = tv >= 0 ? (tgt - head) - tv * kN : 0;
+  for (; first < end; first += kGradThreads * kGradBatch) {
 #pragma unroll
-  for (int u = 0; u < kGradVecs; ++u) {
-    const int i = first + u * kGradThreads;
-    if (i < nv) {
+    for (int u = 0; u < kGradBatch; ++u) {
+      const int i = first + u * kGradThreads;
+      if (i >= end) break;
+      float v[kN];
+      unpack16<T>(w[u], v);
+      const int nx = i + kGradThreads * kGradBatch;
+      if (nx < end) load_one(nx, w[u]);
 #pragma unroll
-      for (int e = 0; e < kN; ++e) v[u][e] = one(v[u][e], head + i * kN + e);
-      store16(g + head + (long)i * kN, v[u]);
+      for (int e = 0; e < kN; ++e) v[e] = one(v[e]);
+      if (i == tv) {
+#pragma unroll
+        for (int e = 0; e < kN; ++e)
+          if (e == te) v[e] = dl + v[e];
+      }
+      store16(g + head + (long)i * kN, v);
     }
   }
 }
@@ -452,12 +500,12 @@ cudaError_t launch_logprobs(const LogprobArgs& a, cudaStream_t st) {
 template <typename T>
 cudaError_t run_logprobs(const LogprobArgs& a, cudaStream_t st) {
   // 512 threads only where each of them has two vectors of the row or more
-  return a.vocab / Vec<T>::kN < 1024 ? launch_logprobs<T, 128>(a, st) : launch_logprobs<T, 512>(a, st);
+  return a.vocab / Vec<T>::kN < 1024 ? launch_logprobs<T, 128>(a, st) : launch_logprobs<T, 256>(a, st);
 }
 
 template <typename T>
 cudaError_t run_grad(LogprobGradArgs a, cudaStream_t st) {
-  const int per_cta = kGradThreads * kGradVecs * Vec<T>::kN;
+  const int per_cta = kGradThreads * kGradBatch * kGradLoops * Vec<T>::kN;
   a.per_row = (a.vocab + per_cta - 1) / per_cta;
   token_logprobs_grad_kernel<T><<<(unsigned)((long)a.rows * a.per_row), kGradThreads, 0, st>>>(a);
   return cudaGetLastError();
