@@ -42,6 +42,7 @@ constexpr int kMaxRows = 16;             // query rows a unit
 constexpr int kStages = 2;               // blocks a warp has in its ring
 constexpr int kStart = 1;                // places a unit's start takes
 constexpr int kMinPiece = 2;             // places a piece at least
+constexpr size_t kPromptUnits = 32;      // units of the prompts' kernel that are worth it
 constexpr float kLn2 = 0.693147180559945f;
 
 struct AttnArgs {
@@ -52,6 +53,7 @@ struct AttnArgs {
   const int32_t *table, *ctx_len, *cu;
   long q_stride;
   int dtype, R, n, Hq, G, max_pages;
+  int few;                               // requests with more rows a K/V head are another kernel's
   float scale2;                          // scale * log2(e)
   uint32_t* counters;                    // [CTAs], zero
   float* warp_part;                      // [CTAs * warps][rows][D + 2]
@@ -560,7 +562,7 @@ __global__ void __launch_bounds__(Tile::kWarps * 32, 1) kv_attn_kernel(AttnArgs 
       long w = 0;
       if (r < a.R) {
         const int rows = (row_start(a, r + 1) - row_start(a, r)) * G, len = a.ctx_len[r];
-        if (rows > 0 && len > 0) w = (long)((rows + kRows - 1) / kRows) * (((len + 31) >> 5) + kStart) * Hkv;
+        if (rows > 0 && rows <= a.few && len > 0) w = (long)((rows + kRows - 1) / kRows) * (((len + 31) >> 5) + kStart) * Hkv;
       }
       long s = w;
       for (int o = 1; o < 32; o <<= 1) {
@@ -895,12 +897,23 @@ int mxq_kv_attention(mxq_ctx c, const mxq_kv_cache* cache, int dtype, const void
   int ctas = ws.sms;
   const int fit = (int)(kServeScratch / ((kMaxWarps + 2) * per));
   if (ctas > fit) ctas = fit;
-  if (ctas > (int)kServeCounters - 1) ctas = (int)kServeCounters - 1;
+  if (ctas > (int)kServeCounters - 3) ctas = (int)kServeCounters - 3;
   a.warp_part = reinterpret_cast<float*>(ws.scratch);
   a.cta_part = reinterpret_cast<float*>(ws.scratch + (size_t)ctas * kMaxWarps * per);
   const size_t rows = max_new * (size_t)a.G;
-  const cudaStream_t st = ctx_stream(c);
+  a.few = 1 << 30;
+  // Prompts' 16-bit rows go to the tensor cores' kernel where they fill at
+  // least kPromptUnits of its units: one SM with it is as fast as 6 with this
+  // one, but its units are not cut along the keys.
   const bool f32 = dtype == MXQ_DT_F32;
+  const size_t units = (n * (size_t)a.G + 255) / 256 * kv.heads;
+  if (!f32 && rows > kMaxRows && n_req <= (size_t)kPromptMaxRequests && units >= kPromptUnits) {
+    a.few = kMaxRows;
+    KvPromptArgs p{kv, q, out, lse, table, ctx_len, cu, (long)q_stride, (int)n_req, (int)n, a.Hq, a.G, a.max_pages,
+                   kMaxRows, dtype == MXQ_DT_BF16, a.scale2, ws.counters + kServeCounters - 2, ctx_status_word(c)};
+    if (int rc = serve_launched(c, launch_kv_prompt(p, ws.sms, ctx_stream(c)), "kv attention of prompts")) return rc;
+  }
+  const cudaStream_t st = ctx_stream(c);
   const cudaError_t e = kv.dim == 64 ? launch_rows<64>(a, rows, f32, ctas, st) : launch_rows<128>(a, rows, f32, ctas, st);
   return serve_launched(c, e, "kv attention");
 }

@@ -1,0 +1,670 @@
+// mxq_kvprompt.cu -- attention of prompts' rows (bf16 or fp16) over the paged
+// 8-bit K/V cache, on tcgen05 with S, P and O in tensor memory.
+//
+// A unit is 256 query rows of one request and K/V head (tokens x the head's
+// query heads), two M = 128 tiles A and B that share every K/V tile of 128 keys.
+// int8 values are exact in bf16 and fp16, so S = q K^T has fp32's accuracy and
+// the blocks' scales are applied where they cost nothing: K's in the fused
+// multiply-add before exp (a block is 32 columns of S, its scale a constant of
+// them), V's exactly in the conversion.  O += P V runs in fp16, whatever q's type
+// is: P keeps 11 bits there, and V' = q_v 2^(e_v - e + 8), e the unit's largest V
+// exponent, is exact while the unit's exponents lie within 2^32 of each other.
+// Where they do not, that unit's P and V are bf16, which takes any exponent (and leaves P 8
+// bits).
+//
+// Warps: 0-3 and 4-7 softmax of tile A and of B, a row a thread; 8-11 bring K
+// and V from their pages, int8 -> 16 bits, into two-stage rings in the 128-byte
+// swizzle; 12 issues the MMAs; 13-15 only fill its warpgroup, which gives its
+// registers to the softmax.  P takes the columns of S that it was made
+// from and is the MMA's A operand in tensor memory.  While one tile's softmax runs the
+// tensor cores work on the other's.  The rows of K are stored in the order of
+// V's 16-byte pieces (token 8 j + 2 c + b of a block is key 8 c + 2 j + b), so
+// neither is shuffled.  A row's maximum is only raised when it grows by 2^8:
+// P stays below 2^15, O is rescaled rarely, and the end result is the same.
+//
+// Units are handed out one by one, the longest of each request first.  Every
+// wait is bounded; one that gives up sets the status word and lets all roles
+// run to the end without waiting.
+#include "mxq_serve.cuh"
+
+namespace mxq {
+
+namespace {
+
+constexpr int kPromptThreads = 16 * 32;
+constexpr int kTileKeys = 128;
+constexpr uint32_t kColS = 0, kColO = 256;        // TMEM columns: S of A, S of B, O of A, O of B
+constexpr float kRise = 8.0f;                     // log2 of what P may grow by before O is rescaled
+constexpr float kLift = 7.0f;                     // P starts at 2^7: fp16 has it normal down to 2^-21 of the maximum
+constexpr float kLn2 = 0.693147180559945f;
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float neg_inf() { return -__int_as_float(0x7f800000); }
+
+#define MXQ_R4(a, i) "=r"(a[i]), "=r"(a[i + 1]), "=r"(a[i + 2]), "=r"(a[i + 3])
+#define MXQ_W4(a, i) "r"(a[i]), "r"(a[i + 1]), "r"(a[i + 2]), "r"(a[i + 3])
+__device__ __forceinline__ void tmem_ld32(uint32_t at, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,"
+      "%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : MXQ_R4(r, 0), MXQ_R4(r, 4), MXQ_R4(r, 8), MXQ_R4(r, 12), MXQ_R4(r, 16), MXQ_R4(r, 20), MXQ_R4(r, 24), MXQ_R4(r, 28)
+      : "r"(at));
+}
+__device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::MXQ_W4(r, 0), MXQ_W4(r, 4), MXQ_W4(r, 8), MXQ_W4(r, 12),
+      MXQ_W4(r, 16), MXQ_W4(r, 20), MXQ_W4(r, 24), MXQ_W4(r, 28), "r"(at)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&r)[32]) {   // the first 16
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::MXQ_W4(r, 0),
+      MXQ_W4(r, 4), MXQ_W4(r, 8), MXQ_W4(r, 12), "r"(at)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// D[tmem] (+)= A[tmem] * B[smem]^T, 16-bit inputs, fp32 accumulate.
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Instruction descriptor: bf16 or fp16 inputs, fp32 accumulator, both K-major.
+__host__ __device__ constexpr uint32_t idesc_16(bool bf16, int M, int N) {
+  return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+
+// Four int8 as two pairs of 16-bit numbers, exact.
+__device__ __forceinline__ void widen_bf16(uint32_t w, uint32_t& a, uint32_t& b) {
+  // 128 + the low seven bits, less 128 or (sign bit set) 256
+  const uint32_t x = __byte_perm(w, 0u, 0x4140), y = __byte_perm(w, 0u, 0x4342);
+  const uint32_t xp = (x & 0x007F007Fu) | 0x43004300u, xm = (x & 0x00800080u) | 0xC300C300u;
+  const uint32_t yp = (y & 0x007F007Fu) | 0x43004300u, ym = (y & 0x00800080u) | 0xC300C300u;
+  asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(a) : "r"(xp), "r"(xm));
+  asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(b) : "r"(yp), "r"(ym));
+}
+__device__ __forceinline__ void widen_f16(uint32_t w, uint32_t& a, uint32_t& b) {
+  // 1024 + (x + 128), less 1152
+  w ^= 0x80808080u;
+  const uint32_t x = __byte_perm(w, 0x64646464u, 0x4140), y = __byte_perm(w, 0x64646464u, 0x4342);
+  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(a) : "r"(x), "r"(0xE480E480u));
+  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(b) : "r"(y), "r"(0xE480E480u));
+}
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t s) {
+  uint32_t r;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(s));
+  return r;
+}
+
+// Where a token of a block is among the K tile's rows (and so S's columns).
+__host__ __device__ __forceinline__ int key_row(int t) { return ((t >> 1) & 3) * 8 + (t >> 3) * 2 + (t & 1); }
+__host__ __device__ __forceinline__ int key_token(int row) { return ((row & 7) >> 1) * 8 + (row >> 3) * 2 + (row & 1); }
+
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t s) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(s));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// 2^e in fp16 (0 below its smallest), e <= 8.
+__device__ __forceinline__ uint32_t f16_pow2(int e) {
+  return e >= -14 ? (uint32_t)(e + 15) << 10 : e >= -24 ? 1u << (e + 24) : 0u;
+}
+// 2^e in bf16 (0 below its smallest).
+__device__ __forceinline__ uint32_t bf16_pow2(int e) {
+  return e >= -126 ? (uint32_t)(e + 127) << 7 : e >= -133 ? 1u << (e + 133) : 0u;
+}
+
+template <int D>
+struct PromptShared {
+  static constexpr int kQTile = 128 * D * 2;      // one M tile of q, D / 64 halves of 128 rows x 128 bytes
+  static constexpr int kKTile = kTileKeys * D * 2;
+  static constexpr int kBytes = 2 * kQTile + 4 * kKTile;
+};
+
+struct Bars {
+  uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sfull[2], pfull[2], pvdone[2], qfull, drain;
+};
+
+// What the softmax needs of a K/V tile's blocks; four tiles deep: the
+// converters are at most two ahead of the softmax.
+struct TileNotes {
+  float f[4];                            // |scale| log2(e) 2^e_k, NaN for a NaN block
+  uint32_t flags;                        // bit i: block i holds keys; bit 4 + i: its V is NaN
+};
+
+template <int D, bool kBf16>
+__global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(KvPromptArgs a) {
+  using S = PromptShared<D>;
+  constexpr int kU = D / 16;             // 16-byte pieces of K, and of V, a converter thread has of a tile
+  extern __shared__ __align__(1024) uint8_t raw_sm[];
+  uint8_t* sm = raw_sm + ((1024u - (smem_u32(raw_sm) & 1023u)) & 1023u);
+  uint8_t* sq = sm;
+  uint8_t* sk = sm + 2 * S::kQTile;
+  uint8_t* sv = sk + 2 * S::kKTile;
+  int* s_sum = reinterpret_cast<int*>(sm + S::kBytes);             // [R + 1] units before a request
+  __shared__ Bars bar;
+  __shared__ TileNotes notes[4];
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_unit[2];
+  __shared__ int s_scan[kPromptThreads / 32];
+  __shared__ int s_top[4], s_low[4];     // largest and smallest V scale byte of the unit, by converter warp
+  __shared__ volatile int s_dead;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int G = a.G, Hkv = a.c.heads, nb = a.c.nb;
+  auto start_of = [&](int r) { return min(max(a.cu[r], 0), a.n); };
+
+  if (warp == 12) tmem_alloc(&s_tmem, 512);
+  if (tid == 0) {
+    s_dead = 0;
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bar.kfull[i], 4);
+      mbar_init(&bar.kempty[i], 1);
+      mbar_init(&bar.vfull[i], 4);
+      mbar_init(&bar.vempty[i], 1);
+      mbar_init(&bar.sfull[i], 1);
+      mbar_init(&bar.pfull[i], 4);
+      mbar_init(&bar.pvdone[i], 1);
+    }
+    mbar_init(&bar.qfull, 8);
+    mbar_init(&bar.drain, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  // ---- units of the requests that this kernel takes
+  {
+    int base = 0;
+    for (int r0 = 0; r0 < a.R; r0 += kPromptThreads) {
+      const int r = r0 + tid;
+      int w = 0;
+      if (r < a.R) {
+        const int rows = (start_of(r + 1) - start_of(r)) * G;
+        if (rows > a.few && a.ctx_len[r] > 0) w = (rows + 255) / 256 * Hkv;
+      }
+      int s = w;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= o) s += u;
+      }
+      __syncthreads();
+      if (lane == 31) s_scan[warp] = s;
+      __syncthreads();
+      int before = base;
+      for (int i = 0; i < kPromptThreads / 32; ++i) {
+        if (i < warp) before += s_scan[i];
+        base += s_scan[i];
+      }
+      if (r < a.R) s_sum[r] = before + s - w;
+    }
+    if (tid == 0) s_sum[a.R] = base;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s_tmem;
+  const int units = s_sum[a.R];
+
+  auto wait = [&](uint64_t* b, uint32_t parity) {
+    if (!s_dead && !mbar_wait(b, parity & 1u, a.status)) s_dead = 1;
+  };
+
+  // largest and smallest V scale byte of the unit (NaN and all-zero blocks aside)
+  auto v_range = [&]() {
+    return make_int2(max(max(s_top[0], s_top[1]), max(s_top[2], s_top[3])),
+                     min(min(s_low[0], s_low[1]), min(s_low[2], s_low[3])));
+  };
+  // ---- the next unit: what every role needs of it
+  struct Unit {
+    int req, row0, rows, ctx, head, first, past;
+    int see_a, see_b, na, nb, n;         // keys that the last row of A and of B sees, their K/V tiles, the larger
+  };
+  uint32_t round = 0;
+  auto next = [&](Unit& u) {
+    if (tid == 0) s_unit[round & 1] = (int)atomicAdd(a.next, 1u);
+    __syncwarp();
+    asm volatile("bar.sync 1, %0;" ::"n"(kPromptThreads) : "memory");   // the last unit is done with shared and tensor memory
+    const int id = s_unit[round & 1];
+    ++round;
+    if (id >= units) return false;
+    int x = 0, y = a.R;
+    while (y - x > 1) {
+      const int mid = (x + y) >> 1;
+      if (s_sum[mid] <= id) x = mid;
+      else y = mid;
+    }
+    u.req = x;
+    u.row0 = start_of(x);
+    u.rows = (start_of(x + 1) - u.row0) * G;
+    u.ctx = a.ctx_len[x];
+    const int in = id - s_sum[x], tiles = (u.rows + 255) / 256;
+    u.head = in % Hkv;
+    u.first = (tiles - 1 - in / Hkv) * 256;
+    u.past = u.ctx - u.rows / G;
+    const int end_a = min(u.first + 128, u.rows), end_b = min(u.first + 256, u.rows);
+    u.see_a = max(0, min(u.ctx, u.past + (end_a - 1) / G + 1));
+    u.see_b = end_b > u.first + 128 ? max(0, min(u.ctx, u.past + (end_b - 1) / G + 1)) : 0;
+    u.na = (u.see_a + kTileKeys - 1) / kTileKeys;
+    u.nb = (u.see_b + kTileKeys - 1) / kTileKeys;
+    u.n = max(u.na, u.nb);
+    return true;
+  };
+  // registers: 256 x 168 + 128 x 112 + 128 x 56 = 64512 of the launch's 512 x 128
+  uint32_t kt = 0;                       // K/V tiles of this CTA so far
+  Unit un;
+
+  if (warp < 8) {
+    // ---------------------------------------------------------- softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+    uint32_t ns = 0, npv = 0;            // S tiles taken, PV products awaited
+    for (; next(un); kt += un.n) {
+      const int x = warp >> 2, my = x ? un.nb : un.na;
+      const int row0 = un.row0, head = un.head, past = un.past;
+      const int row = un.first + x * 128 + (tid & 127);
+      const bool valid = row < un.rows;
+      const int t = row / G, h = head * G + (row - t * G);
+      // the row of q, 16 bytes at a time, into its swizzled place
+      {
+        uint8_t* to = sq + x * S::kQTile;
+        const uint16_t* from = static_cast<const uint16_t*>(a.q) + (long)(row0 + t) * a.q_stride + (long)h * D;
+        const uint32_t flip = a.scale2 < 0.0f ? 0x80008000u : 0u;
+#pragma unroll
+        for (int ch = 0; ch < D / 8; ++ch) {
+          uint4 w = make_uint4(0, 0, 0, 0);
+          if (valid) w = __ldg(reinterpret_cast<const uint4*>(from) + ch);
+          w.x ^= flip; w.y ^= flip; w.z ^= flip; w.w ^= flip;
+          *reinterpret_cast<uint4*>(to + (ch >> 3) * (128 * 128) + sw128_offset(tid & 127, ch & 7)) = w;
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar.qfull);
+      }
+      const uint32_t quad = (uint32_t)(warp & 3) << 21;               // lane 32 * (warp % 4) of tensor memory
+      const uint32_t ts = tmem + quad + kColS + x * 128, to = tmem + quad + kColO + x * 128;
+      const int last = valid ? past + t : -1;
+      float m = neg_inf(), l = 0.0f, unscale = 1.0f;
+      bool half = true;
+      for (int j = 0; j < my; ++j) {
+        wait(&bar.sfull[x], ns & 1);
+        ++ns;
+        tc_fence_after();
+        const TileNotes nt = notes[(kt + j) & 3];
+        const bool cut = __any_sync(0xffffffffu, j * kTileKeys + kTileKeys - 1 > last) || (nt.flags & 15u) != 15u;
+        // a column of block k is seen
+        auto seen = [&](int k, int c) {
+          return j * kTileKeys + k * 32 + key_token(c) <= last && (nt.flags >> k & 1u);
+        };
+        float top = neg_inf();
+#pragma unroll
+        for (int k = 0; k < 4; k += 2) {
+          uint32_t s0[32], s1[32];
+          tmem_ld32(ts + k * 32, s0);
+          tmem_ld32(ts + k * 32 + 32, s1);
+          tmem_ld_wait();
+          float u0 = neg_inf(), u1 = neg_inf();
+          if (cut) {
+#pragma unroll
+            for (int c = 0; c < 32; ++c) {
+              if (seen(k, c)) u0 = fmaxf(u0, __uint_as_float(s0[c]));
+              if (seen(k + 1, c)) u1 = fmaxf(u1, __uint_as_float(s1[c]));
+            }
+          } else {
+            float v0 = u0, v1 = u1;
+#pragma unroll
+            for (int c = 0; c < 32; c += 4) {
+              u0 = fmaxf(fmaxf(u0, __uint_as_float(s0[c])), __uint_as_float(s0[c + 1]));
+              v0 = fmaxf(fmaxf(v0, __uint_as_float(s0[c + 2])), __uint_as_float(s0[c + 3]));
+              u1 = fmaxf(fmaxf(u1, __uint_as_float(s1[c])), __uint_as_float(s1[c + 1]));
+              v1 = fmaxf(fmaxf(v1, __uint_as_float(s1[c + 2])), __uint_as_float(s1[c + 3]));
+            }
+            u0 = fmaxf(u0, v0);
+            u1 = fmaxf(u1, v1);
+          }
+          if (u0 > neg_inf()) top = fmaxf(top, u0 * nt.f[k]);
+          if (u1 > neg_inf()) top = fmaxf(top, u1 * nt.f[k + 1]);
+        }
+        const bool raise = top > (m == neg_inf() ? m : m + kRise);
+        if (__any_sync(0xffffffffu, raise)) {
+          const float mn = raise ? top : m;
+          const float alpha = m == neg_inf() || !raise ? 1.0f : ex2(m - mn);   // a row without keys so far has O = 0
+          l *= alpha;
+          m = mn;
+          if (j > 0) {
+            wait(&bar.pvdone[x], npv & 1);       // the product before this one
+            tc_fence_after();
+#pragma unroll
+            for (int k = 0; k < D / 32; ++k) {
+              uint32_t r[32];
+              tmem_ld32(to + k * 32, r);
+              tmem_ld_wait();
+#pragma unroll
+              for (int c = 0; c < 32; ++c) r[c] = __float_as_uint(__uint_as_float(r[c]) * alpha);
+              tmem_st32(to + k * 32, r);
+            }
+            tmem_st_wait();
+          }
+        }
+        if (j > 0) ++npv;
+        const float base = m == neg_inf() ? 0.0f : m - kLift;
+        if (j == 0) {
+          wait(&bar.vfull[kt & 1], kt >> 1);     // the unit's V exponents are known
+          const int2 e = v_range();
+          half = e.x - e.y <= 32;
+          unscale = pow2_exact(e.x - 127 - 8);
+        }
+        uint32_t s[2][32];
+        tmem_ld32(ts, s[0]);
+        tmem_ld_wait();
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (k < 3) tmem_ld32(ts + (k + 1) * 32, s[(k + 1) & 1]);
+          float part = 0.0f;
+          const float f = nt.f[k];
+#pragma unroll
+          for (int c = 0; c < 32; c += 2) {
+            float p0 = ex2(fmaf(__uint_as_float(s[k & 1][c]), f, -base));
+            float p1 = ex2(fmaf(__uint_as_float(s[k & 1][c + 1]), f, -base));
+            if (cut) {
+              if (!seen(k, c)) p0 = 0.0f;
+              if (!seen(k, c + 1)) p1 = 0.0f;
+            }
+            part += p0 + p1;
+            s[k & 1][c / 2] = half ? pack_f16(p0, p1) : pack_bf16(p0, p1);
+          }
+          l += nt.flags >> (4 + k) & 1u && part > 0.0f ? __int_as_float(0x7fc00000) : part;
+          if (k < 3) tmem_ld_wait();             // columns 32 (k + 1) .. are read: P's may be written over S
+          tmem_st16(ts + k * 16, s[k & 1]);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar.pfull[x]);
+      }
+      if (my > 0) {
+        wait(&bar.pvdone[x], npv & 1);
+        ++npv;
+        tc_fence_after();
+      }
+      const float inv = l == 0.0f ? 0.0f : unscale / l;
+      const long at = (long)(row0 + t) * a.Hq + h;
+#pragma unroll
+      for (int k = 0; k < D / 32; ++k) {
+        uint32_t r[32];
+        if (my > 0) {
+          tmem_ld32(to + k * 32, r);
+          tmem_ld_wait();
+        }
+        if (valid) {
+          uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + at * D + k * 32);
+#pragma unroll
+          for (int c = 0; c < 32; c += 8) {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float y0 = my > 0 ? __uint_as_float(r[c + 2 * e]) * inv : 0.0f;
+              const float y1 = my > 0 ? __uint_as_float(r[c + 2 * e + 1]) * inv : 0.0f;
+              w[e] = kBf16 ? pack_bf16(y0, y1) : pack_f16(y0, y1);
+            }
+            dst[c / 8] = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+      }
+      if (valid && a.lse) a.lse[at] = l == 0.0f ? neg_inf() : (m - kLift) * kLn2 + logf(l);
+      tc_fence_before();                         // O may be written over after the next unit's barrier
+    }
+  } else if (warp < 12) {
+    // ------------------------------------------------------- converters
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
+    for (; next(un); kt += un.n) {
+      const int w = warp - 8, ct = tid - 256, req = un.req, head = un.head, n = un.n;
+      const int nblk = (max(un.see_a, un.see_b) + 31) >> 5;
+      // lanes 0-3: block 4 j + lane of tile j and its scales
+      auto look = [&](int j, long& pl, uint32_t& sc) {
+        pl = -1;
+        sc = 0;
+        const int b = 4 * j + lane, pg = b / nb;
+        if (lane < 4 && b < nblk && pg < a.max_pages) {
+          const int page = a.table[(long)req * a.max_pages + pg];
+          if (page >= 0 && page < a.c.n_pages) {
+            pl = kv_block(a.c, page, head, b - pg * nb);
+            sc = (uint32_t)a.c.ks[pl] | (uint32_t)a.c.vs[pl] << 8;
+          }
+        }
+      };
+      uint4 kr[kU], vr[kU];
+      auto load_k = [&](long pl) {
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+          const int piece = u * 128 + ct, key = piece / (D / 16);
+          const long at = __shfl_sync(0xffffffffu, pl, key >> 5);
+          kr[u] = make_uint4(0, 0, 0, 0);
+          if (at >= 0) kr[u] = __ldg(reinterpret_cast<const uint4*>(a.c.k + at * (32 * D) + (key & 31) * D) + piece % (D / 16));
+        }
+      };
+      const int vc = lane & 3, vkb = (lane >> 2) & 1, vpr = lane >> 3;
+      auto load_v = [&](long pl) {
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+          const int pair = (u >> 1) * 16 + w * 4 + vpr;
+          const long at = __shfl_sync(0xffffffffu, pl, (u & 1) * 2 + vkb);
+          vr[u] = make_uint4(0, 0, 0, 0);
+          if (at >= 0) vr[u] = __ldg(reinterpret_cast<const uint4*>(a.c.v + at * (32 * D)) + pair * 4 + vc);
+        }
+      };
+      long pl, pl_next;
+      uint32_t sc, sc_next;
+      look(0, pl, sc);
+      if (n > 0) {
+        load_k(pl);
+        load_v(pl);
+      }
+      look(1, pl_next, sc_next);
+      {
+        int top = 1, low = 254;
+        for (int b = ct; b < nblk; b += 128) {
+          const int pg = b / nb, page = pg < a.max_pages ? a.table[(long)req * a.max_pages + pg] : -1;
+          if (page >= 0 && page < a.c.n_pages) {
+            const int v = a.c.vs[kv_block(a.c, page, head, b - pg * nb)];
+            if (v > 0 && v < 255) top = max(top, v), low = min(low, v);
+          }
+        }
+        top = __reduce_max_sync(0xffffffffu, top);
+        low = __reduce_min_sync(0xffffffffu, low);
+        if (lane == 0) s_top[w] = top, s_low[w] = low;
+        asm volatile("bar.sync 2, 128;" ::: "memory");
+      }
+      const int2 range = v_range();
+      const bool half = range.x - range.y <= 32;
+      for (int j = 0; j < n; ++j) {
+        const uint32_t g = kt + j;
+        const int st = g & 1;
+        if (w == 0 && lane < 4) {
+          const uint32_t ks = sc & 0xFF;
+          notes[g & 3].f[lane] = pl < 0 ? 0.0f : e8m0_to_float(ks) * fabsf(a.scale2);
+        }
+        const uint32_t there = __ballot_sync(0xffffffffu, lane < 4 && pl >= 0);
+        const uint32_t vnan = __ballot_sync(0xffffffffu, lane < 4 && pl >= 0 && (sc >> 8) == 255u);
+        if (w == 0 && lane == 0) notes[g & 3].flags = there | vnan << 4;
+        if (g >= 2) wait(&bar.kempty[st], (g >> 1) - 1);
+        uint8_t* kd = sk + st * S::kKTile;
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+          const int piece = u * 128 + ct, key = piece / (D / 16), col = piece % (D / 16);
+          const int row = (key & ~31) + key_row(key & 31);
+          uint32_t o[8];
+          const uint32_t q[4] = {kr[u].x, kr[u].y, kr[u].z, kr[u].w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if (kBf16) widen_bf16(q[e], o[2 * e], o[2 * e + 1]);
+            else widen_f16(q[e], o[2 * e], o[2 * e + 1]);
+          }
+          uint8_t* part = kd + (col >> 2) * (128 * 128);
+          const uint4 lo = make_uint4(o[0], o[1], o[2], o[3]), hi = make_uint4(o[4], o[5], o[6], o[7]);
+          // lanes 4-7 of a quarter warp are in the other half (D = 128): they
+          // store their pieces in the other order, so that the eight hit all banks
+          const int swap = D == 128 ? (lane >> 2) & 1 : 0;
+          *reinterpret_cast<uint4*>(part + sw128_offset(row, (col & 3) * 2 + swap)) = swap ? hi : lo;
+          *reinterpret_cast<uint4*>(part + sw128_offset(row, (col & 3) * 2 + 1 - swap)) = swap ? lo : hi;
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar.kfull[st]);
+        if (j + 1 < n) load_k(pl_next);
+        if (g >= 2) wait(&bar.vempty[st], (g >> 1) - 1);
+        uint8_t* vd = sv + st * S::kKTile;
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+          const int pair = (u >> 1) * 16 + w * 4 + vpr, kb = (u & 1) * 2 + vkb;
+          const int vs = (int)(__shfl_sync(0xffffffffu, sc, kb) >> 8);
+          // the block's step as a pair; a NaN block's values count as 0 (its rows' sums become NaN instead)
+          uint32_t one = 0;
+          if (vs != 255) one = half ? f16_pow2(vs - range.x + 8) : bf16_pow2(vs - range.x + 8);
+          one |= one << 16;
+          uint32_t o[8];
+          const uint32_t q[4] = {vr[u].x, vr[u].y, vr[u].z, vr[u].w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if (half) {
+              widen_f16(q[e], o[2 * e], o[2 * e + 1]);
+              o[2 * e] = mul_f16x2(o[2 * e], one);
+              o[2 * e + 1] = mul_f16x2(o[2 * e + 1], one);
+            } else {
+              widen_bf16(q[e], o[2 * e], o[2 * e + 1]);
+              o[2 * e] = mul_bf16x2(o[2 * e], one);
+              o[2 * e + 1] = mul_bf16x2(o[2 * e + 1], one);
+            }
+          }
+          uint8_t* part = vd + (kb >> 1) * (D * 128);
+          const int ch = (kb & 1) * 4 + vc;
+          *reinterpret_cast<uint4*>(part + sw128_offset(2 * pair, ch)) = make_uint4(o[0], o[1], o[2], o[3]);
+          *reinterpret_cast<uint4*>(part + sw128_offset(2 * pair + 1, ch)) = make_uint4(o[4], o[5], o[6], o[7]);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar.vfull[st]);
+        if (j + 1 < n) load_v(pl_next);
+        pl = pl_next;
+        sc = sc_next;
+        look(j + 2, pl_next, sc_next);
+      }
+    }
+  } else {
+    // ----------------------------------------------------------- issuer
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    uint32_t pa = 0, pb = 0;             // P tiles taken of A, of B
+    for (; next(un); kt += un.n) {
+      if (warp != 12 || lane != 0) continue;
+      const int na = un.na, ntb = un.nb, n = un.n;
+      constexpr uint32_t kIdS = idesc_16(kBf16, 128, kTileKeys);
+      uint32_t id_o = idesc_16(false, 128, D);
+      const uint64_t dq = sw128_kmajor_desc(smem_u32(sq)), dk = sw128_kmajor_desc(smem_u32(sk)),
+                     dv = sw128_kmajor_desc(smem_u32(sv));
+      // S of tile x: D / 16 steps of 32 bytes, a 16 KB half every four
+      auto scores = [&](int x, int st) {
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t at = (k >> 2) * (128 * 128) + (k & 3) * 32;
+          mma_bf16_ss(tmem + kColS + x * 128, dq + ((x * S::kQTile + at) >> 4), dk + ((st * S::kKTile + at) >> 4), kIdS, k > 0);
+        }
+        mma_commit(&bar.sfull[x]);
+      };
+      auto product = [&](int x, int st, bool more) {
+#pragma unroll
+        for (int k = 0; k < kTileKeys / 16; ++k) {
+          const uint32_t at = (k >> 2) * (D * 128) + (k & 3) * 32;
+          mma_ts(tmem + kColO + x * 128, tmem + kColS + x * 128 + k * 8, dv + ((st * S::kKTile + at) >> 4), id_o, more || k > 0);
+        }
+        mma_commit(&bar.pvdone[x]);
+      };
+      wait(&bar.qfull, round - 1);
+      if (n > 0) {
+        wait(&bar.kfull[kt & 1], kt >> 1);
+        tc_fence_after();
+        if (!s_dead) {
+          if (0 < na) scores(0, kt & 1);
+          if (0 < ntb) scores(1, kt & 1);
+          mma_commit(&bar.kempty[kt & 1]);
+        }
+      }
+      for (int j = 0; j < n; ++j) {
+        const uint32_t g = kt + j;
+        const int st = g & 1, sn = st ^ 1;
+        wait(&bar.vfull[st], g >> 1);
+        if (j == 0) {
+          const int2 e = v_range();
+          if (e.x - e.y > 32) id_o = idesc_16(true, 128, D);
+        }
+        // A's product, A's next S; B's product, B's next S: one tile's softmax
+        // has the time of the other's MMAs
+        if (j < na) {
+          wait(&bar.pfull[0], pa++);
+          tc_fence_after();
+          if (!s_dead) product(0, st, j > 0);
+        }
+        if (j + 1 < n) {
+          wait(&bar.kfull[sn], (g + 1) >> 1);
+          tc_fence_after();
+          if (j + 1 < na && !s_dead) scores(0, sn);
+        }
+        if (j < ntb) {
+          wait(&bar.pfull[1], pb++);
+          tc_fence_after();
+          if (!s_dead) product(1, st, j > 0);
+        }
+        if (!s_dead) mma_commit(&bar.vempty[st]);
+        if (j + 1 < n && !s_dead) {
+          if (j + 1 < ntb) scores(1, sn);
+          mma_commit(&bar.kempty[sn]);
+        }
+      }
+    }
+  }
+  // ---- every MMA has ended before tensor memory goes
+  if (warp == 12 && lane == 0) {
+    mma_commit(&bar.drain);
+    (void)mbar_wait(&bar.drain, 0, a.status);
+  }
+  __syncwarp();
+  __syncthreads();
+  if (warp == 12) tmem_dealloc(tmem, 512);
+  // the last CTA leaves the counters at zero
+  if (tid == 0 && atomicAdd(a.next + 1, 1u) == gridDim.x - 1) {
+    a.next[0] = 0;
+    a.next[1] = 0;
+  }
+}
+
+template <int D, bool kBf16>
+cudaError_t launch(const KvPromptArgs& a, int ctas, cudaStream_t st) {
+  static SmemAttr attr;
+  const size_t smem = 1024 + PromptShared<D>::kBytes + ((size_t)a.R + 1) * 4;
+  const cudaError_t e = attr.ensure(kv_prompt_kernel<D, kBf16>, smem);
+  if (e != cudaSuccess) return e;
+  kv_prompt_kernel<D, kBf16><<<(unsigned)ctas, kPromptThreads, smem, st>>>(a);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_kv_prompt(const KvPromptArgs& a, int ctas, cudaStream_t st) {
+  if (a.c.dim == 64) return a.bf16 ? launch<64, true>(a, ctas, st) : launch<64, false>(a, ctas, st);
+  return a.bf16 ? launch<128, true>(a, ctas, st) : launch<128, false>(a, ctas, st);
+}
+
+}  // namespace mxq

@@ -17,6 +17,23 @@ struct KvView {
   int n_pages, page, nb, heads, dim;   // nb: blocks a page
 };
 
+// Attention of the requests with more than `few` query rows a K/V head, 16-bit
+// rows (mxq_kvprompt.cu).
+struct KvPromptArgs {
+  KvView c;
+  const void* q;
+  void* out;
+  float* lse;
+  const int32_t *table, *ctx_len, *cu;
+  long q_stride;
+  int R, n, Hq, G, max_pages, few, bf16;
+  float scale2;                          // scale * log2(e)
+  uint32_t* next;                        // two words, zero
+  uint32_t* status;
+};
+constexpr int kPromptMaxRequests = 4096;
+cudaError_t launch_kv_prompt(const KvPromptArgs& a, int ctas, cudaStream_t st);
+
 // Index of (page, head, block of the page): its scale's place; its values
 // start at 32 * dim times it.
 __device__ __forceinline__ long kv_block(const KvView& c, int page, int head, int b) {

@@ -165,6 +165,101 @@ def test_prompt_chunks(ctx):
         Case([(700, 300), (1000, 512), (130, 130)], 2, 4, 128, 64, dtype, seed=8).check(ctx)
 
 
+# enough rows for the tensor cores' kernel (32 units of 256 rows a K/V head)
+LONG = {
+    "even": (8, 4, [(512, 512), (1024, 512)]),
+    "ragged": (8, 4, [(700, 300), (1000, 513), (130, 130), (40, 3), (900, 1), (5, 5), (0, 0), (300, 17)]),
+    "heads": (32, 1, [(300, 300), (77, 33)]),
+    "odd_group": (4, 5, [(1500, 500), (333, 299)]),
+    "wide_group": (2, 16, [(257, 257), (500, 129)]),
+    "one_page": (16, 8, [(64, 64), (31, 31), (128, 127)])}
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D,P", [(128, 64), (64, 32), (128, 256)])
+@pytest.mark.parametrize("name", sorted(LONG))
+def test_prompts_on_the_tensor_cores(ctx, name, D, P, dtype):
+    Hkv, G, spans = LONG[name]
+    Case(spans, Hkv, G, D, P, dtype, seed=31, extra_rows=2, q_pad=64, wide=1).check(ctx)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_prompts_with_missing_pages_and_rows_without_keys(ctx, dtype):
+    c = Case([(600, 400), (300, 500), (256, 256), (0, 90), (-3, 40)], 8, 4, 128, 32, dtype, seed=32)
+    c.table[0, 3] = -1
+    c.table[0, 18] = 10 ** 8
+    c.table[2, 0] = -1                               # the first rows see no key at all
+    c.table[2, 7] = -5
+    c.check(ctx)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_prompts_with_scales(ctx, dtype):
+    c = Case([(600, 600), (300, 200)], 8, 4, 64, 64, dtype, seed=33, spread=10)
+    c.check(ctx)
+    c.check(ctx, scale=0.0)
+    c.check(ctx, scale=-0.125)
+    c.vs[:, 1] = 0                                   # blocks of zeros have the smallest scale
+    c.v[:, 1] = 0
+    c.check(ctx)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_prompts_with_v_scales_too_far_apart_for_fp16(ctx, dtype):
+    """Exponents of V more than 2^32 apart: that unit's P is bf16, 8 bits (2^-9
+    in the 2-norm), beside the result's rounding."""
+    c = Case([(600, 600), (300, 200)], 8, 4, 128, 64, dtype, seed=40)
+    c.vs[:, 1, 1] -= 70                              # head 1: every other block tiny
+    c.vs[int(c.table[1, 0]), 2, :] = 250             # head 2 of request 1: two blocks huge
+    c.vs[int(c.table[1, 1]), 3, 0] = 1
+    out, lse = c.run(ctx)
+    want, wl = c.ref()
+    assert torch.isfinite(lse).all() and ((lse.double() - wl).abs() <= 5e-4).all()
+    tol = (TOL[dtype] ** 2 + 2.0 ** -18) ** 0.5
+    for h in range(8):
+        for a, b in ((0, 600), (600, 800)):
+            g, w = out[a:b, 4 * h:4 * h + 4].double(), want[a:b, 4 * h:4 * h + 4]
+            if dtype == torch.float16 and float(w.abs().max()) > 65504:
+                continue
+            assert float((g - w).norm() / w.norm()) <= tol, (h, a)
+
+
+def test_prompts_with_nan_in_masked_places(ctx):
+    c = Case([(512, 512)], 8, 8, 128, 128, torch.bfloat16, seed=34)
+    want, wl = c.ref()
+    pg = int(c.table[0, 2])                          # keys 256 .. 383
+    c.ks[pg, 0, 1] = 255                             # head 0: keys 288 .. 319
+    c.vs[pg, 1, 3] = 255                             # head 1: keys 352 .. 383
+    out, lse = c.run(ctx)
+    tol = TOL[torch.bfloat16]
+    near = lambda a, b: float((a.double() - b).norm() / b.norm()) <= tol
+    assert near(out[:288, :8], want[:288, :8]) and torch.isnan(out[319:, :8]).all() and torch.isnan(lse[319:, :8]).all()
+    assert near(out[:352, 8:16], want[:352, 8:16]) and torch.isnan(out[384:, 8:16]).all()
+    assert near(out[:, 16:], want[:, 16:])
+    c = Case([(512, 512)], 8, 8, 128, 128, torch.float16, seed=35)
+    want, _ = c.ref()
+    c.q[100, 5, 7] = float("inf")
+    out, lse = c.run(ctx)
+    assert torch.isnan(out[100, 5]).all()
+    keep = torch.ones((512, 64), dtype=torch.bool)
+    keep[100, 5] = False
+    assert float((out[keep].double() - want[keep]).norm() / want[keep].norm()) <= TOL[torch.float16]
+
+
+def test_prompts_repeat_and_run_on_two_streams(ctx):
+    cs = [Case([(900, 700), (1300, 1000 + i)], 8, 2, 128, 64, torch.bfloat16, seed=36 + i) for i in range(2)]
+    want = [c.run(ctx) for c in cs]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    outs = []
+    for i in range(12):
+        with torch.cuda.stream(streams[i % 2]):
+            outs.append(cs[i % 2].run(ctx))
+    torch.cuda.synchronize()
+    for i, (o, l) in enumerate(outs):
+        assert torch.equal(o, want[i % 2][0]) and torch.equal(l, want[i % 2][1])
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_rows_that_see_nothing(ctx, dtype):
     """No new rows, no context, fewer keys than rows, rows of no request,
