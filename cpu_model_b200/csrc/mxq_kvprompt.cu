@@ -3,14 +3,15 @@
 //
 // A unit is 256 query rows of one request and K/V head (tokens x the head's
 // query heads), two M = 128 tiles A and B that share every K/V tile of 128 keys.
-// int8 values are exact in bf16 and fp16, so S = q K^T has fp32's accuracy and
-// the blocks' scales are applied where they cost nothing: K's in the fused
-// multiply-add before exp (a block is 32 columns of S, its scale a constant of
-// them), V's exactly in the conversion.  O += P V runs in fp16, whatever q's type
-// is: P keeps 11 bits there, and V' = q_v 2^(e_v - e + 8), e the unit's largest V
-// exponent, is exact while the unit's exponents lie within 2^32 of each other.
-// Where they do not, that unit's P and V are bf16, which takes any exponent (and leaves P 8
-// bits).
+// int8 values are exact in fp16, and so is a bf16 row of q once a power of two
+// has brought its largest element to 2^15 (what fp16 then rounds is below 2^-39 of it),
+// so S = q K^T has fp32's accuracy.  The scales are applied where they cost
+// nothing: K's and the row's in the fused multiply-add before exp (a block is 32 columns of
+// S, its scale a constant of them), V's exactly in the conversion.  O += P V
+// runs in fp16 too: P keeps 11 bits, and V' = q_v 2^(e_v - e + 8), e the unit's
+// largest V exponent, is exact while the unit's exponents lie within 2^32 of
+// each other.  Where they do not, that unit's P and V are bf16, which takes any
+// exponent (and leaves P 8 bits).
 //
 // Warps: 0-3 and 4-7 softmax of tile A and of B, a row a thread; 8-11 bring K
 // and V from their pages, int8 -> 16 bits, into two-stage rings in the 128-byte
@@ -109,6 +110,30 @@ __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t s) {
 __host__ __device__ __forceinline__ int key_row(int t) { return ((t >> 1) & 3) * 8 + (t >> 3) * 2 + (t & 1); }
 __host__ __device__ __forceinline__ int key_token(int row) { return ((row & 7) >> 1) * 8 + (row >> 3) * 2 + (row & 1); }
 
+// Pairs of fp32 in one instruction, and the largest of three.
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& x, float& y) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 __device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t s) {
   uint32_t r;
   asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(s));
@@ -147,7 +172,7 @@ struct Bars {
 // What the softmax needs of a K/V tile's blocks; four tiles deep: the
 // converters are at most two ahead of the softmax.
 struct TileNotes {
-  float f[4];                            // |scale| log2(e) 2^e_k, NaN for a NaN block
+  float f[4];                            // 2^e_k, NaN for a NaN block
   uint32_t flags;                        // bit i: block i holds keys; bit 4 + i: its V is NaN
 };
 
@@ -279,17 +304,39 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(KvPromptAr
       const int row = un.first + x * 128 + (tid & 127);
       const bool valid = row < un.rows;
       const int t = row / G, h = head * G + (row - t * G);
-      // the row of q, 16 bytes at a time, into its swizzled place
+      // the row of q, 16 bytes at a time, into its swizzled place, as fp16
+      float qs = fabsf(a.scale2);                // |scale| log2(e) over the row's power of two
       {
         uint8_t* to = sq + x * S::kQTile;
         const uint16_t* from = static_cast<const uint16_t*>(a.q) + (long)(row0 + t) * a.q_stride + (long)h * D;
         const uint32_t flip = a.scale2 < 0.0f ? 0x80008000u : 0u;
-#pragma unroll
+        float lift = 1.0f;
+        if (kBf16) {
+          uint32_t top = 0;                      // the largest |q|, as bf16 bits
+          if (valid)
+#pragma unroll 4
+            for (int ch = 0; ch < D / 8; ++ch) {
+              const uint4 w = __ldg(reinterpret_cast<const uint4*>(from) + ch);
+              const uint32_t m0 = __vmaxu2(w.x & 0x7FFF7FFFu, w.y & 0x7FFF7FFFu);
+              top = __vmaxu2(top, __vmaxu2(m0, __vmaxu2(w.z & 0x7FFF7FFFu, w.w & 0x7FFF7FFFu)));
+            }
+          top = max(top & 0xFFFFu, top >> 16);
+          const int e = (int)(top >> 7);         // its exponent field; 255: inf or NaN
+          // 2^(14 - exponent): |q| below 2^15
+          const int up = min(14 - (e - 127), 126);
+          lift = e == 255 ? 0.0f : __int_as_float((up + 127) << 23);
+          qs = e == 255 ? __int_as_float(0x7fc00000) : qs * __int_as_float((127 - up) << 23);
+        }
+#pragma unroll 4
         for (int ch = 0; ch < D / 8; ++ch) {
           uint4 w = make_uint4(0, 0, 0, 0);
-          if (valid) w = __ldg(reinterpret_cast<const uint4*>(from) + ch);
-          w.x ^= flip; w.y ^= flip; w.z ^= flip; w.w ^= flip;
-          *reinterpret_cast<uint4*>(to + (ch >> 3) * (128 * 128) + sw128_offset(tid & 127, ch & 7)) = w;
+          if (valid && lift != 0.0f) w = __ldg(reinterpret_cast<const uint4*>(from) + ch);
+          uint32_t v[4] = {w.x ^ flip, w.y ^ flip, w.z ^ flip, w.w ^ flip};
+          if (kBf16)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              v[e] = pack_f16(__uint_as_float(v[e] << 16) * lift, __uint_as_float(v[e] & 0xFFFF0000u) * lift);
+          *reinterpret_cast<uint4*>(to + (ch >> 3) * (128 * 128) + sw128_offset(tid & 127, ch & 7)) = make_uint4(v[0], v[1], v[2], v[3]);
         }
         fence_proxy_async_smem();
         __syncwarp();
@@ -305,39 +352,44 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(KvPromptAr
         ++ns;
         tc_fence_after();
         const TileNotes nt = notes[(kt + j) & 3];
-        const bool cut = __any_sync(0xffffffffu, j * kTileKeys + kTileKeys - 1 > last) || (nt.flags & 15u) != 15u;
-        // a column of block k is seen
-        auto seen = [&](int k, int c) {
-          return j * kTileKeys + k * 32 + key_token(c) <= last && (nt.flags >> k & 1u);
-        };
+        const int limit = last - j * kTileKeys;  // keys 0 .. limit of the tile are seen
+        const bool cut = __any_sync(0xffffffffu, limit < kTileKeys - 1) || (nt.flags & 15u) != 15u;
+        float f[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) f[k] = nt.f[k] * qs;
+        // tokens of block k that are seen: below this
+        auto seen_below = [&](int k) { return nt.flags >> k & 1u ? limit - k * 32 + 1 : 0; };
         float top = neg_inf();
+        if (!cut) {
 #pragma unroll
-        for (int k = 0; k < 4; k += 2) {
-          uint32_t s0[32], s1[32];
-          tmem_ld32(ts + k * 32, s0);
-          tmem_ld32(ts + k * 32 + 32, s1);
-          tmem_ld_wait();
-          float u0 = neg_inf(), u1 = neg_inf();
-          if (cut) {
-#pragma unroll
-            for (int c = 0; c < 32; ++c) {
-              if (seen(k, c)) u0 = fmaxf(u0, __uint_as_float(s0[c]));
-              if (seen(k + 1, c)) u1 = fmaxf(u1, __uint_as_float(s1[c]));
-            }
-          } else {
-            float v0 = u0, v1 = u1;
+          for (int k = 0; k < 4; k += 2) {
+            uint32_t s0[32], s1[32];
+            tmem_ld32(ts + k * 32, s0);
+            tmem_ld32(ts + k * 32 + 32, s1);
+            tmem_ld_wait();
+            float u[2] = {neg_inf(), neg_inf()}, v[2] = {neg_inf(), neg_inf()};
 #pragma unroll
             for (int c = 0; c < 32; c += 4) {
-              u0 = fmaxf(fmaxf(u0, __uint_as_float(s0[c])), __uint_as_float(s0[c + 1]));
-              v0 = fmaxf(fmaxf(v0, __uint_as_float(s0[c + 2])), __uint_as_float(s0[c + 3]));
-              u1 = fmaxf(fmaxf(u1, __uint_as_float(s1[c])), __uint_as_float(s1[c + 1]));
-              v1 = fmaxf(fmaxf(v1, __uint_as_float(s1[c + 2])), __uint_as_float(s1[c + 3]));
+              u[0] = max3(u[0], __uint_as_float(s0[c]), __uint_as_float(s0[c + 1]));
+              v[0] = max3(v[0], __uint_as_float(s0[c + 2]), __uint_as_float(s0[c + 3]));
+              u[1] = max3(u[1], __uint_as_float(s1[c]), __uint_as_float(s1[c + 1]));
+              v[1] = max3(v[1], __uint_as_float(s1[c + 2]), __uint_as_float(s1[c + 3]));
             }
-            u0 = fmaxf(u0, v0);
-            u1 = fmaxf(u1, v1);
+            top = max3(top, fmaxf(u[0], v[0]) * f[k], fmaxf(u[1], v[1]) * f[k + 1]);
           }
-          if (u0 > neg_inf()) top = fmaxf(top, u0 * nt.f[k]);
-          if (u1 > neg_inf()) top = fmaxf(top, u1 * nt.f[k + 1]);
+        } else {
+#pragma unroll 1
+          for (int k = 0; k < 4; ++k) {
+            uint32_t s0[32];
+            tmem_ld32(ts + k * 32, s0);
+            tmem_ld_wait();
+            const int below = seen_below(k);
+            float u = neg_inf();
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+              if (key_token(c) < below) u = fmaxf(u, __uint_as_float(s0[c]));
+            if (u > neg_inf()) top = fmaxf(top, u * (k == 0 ? f[0] : k == 1 ? f[1] : k == 2 ? f[2] : f[3]));
+          }
         }
         const bool raise = top > (m == neg_inf() ? m : m + kRise);
         if (__any_sync(0xffffffffu, raise)) {
@@ -348,7 +400,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(KvPromptAr
           if (j > 0) {
             wait(&bar.pvdone[x], npv & 1);       // the product before this one
             tc_fence_after();
-#pragma unroll
+#pragma unroll 1
             for (int k = 0; k < D / 32; ++k) {
               uint32_t r[32];
               tmem_ld32(to + k * 32, r);
@@ -368,28 +420,56 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(KvPromptAr
           half = e.x - e.y <= 32;
           unscale = pow2_exact(e.x - 127 - 8);
         }
-        uint32_t s[2][32];
-        tmem_ld32(ts, s[0]);
-        tmem_ld_wait();
+        const bool odd = (nt.flags >> 4) != 0u;  // a NaN block of V
+        if (!cut && half && !odd) {
+          // the common tile: two blocks at a time, the next one on its way
+          const uint64_t nb2 = pair(-base, -base);
+          uint64_t part = 0;
+          uint32_t s0[32], s1[32];
+          tmem_ld32(ts, s0);
+          tmem_ld_wait();
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          if (k < 3) tmem_ld32(ts + (k + 1) * 32, s[(k + 1) & 1]);
-          float part = 0.0f;
-          const float f = nt.f[k];
+          for (int k = 0; k < 4; ++k) {
+            uint32_t(&s)[32] = k & 1 ? s1 : s0;
+            uint32_t(&next_s)[32] = k & 1 ? s0 : s1;
+            if (k < 3) tmem_ld32(ts + (k + 1) * 32, next_s);
+            const uint64_t f2 = pair(f[k], f[k]);
 #pragma unroll
-          for (int c = 0; c < 32; c += 2) {
-            float p0 = ex2(fmaf(__uint_as_float(s[k & 1][c]), f, -base));
-            float p1 = ex2(fmaf(__uint_as_float(s[k & 1][c + 1]), f, -base));
-            if (cut) {
-              if (!seen(k, c)) p0 = 0.0f;
-              if (!seen(k, c + 1)) p1 = 0.0f;
+            for (int c = 0; c < 32; c += 2) {
+              float p0, p1;
+              unpair(fma2(pair(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), f2, nb2), p0, p1);
+              p0 = ex2(p0);
+              p1 = ex2(p1);
+              part = add2(part, pair(p0, p1));
+              s[c / 2] = pack_f16(p0, p1);
             }
-            part += p0 + p1;
-            s[k & 1][c / 2] = half ? pack_f16(p0, p1) : pack_bf16(p0, p1);
+            if (k < 3) tmem_ld_wait();           // columns 32 (k + 1) .. are read: P's may be written over S
+            tmem_st16(ts + k * 16, s);
           }
-          l += nt.flags >> (4 + k) & 1u && part > 0.0f ? __int_as_float(0x7fc00000) : part;
-          if (k < 3) tmem_ld_wait();             // columns 32 (k + 1) .. are read: P's may be written over S
-          tmem_st16(ts + k * 16, s[k & 1]);
+          float p0, p1;
+          unpair(part, p0, p1);
+          l += p0 + p1;
+        } else {
+#pragma unroll 1
+          for (int k = 0; k < 4; ++k) {
+            uint32_t s[32];
+            tmem_ld32(ts + k * 32, s);
+            tmem_ld_wait();
+            const float fk = k == 0 ? f[0] : k == 1 ? f[1] : k == 2 ? f[2] : f[3];
+            const int below = seen_below(k);
+            float part = 0.0f;
+#pragma unroll
+            for (int c = 0; c < 32; c += 2) {
+              float p0 = ex2(fmaf(__uint_as_float(s[c]), fk, -base));
+              float p1 = ex2(fmaf(__uint_as_float(s[c + 1]), fk, -base));
+              if (key_token(c) >= below) p0 = 0.0f;
+              if (key_token(c + 1) >= below) p1 = 0.0f;
+              part += p0 + p1;
+              s[c / 2] = half ? pack_f16(p0, p1) : pack_bf16(p0, p1);
+            }
+            l += (nt.flags >> (4 + k) & 1u) && part > 0.0f ? __int_as_float(0x7fc00000) : part;
+            tmem_st16(ts + k * 16, s);
+          }
         }
         tmem_st_wait();
         tc_fence_before();
@@ -403,7 +483,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(KvPromptAr
       }
       const float inv = l == 0.0f ? 0.0f : unscale / l;
       const long at = (long)(row0 + t) * a.Hq + h;
-#pragma unroll
+#pragma unroll 1
       for (int k = 0; k < D / 32; ++k) {
         uint32_t r[32];
         if (my > 0) {
@@ -448,25 +528,46 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(KvPromptAr
         }
       };
       uint4 kr[kU], vr[kU];
+      // K: piece u of a thread is key u * kKeys + ct / (D / 16) of the tile, 16 dimensions of it
+      constexpr int kKeys = 128 / (D / 16);      // keys a pass of the 128 threads: 16 or 32
+      const int kq = ct / (D / 16), col = ct % (D / 16);
       auto load_k = [&](long pl) {
 #pragma unroll
-        for (int u = 0; u < kU; ++u) {
-          const int piece = u * 128 + ct, key = piece / (D / 16);
-          const long at = __shfl_sync(0xffffffffu, pl, key >> 5);
-          kr[u] = make_uint4(0, 0, 0, 0);
-          if (at >= 0) kr[u] = __ldg(reinterpret_cast<const uint4*>(a.c.k + at * (32 * D) + (key & 31) * D) + piece % (D / 16));
+        for (int b = 0; b < 4; ++b) {
+          const long at = __shfl_sync(0xffffffffu, pl, b);
+          const uint4* from = reinterpret_cast<const uint4*>(a.c.k + at * (32 * D)) + kq * (D / 16) + col;
+#pragma unroll
+          for (int u = 0; u < 32 / kKeys; ++u) {
+            uint4 w = make_uint4(0, 0, 0, 0);
+            if (at >= 0) w = __ldg(from + u * 128);
+            kr[b * (32 / kKeys) + u] = w;
+          }
         }
       };
+      // V: piece u is dimensions 2 pair, 2 pair + 1 of block kb, tokens of group vc
       const int vc = lane & 3, vkb = (lane >> 2) & 1, vpr = lane >> 3;
       auto load_v = [&](long pl) {
 #pragma unroll
-        for (int u = 0; u < kU; ++u) {
-          const int pair = (u >> 1) * 16 + w * 4 + vpr;
-          const long at = __shfl_sync(0xffffffffu, pl, (u & 1) * 2 + vkb);
-          vr[u] = make_uint4(0, 0, 0, 0);
-          if (at >= 0) vr[u] = __ldg(reinterpret_cast<const uint4*>(a.c.v + at * (32 * D)) + pair * 4 + vc);
+        for (int q = 0; q < 2; ++q) {
+          const long at = __shfl_sync(0xffffffffu, pl, q * 2 + vkb);
+          const uint4* from = reinterpret_cast<const uint4*>(a.c.v + at * (32 * D)) + (w * 4 + vpr) * 4 + vc;
+#pragma unroll
+          for (int u = 0; u < kU / 2; ++u) {
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if (at >= 0) x = __ldg(from + u * 64);
+            vr[u * 2 + q] = x;
+          }
         }
       };
+      // places in the tiles: a K key of token t is row key_row(t) of its block;
+      // passes of 16 keys alternate between rows r and r + 4 of the swizzle
+      const int krow = key_row(kq);
+      const uint32_t kcol = (uint32_t)(col >> 2) * (128 * 128);
+      // lanes 4-7 of a quarter warp are in the other half (D = 128): they store
+      // their pieces in the other order, so that the eight hit all banks
+      const uint32_t swap = D == 128 ? (lane >> 2) & 1 : 0;
+      const uint32_t kat = kcol + sw128_offset(krow, (col & 3) * 2 + swap), kat2 = kcol + sw128_offset(krow, (col & 3) * 2 + 1 - swap);
+      const uint32_t vat = sw128_offset(2 * (w * 4 + vpr), vkb * 4 + vc), vat2 = sw128_offset(2 * (w * 4 + vpr) + 1, vkb * 4 + vc);
       long pl, pl_next;
       uint32_t sc, sc_next;
       look(0, pl, sc);
@@ -496,7 +597,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(KvPromptAr
         const int st = g & 1;
         if (w == 0 && lane < 4) {
           const uint32_t ks = sc & 0xFF;
-          notes[g & 3].f[lane] = pl < 0 ? 0.0f : e8m0_to_float(ks) * fabsf(a.scale2);
+          notes[g & 3].f[lane] = pl < 0 ? 0.0f : e8m0_to_float(ks);
         }
         const uint32_t there = __ballot_sync(0xffffffffu, lane < 4 && pl >= 0);
         const uint32_t vnan = __ballot_sync(0xffffffffu, lane < 4 && pl >= 0 && (sc >> 8) == 255u);
@@ -505,22 +606,17 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(KvPromptAr
         uint8_t* kd = sk + st * S::kKTile;
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
-          const int piece = u * 128 + ct, key = piece / (D / 16), col = piece % (D / 16);
-          const int row = (key & ~31) + key_row(key & 31);
           uint32_t o[8];
-          const uint32_t q[4] = {kr[u].x, kr[u].y, kr[u].z, kr[u].w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if (kBf16) widen_bf16(q[e], o[2 * e], o[2 * e + 1]);
-            else widen_f16(q[e], o[2 * e], o[2 * e + 1]);
-          }
-          uint8_t* part = kd + (col >> 2) * (128 * 128);
+          widen_f16(kr[u].x, o[0], o[1]);
+          widen_f16(kr[u].y, o[2], o[3]);
+          widen_f16(kr[u].z, o[4], o[5]);
+          widen_f16(kr[u].w, o[6], o[7]);
           const uint4 lo = make_uint4(o[0], o[1], o[2], o[3]), hi = make_uint4(o[4], o[5], o[6], o[7]);
-          // lanes 4-7 of a quarter warp are in the other half (D = 128): they
-          // store their pieces in the other order, so that the eight hit all banks
-          const int swap = D == 128 ? (lane >> 2) & 1 : 0;
-          *reinterpret_cast<uint4*>(part + sw128_offset(row, (col & 3) * 2 + swap)) = swap ? hi : lo;
-          *reinterpret_cast<uint4*>(part + sw128_offset(row, (col & 3) * 2 + 1 - swap)) = swap ? lo : hi;
+          // 16 keys a pass: 4 rows on (which turns bit 2 of the swizzle), then the next block
+          const uint32_t up = kKeys == 32 ? u * 32 * 128 : (u >> 1) * 32 * 128 + (u & 1) * 4 * 128;
+          const uint32_t turn = kKeys == 32 ? 0 : (u & 1) * 64;
+          *reinterpret_cast<uint4*>(kd + (kat ^ turn) + up) = swap ? hi : lo;
+          *reinterpret_cast<uint4*>(kd + (kat2 ^ turn) + up) = swap ? lo : hi;
         }
         fence_proxy_async_smem();
         __syncwarp();
@@ -528,32 +624,43 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(KvPromptAr
         if (j + 1 < n) load_k(pl_next);
         if (g >= 2) wait(&bar.vempty[st], (g >> 1) - 1);
         uint8_t* vd = sv + st * S::kKTile;
+        // the blocks' steps as pairs; a NaN block's values count as 0 (its rows' sums become NaN instead)
+        uint32_t step[2];
 #pragma unroll
-        for (int u = 0; u < kU; ++u) {
-          const int pair = (u >> 1) * 16 + w * 4 + vpr, kb = (u & 1) * 2 + vkb;
-          const int vs = (int)(__shfl_sync(0xffffffffu, sc, kb) >> 8);
-          // the block's step as a pair; a NaN block's values count as 0 (its rows' sums become NaN instead)
-          uint32_t one = 0;
-          if (vs != 255) one = half ? f16_pow2(vs - range.x + 8) : bf16_pow2(vs - range.x + 8);
-          one |= one << 16;
-          uint32_t o[8];
-          const uint32_t q[4] = {vr[u].x, vr[u].y, vr[u].z, vr[u].w};
+        for (int q = 0; q < 2; ++q) {
+          const int vs = (int)(__shfl_sync(0xffffffffu, sc, q * 2 + vkb) >> 8);
+          step[q] = vs == 255 ? 0u : half ? f16_pow2(vs - range.x + 8) : bf16_pow2(vs - range.x + 8);
+          step[q] |= step[q] << 16;
+        }
+        auto store_v = [&](int u, const uint32_t (&o)[8]) {
+          const uint32_t up = (u & 1) * (D * 128) + (u >> 1) * 32 * 128;
+          *reinterpret_cast<uint4*>(vd + vat + up) = make_uint4(o[0], o[1], o[2], o[3]);
+          *reinterpret_cast<uint4*>(vd + vat2 + up) = make_uint4(o[4], o[5], o[6], o[7]);
+        };
+        if (half) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if (half) {
-              widen_f16(q[e], o[2 * e], o[2 * e + 1]);
-              o[2 * e] = mul_f16x2(o[2 * e], one);
-              o[2 * e + 1] = mul_f16x2(o[2 * e + 1], one);
-            } else {
-              widen_bf16(q[e], o[2 * e], o[2 * e + 1]);
-              o[2 * e] = mul_bf16x2(o[2 * e], one);
-              o[2 * e + 1] = mul_bf16x2(o[2 * e + 1], one);
-            }
+          for (int u = 0; u < kU; ++u) {
+            uint32_t o[8];
+            widen_f16(vr[u].x, o[0], o[1]);
+            widen_f16(vr[u].y, o[2], o[3]);
+            widen_f16(vr[u].z, o[4], o[5]);
+            widen_f16(vr[u].w, o[6], o[7]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[e] = mul_f16x2(o[e], step[u & 1]);
+            store_v(u, o);
           }
-          uint8_t* part = vd + (kb >> 1) * (D * 128);
-          const int ch = (kb & 1) * 4 + vc;
-          *reinterpret_cast<uint4*>(part + sw128_offset(2 * pair, ch)) = make_uint4(o[0], o[1], o[2], o[3]);
-          *reinterpret_cast<uint4*>(part + sw128_offset(2 * pair + 1, ch)) = make_uint4(o[4], o[5], o[6], o[7]);
+        } else {
+#pragma unroll
+          for (int u = 0; u < kU; ++u) {
+            uint32_t o[8];
+            widen_bf16(vr[u].x, o[0], o[1]);
+            widen_bf16(vr[u].y, o[2], o[3]);
+            widen_bf16(vr[u].z, o[4], o[5]);
+            widen_bf16(vr[u].w, o[6], o[7]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[e] = mul_bf16x2(o[e], step[u & 1]);
+            store_v(u, o);
+          }
         }
         fence_proxy_async_smem();
         __syncwarp();
@@ -571,7 +678,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(KvPromptAr
     for (; next(un); kt += un.n) {
       if (warp != 12 || lane != 0) continue;
       const int na = un.na, ntb = un.nb, n = un.n;
-      constexpr uint32_t kIdS = idesc_16(kBf16, 128, kTileKeys);
+      constexpr uint32_t kIdS = idesc_16(false, 128, kTileKeys);
       uint32_t id_o = idesc_16(false, 128, D);
       const uint64_t dq = sw128_kmajor_desc(smem_u32(sq)), dk = sw128_kmajor_desc(smem_u32(sk)),
                      dv = sw128_kmajor_desc(smem_u32(sv));
