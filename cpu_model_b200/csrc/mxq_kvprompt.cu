@@ -676,28 +676,39 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(KvPromptAr
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     uint32_t pa = 0, pb = 0;             // P tiles taken of A, of B
     for (; next(un); kt += un.n) {
-      if (warp != 12 || lane != 0) continue;
+      if (warp != 12) continue;
       const int na = un.na, ntb = un.nb, n = un.n;
       constexpr uint32_t kIdS = idesc_16(false, 128, kTileKeys);
       uint32_t id_o = idesc_16(false, 128, D);
       const uint64_t dq = sw128_kmajor_desc(smem_u32(sq)), dk = sw128_kmajor_desc(smem_u32(sk)),
                      dv = sw128_kmajor_desc(smem_u32(sv));
+      // The warp stays together and elects the lane that issues.
       // S of tile x: D / 16 steps of 32 bytes, a 16 KB half every four
       auto scores = [&](int x, int st) {
+        if (elect_one()) {
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t at = (k >> 2) * (128 * 128) + (k & 3) * 32;
-          mma_bf16_ss(tmem + kColS + x * 128, dq + ((x * S::kQTile + at) >> 4), dk + ((st * S::kKTile + at) >> 4), kIdS, k > 0);
+          for (int k = 0; k < D / 16; ++k) {
+            const uint32_t at = (k >> 2) * (128 * 128) + (k & 3) * 32;
+            mma_bf16_ss(tmem + kColS + x * 128, dq + ((x * S::kQTile + at) >> 4), dk + ((st * S::kKTile + at) >> 4), kIdS, k > 0);
+          }
+          mma_commit(&bar.sfull[x]);
         }
-        mma_commit(&bar.sfull[x]);
+        __syncwarp();
       };
       auto product = [&](int x, int st, bool more) {
+        if (elect_one()) {
 #pragma unroll
-        for (int k = 0; k < kTileKeys / 16; ++k) {
-          const uint32_t at = (k >> 2) * (D * 128) + (k & 3) * 32;
-          mma_ts(tmem + kColO + x * 128, tmem + kColS + x * 128 + k * 8, dv + ((st * S::kKTile + at) >> 4), id_o, more || k > 0);
+          for (int k = 0; k < kTileKeys / 16; ++k) {
+            const uint32_t at = (k >> 2) * (D * 128) + (k & 3) * 32;
+            mma_ts(tmem + kColO + x * 128, tmem + kColS + x * 128 + k * 8, dv + ((st * S::kKTile + at) >> 4), id_o, more || k > 0);
+          }
+          mma_commit(&bar.pvdone[x]);
         }
-        mma_commit(&bar.pvdone[x]);
+        __syncwarp();
+      };
+      auto release = [&](uint64_t* b) {
+        if (elect_one()) mma_commit(b);
+        __syncwarp();
       };
       wait(&bar.qfull, round - 1);
       if (n > 0) {
@@ -706,7 +717,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(KvPromptAr
         if (!s_dead) {
           if (0 < na) scores(0, kt & 1);
           if (0 < ntb) scores(1, kt & 1);
-          mma_commit(&bar.kempty[kt & 1]);
+          release(&bar.kempty[kt & 1]);
         }
       }
       for (int j = 0; j < n; ++j) {
@@ -734,20 +745,19 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(KvPromptAr
           tc_fence_after();
           if (!s_dead) product(1, st, j > 0);
         }
-        if (!s_dead) mma_commit(&bar.vempty[st]);
+        if (!s_dead) release(&bar.vempty[st]);
         if (j + 1 < n && !s_dead) {
           if (j + 1 < ntb) scores(1, sn);
-          mma_commit(&bar.kempty[sn]);
+          release(&bar.kempty[sn]);
         }
       }
     }
   }
   // ---- every MMA has ended before tensor memory goes
-  if (warp == 12 && lane == 0) {
-    mma_commit(&bar.drain);
+  if (warp == 12) {
+    if (elect_one()) mma_commit(&bar.drain);
     (void)mbar_wait(&bar.drain, 0, a.status);
   }
-  __syncwarp();
   __syncthreads();
   if (warp == 12) tmem_dealloc(tmem, 512);
   // the last CTA leaves the counters at zero
