@@ -2,7 +2,8 @@
 // 8-bit K/V cache, on tcgen05 with S, P and O in tensor memory.
 //
 // A unit is 256 query rows of one request and K/V head (tokens x the head's
-// query heads), two M = 128 tiles A and B that share every K/V tile of 128 keys.
+// query heads), two M = 128 tiles A and B that share every K/V tile of 128 keys
+// and take it in two steps of 64.
 // int8 values are exact in fp16, and so is a bf16 row of q once a power of two
 // has brought its largest element to 2^15 (what fp16 then rounds is below 2^-39 of it),
 // so S = q K^T has fp32's accuracy.  The scales are applied where they cost
@@ -15,10 +16,11 @@
 //
 // Warps: 0-3 and 4-7 softmax of tile A and of B, a row a thread; 8-11 bring K
 // and V from their pages, int8 -> 16 bits, into two-stage rings in the 128-byte
-// swizzle; 12 issues the MMAs; 13-15 only fill its warpgroup, which gives its
-// registers to the softmax.  P takes the columns of S that it was made
-// from and is the MMA's A operand in tensor memory.  While one tile's softmax runs the
-// tensor cores work on the other's.  The rows of K are stored in the order of
+// swizzle; 12 issues the MMAs of A and 13 those of B (an MMA takes a warp about
+// 100 cycles to issue, more than the tensor cores need for it); 14 and 15 only fill the
+// warpgroup, which gives its registers to the softmax.  P takes the columns of S that it was made
+// from and is the MMA's A operand in tensor memory.  S of a step has one of two
+// places, so the next step's is there when the softmax gets to it.  The rows of K are stored in the order of
 // V's 16-byte pieces (token 8 j + 2 c + b of a block is key 8 c + 2 j + b), so
 // neither is shuffled.  A row's maximum is only raised when it grows by 2^8:
 // P stays below 2^15, O is rescaled rarely, and the end result is the same.
@@ -33,7 +35,8 @@ namespace mxq {
 namespace {
 
 constexpr int kPromptThreads = 16 * 32;
-constexpr int kTileKeys = 128;
+constexpr int kTileKeys = 128;                    // keys the converters bring at a time
+constexpr int kStepKeys = 64;                     // keys of an S
 constexpr uint32_t kColS = 0, kColO = 256;        // TMEM columns: S of A, S of B, O of A, O of B
 constexpr float kRise = 8.0f;                     // log2 of what P may grow by before O is rescaled
 constexpr float kLift = 7.0f;                     // P starts at 2^7: fp16 has it normal down to 2^-21 of the maximum
@@ -62,7 +65,13 @@ __device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t (&r)[32]) 
       MXQ_W4(r, 16), MXQ_W4(r, 20), MXQ_W4(r, 24), MXQ_W4(r, 28), "r"(at)
       : "memory");
 }
-__device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&r)[32]) {   // the first 16
+__device__ __forceinline__ void tmem_ld16(uint32_t at, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : MXQ_R4(r, 0), MXQ_R4(r, 4), MXQ_R4(r, 8), MXQ_R4(r, 12)
+      : "r"(at));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::MXQ_W4(r, 0),
       MXQ_W4(r, 4), MXQ_W4(r, 8), MXQ_W4(r, 12), "r"(at)
@@ -105,6 +114,8 @@ __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t s) {
   asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(s));
   return r;
 }
+
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
 
 // Where a token of a block is among the K tile's rows (and so S's columns).
 __host__ __device__ __forceinline__ int key_row(int t) { return ((t >> 1) & 3) * 8 + (t >> 3) * 2 + (t & 1); }
@@ -166,7 +177,8 @@ struct PromptShared {
 };
 
 struct Bars {
-  uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sfull[2], pfull[2], pvdone[2], qfull, drain;
+  uint64_t kfull[2], kempty[2], vfull[2], vempty[2], qfull[2], drain;
+  uint64_t sfull[2][2], pfull[2][2], pvdone[2][2];   // [A, B][place]: two steps may be under way
 };
 
 // What the softmax needs of a K/V tile's blocks; four tiles deep: the
@@ -202,15 +214,18 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(KvPromptAr
     s_dead = 0;
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bar.kfull[i], 4);
-      mbar_init(&bar.kempty[i], 1);
+      mbar_init(&bar.kempty[i], 2);
       mbar_init(&bar.vfull[i], 4);
-      mbar_init(&bar.vempty[i], 1);
-      mbar_init(&bar.sfull[i], 1);
-      mbar_init(&bar.pfull[i], 4);
-      mbar_init(&bar.pvdone[i], 1);
+      mbar_init(&bar.vempty[i], 2);
+      for (int b = 0; b < 2; ++b) {
+        mbar_init(&bar.pvdone[i][b], 1);
+        mbar_init(&bar.sfull[i][b], 1);
+        mbar_init(&bar.pfull[i][b], 4);
+      }
     }
-    mbar_init(&bar.qfull, 8);
-    mbar_init(&bar.drain, 1);
+    mbar_init(&bar.qfull[0], 4);
+    mbar_init(&bar.qfull[1], 4);
+    mbar_init(&bar.drain, 2);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   // ---- units of the requests that this kernel takes
@@ -258,7 +273,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(KvPromptAr
   // ---- the next unit: what every role needs of it
   struct Unit {
     int req, row0, rows, ctx, head, first, past;
-    int see_a, see_b, na, nb, n;         // keys that the last row of A and of B sees, their K/V tiles, the larger
+    int see_a, see_b, na, nb, n;         // keys that the last row of A and of B sees, their steps; K/V tiles
   };
   uint32_t round = 0;
   auto next = [&](Unit& u) {
@@ -285,9 +300,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(KvPromptAr
     const int end_a = min(u.first + 128, u.rows), end_b = min(u.first + 256, u.rows);
     u.see_a = max(0, min(u.ctx, u.past + (end_a - 1) / G + 1));
     u.see_b = end_b > u.first + 128 ? max(0, min(u.ctx, u.past + (end_b - 1) / G + 1)) : 0;
-    u.na = (u.see_a + kTileKeys - 1) / kTileKeys;
-    u.nb = (u.see_b + kTileKeys - 1) / kTileKeys;
-    u.n = max(u.na, u.nb);
+    u.na = (u.see_a + kStepKeys - 1) / kStepKeys;
+    u.nb = (u.see_b + kStepKeys - 1) / kStepKeys;
+    u.n = (max(u.na, u.nb) + 1) >> 1;
     return true;
   };
   // registers: 256 x 168 + 128 x 112 + 128 x 56 = 64512 of the launch's 512 x 128
@@ -297,7 +312,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(KvPromptAr
   if (warp < 8) {
     // ---------------------------------------------------------- softmax
     asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
-    uint32_t ns = 0, npv = 0;            // S tiles taken, PV products awaited
+    uint32_t taken0 = 0, taken1 = 0;     // S taken from each place, and so P left there
     for (; next(un); kt += un.n) {
       const int x = warp >> 2, my = x ? un.nb : un.na;
       const int row0 = un.row0, head = un.head, past = un.past;
@@ -340,57 +355,53 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(KvPromptAr
         }
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bar.qfull);
+        if (lane == 0) mbar_arrive(&bar.qfull[x]);
       }
       const uint32_t quad = (uint32_t)(warp & 3) << 21;               // lane 32 * (warp % 4) of tensor memory
       const uint32_t ts = tmem + quad + kColS + x * 128, to = tmem + quad + kColO + x * 128;
       const int last = valid ? past + t : -1;
       float m = neg_inf(), l = 0.0f, unscale = 1.0f;
       bool half = true;
+#pragma unroll 1
       for (int j = 0; j < my; ++j) {
-        wait(&bar.sfull[x], ns & 1);
-        ++ns;
+        const int place = j & 1;
+        const uint32_t tp = ts + place * 64;
+        const uint32_t before = place ? taken0 : taken1;               // P left in the other place
+        wait(&bar.sfull[x][place], place ? taken1 : taken0);
+        taken0 += place ^ 1;
+        taken1 += place;
         tc_fence_after();
-        const TileNotes nt = notes[(kt + j) & 3];
-        const int limit = last - j * kTileKeys;  // keys 0 .. limit of the tile are seen
-        const bool cut = __any_sync(0xffffffffu, limit < kTileKeys - 1) || (nt.flags & 15u) != 15u;
-        float f[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) f[k] = nt.f[k] * qs;
-        // tokens of block k that are seen: below this
-        auto seen_below = [&](int k) { return nt.flags >> k & 1u ? limit - k * 32 + 1 : 0; };
-        float top = neg_inf();
+        uint32_t s0[32], s1[32];
+        tmem_ld32(tp, s0);
+        tmem_ld32(tp + 32, s1);
+        const TileNotes& nt = notes[(kt + (j >> 1)) & 3];
+        const uint32_t flags = nt.flags >> (2 * place);                // bits 0, 1: keys; 4, 5: NaN in V
+        const float f0 = nt.f[2 * place] * qs, f1 = nt.f[2 * place + 1] * qs;
+        const int limit = last - j * kStepKeys;  // keys 0 .. limit of the step are seen
+        const bool cut = __any_sync(0xffffffffu, limit < kStepKeys - 1) || (flags & 3u) != 3u;
+        // tokens of its two blocks that are seen: below these
+        const int below0 = flags & 1u ? limit + 1 : 0, below1 = flags & 2u ? limit - 31 : 0;
+        tmem_ld_wait();
+        float u[4] = {neg_inf(), neg_inf(), neg_inf(), neg_inf()};
         if (!cut) {
 #pragma unroll
-          for (int k = 0; k < 4; k += 2) {
-            uint32_t s0[32], s1[32];
-            tmem_ld32(ts + k * 32, s0);
-            tmem_ld32(ts + k * 32 + 32, s1);
-            tmem_ld_wait();
-            float u[2] = {neg_inf(), neg_inf()}, v[2] = {neg_inf(), neg_inf()};
-#pragma unroll
-            for (int c = 0; c < 32; c += 4) {
-              u[0] = max3(u[0], __uint_as_float(s0[c]), __uint_as_float(s0[c + 1]));
-              v[0] = max3(v[0], __uint_as_float(s0[c + 2]), __uint_as_float(s0[c + 3]));
-              u[1] = max3(u[1], __uint_as_float(s1[c]), __uint_as_float(s1[c + 1]));
-              v[1] = max3(v[1], __uint_as_float(s1[c + 2]), __uint_as_float(s1[c + 3]));
-            }
-            top = max3(top, fmaxf(u[0], v[0]) * f[k], fmaxf(u[1], v[1]) * f[k + 1]);
+          for (int c = 0; c < 32; c += 4) {
+            u[0] = max3(u[0], __uint_as_float(s0[c]), __uint_as_float(s0[c + 1]));
+            u[1] = max3(u[1], __uint_as_float(s0[c + 2]), __uint_as_float(s0[c + 3]));
+            u[2] = max3(u[2], __uint_as_float(s1[c]), __uint_as_float(s1[c + 1]));
+            u[3] = max3(u[3], __uint_as_float(s1[c + 2]), __uint_as_float(s1[c + 3]));
           }
         } else {
-#pragma unroll 1
-          for (int k = 0; k < 4; ++k) {
-            uint32_t s0[32];
-            tmem_ld32(ts + k * 32, s0);
-            tmem_ld_wait();
-            const int below = seen_below(k);
-            float u = neg_inf();
 #pragma unroll
-            for (int c = 0; c < 32; ++c)
-              if (key_token(c) < below) u = fmaxf(u, __uint_as_float(s0[c]));
-            if (u > neg_inf()) top = fmaxf(top, u * (k == 0 ? f[0] : k == 1 ? f[1] : k == 2 ? f[2] : f[3]));
+          for (int c = 0; c < 32; ++c) {
+            if (key_token(c) < below0) u[0] = fmaxf(u[0], __uint_as_float(s0[c]));
+            if (key_token(c) < below1) u[2] = fmaxf(u[2], __uint_as_float(s1[c]));
           }
         }
+        u[0] = fmaxf(u[0], u[1]);
+        u[2] = fmaxf(u[2], u[3]);
+        // nothing seen is no 0 (a scale of 0 times -inf)
+        const float top = fmaxf(u[0] > neg_inf() ? u[0] * f0 : u[0], u[2] > neg_inf() ? u[2] * f1 : u[2]);
         const bool raise = top > (m == neg_inf() ? m : m + kRise);
         if (__any_sync(0xffffffffu, raise)) {
           const float mn = raise ? top : m;
@@ -398,21 +409,21 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(KvPromptAr
           l *= alpha;
           m = mn;
           if (j > 0) {
-            wait(&bar.pvdone[x], npv & 1);       // the product before this one
+            // the product before this one; the one before that ended before this S began
+            wait(&bar.pvdone[x][place ^ 1], before - 1);
             tc_fence_after();
 #pragma unroll 1
-            for (int k = 0; k < D / 32; ++k) {
-              uint32_t r[32];
-              tmem_ld32(to + k * 32, r);
+            for (int k = 0; k < D / 16; ++k) {
+              uint32_t r[16];
+              tmem_ld16(to + k * 16, r);
               tmem_ld_wait();
 #pragma unroll
-              for (int c = 0; c < 32; ++c) r[c] = __float_as_uint(__uint_as_float(r[c]) * alpha);
-              tmem_st32(to + k * 32, r);
+              for (int c = 0; c < 16; ++c) r[c] = __float_as_uint(__uint_as_float(r[c]) * alpha);
+              tmem_st16(to + k * 16, r);
             }
             tmem_st_wait();
           }
         }
-        if (j > 0) ++npv;
         const float base = m == neg_inf() ? 0.0f : m - kLift;
         if (j == 0) {
           wait(&bar.vfull[kt & 1], kt >> 1);     // the unit's V exponents are known
@@ -420,65 +431,55 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(KvPromptAr
           half = e.x - e.y <= 32;
           unscale = pow2_exact(e.x - 127 - 8);
         }
-        const bool odd = (nt.flags >> 4) != 0u;  // a NaN block of V
-        if (!cut && half && !odd) {
-          // the common tile: two blocks at a time, the next one on its way
-          const uint64_t nb2 = pair(-base, -base);
-          uint64_t part = 0;
-          uint32_t s0[32], s1[32];
-          tmem_ld32(ts, s0);
-          tmem_ld_wait();
+        uint32_t p[32];
+        if (!cut && half && !(flags & 0x30u)) {  // the common step
+          const uint64_t nb2 = pair(-base, -base), f02 = pair(f0, f0), f12 = pair(f1, f1);
+          uint64_t part0 = 0, part1 = 0;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            uint32_t(&s)[32] = k & 1 ? s1 : s0;
-            uint32_t(&next_s)[32] = k & 1 ? s0 : s1;
-            if (k < 3) tmem_ld32(ts + (k + 1) * 32, next_s);
-            const uint64_t f2 = pair(f[k], f[k]);
-#pragma unroll
-            for (int c = 0; c < 32; c += 2) {
-              float p0, p1;
-              unpair(fma2(pair(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), f2, nb2), p0, p1);
-              p0 = ex2(p0);
-              p1 = ex2(p1);
-              part = add2(part, pair(p0, p1));
-              s[c / 2] = pack_f16(p0, p1);
-            }
-            if (k < 3) tmem_ld_wait();           // columns 32 (k + 1) .. are read: P's may be written over S
-            tmem_st16(ts + k * 16, s);
+          for (int c = 0; c < 32; c += 2) {
+            float p0, p1, q0, q1;
+            unpair(fma2(pair(__uint_as_float(s0[c]), __uint_as_float(s0[c + 1])), f02, nb2), p0, p1);
+            unpair(fma2(pair(__uint_as_float(s1[c]), __uint_as_float(s1[c + 1])), f12, nb2), q0, q1);
+            p0 = ex2(p0);
+            p1 = ex2(p1);
+            q0 = ex2(q0);
+            q1 = ex2(q1);
+            part0 = add2(part0, pair(p0, p1));
+            part1 = add2(part1, pair(q0, q1));
+            p[c / 2] = pack_f16(p0, p1);
+            p[16 + c / 2] = pack_f16(q0, q1);
           }
           float p0, p1;
-          unpair(part, p0, p1);
+          unpair(add2(part0, part1), p0, p1);
           l += p0 + p1;
         } else {
-#pragma unroll 1
-          for (int k = 0; k < 4; ++k) {
-            uint32_t s[32];
-            tmem_ld32(ts + k * 32, s);
-            tmem_ld_wait();
-            const float fk = k == 0 ? f[0] : k == 1 ? f[1] : k == 2 ? f[2] : f[3];
-            const int below = seen_below(k);
-            float part = 0.0f;
+          float part0 = 0.0f, part1 = 0.0f;
 #pragma unroll
-            for (int c = 0; c < 32; c += 2) {
-              float p0 = ex2(fmaf(__uint_as_float(s[c]), fk, -base));
-              float p1 = ex2(fmaf(__uint_as_float(s[c + 1]), fk, -base));
-              if (key_token(c) >= below) p0 = 0.0f;
-              if (key_token(c + 1) >= below) p1 = 0.0f;
-              part += p0 + p1;
-              s[c / 2] = half ? pack_f16(p0, p1) : pack_bf16(p0, p1);
-            }
-            l += (nt.flags >> (4 + k) & 1u) && part > 0.0f ? __int_as_float(0x7fc00000) : part;
-            tmem_st16(ts + k * 16, s);
+          for (int c = 0; c < 32; c += 2) {
+            float p0 = ex2(fmaf(__uint_as_float(s0[c]), f0, -base)), p1 = ex2(fmaf(__uint_as_float(s0[c + 1]), f0, -base));
+            float q0 = ex2(fmaf(__uint_as_float(s1[c]), f1, -base)), q1 = ex2(fmaf(__uint_as_float(s1[c + 1]), f1, -base));
+            if (key_token(c) >= below0) p0 = 0.0f;
+            if (key_token(c + 1) >= below0) p1 = 0.0f;
+            if (key_token(c) >= below1) q0 = 0.0f;
+            if (key_token(c + 1) >= below1) q1 = 0.0f;
+            part0 += p0 + p1;
+            part1 += q0 + q1;
+            p[c / 2] = half ? pack_f16(p0, p1) : pack_bf16(p0, p1);
+            p[16 + c / 2] = half ? pack_f16(q0, q1) : pack_bf16(q0, q1);
           }
+          if ((flags & 0x10u) && part0 > 0.0f) part0 = __int_as_float(0x7fc00000);
+          if ((flags & 0x20u) && part1 > 0.0f) part1 = __int_as_float(0x7fc00000);
+          l += part0 + part1;
         }
+        tmem_st32(tp, p);                        // over S, which has been read
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bar.pfull[x]);
+        if (lane == 0) mbar_arrive(&bar.pfull[x][place]);
       }
       if (my > 0) {
-        wait(&bar.pvdone[x], npv & 1);
-        ++npv;
+        const bool second = !(my & 1);
+        wait(&bar.pvdone[x][second], (second ? taken1 : taken0) - 1);   // the last product, and so all
         tc_fence_after();
       }
       const float inv = l == 0.0f ? 0.0f : unscale / l;
@@ -674,87 +675,71 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(KvPromptAr
   } else {
     // ----------------------------------------------------------- issuer
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    uint32_t pa = 0, pb = 0;             // P tiles taken of A, of B
+    const int x = warp - 12;             // the tile that this warp issues for
+    uint32_t np0 = 0, np1 = 0;           // P taken from each place
     for (; next(un); kt += un.n) {
-      if (warp != 12) continue;
-      const int na = un.na, ntb = un.nb, n = un.n;
-      constexpr uint32_t kIdS = idesc_16(false, 128, kTileKeys);
+      if (x > 1) continue;
+      const int my = uniform(x ? un.nb : un.na), n = uniform(un.n) * 2;   // steps of this tile; of the unit, in whole K/V tiles
+      const uint32_t kt0 = uniform(kt), tm = uniform(tmem);
+      constexpr uint32_t kIdS = idesc_16(false, 128, kStepKeys);
       uint32_t id_o = idesc_16(false, 128, D);
-      const uint64_t dq = sw128_kmajor_desc(smem_u32(sq)), dk = sw128_kmajor_desc(smem_u32(sk)),
+      const uint64_t dq = sw128_kmajor_desc(smem_u32(sq + x * S::kQTile)), dk = sw128_kmajor_desc(smem_u32(sk)),
                      dv = sw128_kmajor_desc(smem_u32(sv));
-      // The warp stays together and elects the lane that issues.
-      // S of tile x: D / 16 steps of 32 bytes, a 16 KB half every four
-      auto scores = [&](int x, int st) {
-        if (elect_one()) {
+      const uint32_t to = tm + kColO + x * 128;
+      auto alive = [&]() { return __all_sync(0xffffffffu, !s_dead) != 0; };   // the same in all lanes
+      wait(&bar.qfull[x], round - 1);
+      // step i: the product of step i - 2, and S of step i, whose place it frees
+#pragma unroll 1
+      for (int i = 0; i < n + 2; ++i) {
+        const int j = i - 2, place = i & 1;
+        const uint32_t g = kt0 + (j >> 1), gk = kt0 + (i >> 1);
+        const uint32_t ts = tm + kColS + x * 128 + place * 64;
+        if (j >= 0 && !place) {
+          wait(&bar.vfull[g & 1], g >> 1);
+          const int2 e = v_range();
+          id_o = idesc_16(e.x - e.y > 32, 128, D);
+        }
+        if (j >= 0 && j < my) {
+          wait(&bar.pfull[x][place], place ? np1 : np0);
+          np0 += place ^ 1;
+          np1 += place;
+          tc_fence_after();
+          if (alive() && elect_one()) {
+            // O += P of the step and its half of the V tile
+            const uint64_t db = dv + (((g & 1) * S::kKTile + place * (D * 128)) >> 4);
+#pragma unroll
+            for (int k = 0; k < kStepKeys / 16; ++k) mma_ts(to, ts + k * 8, db + k * 2, id_o, j > 0 || k > 0);
+            mma_commit(&bar.pvdone[x][place]);
+          }
+          __syncwarp();
+        }
+        if (i < n && !place) {
+          wait(&bar.kfull[gk & 1], gk >> 1);
+          tc_fence_after();
+        }
+        if (i < my && alive() && elect_one()) {
+          // S: D / 16 MMAs of 32 bytes a row, a 16 KB half every four; the step's
+          // keys are rows place * 64 .. of the K tile
+          const uint64_t db = dk + (((gk & 1) * S::kKTile + place * (kStepKeys * 128)) >> 4);
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
-            const uint32_t at = (k >> 2) * (128 * 128) + (k & 3) * 32;
-            mma_bf16_ss(tmem + kColS + x * 128, dq + ((x * S::kQTile + at) >> 4), dk + ((st * S::kKTile + at) >> 4), kIdS, k > 0);
+            const uint32_t at = ((k >> 2) * (128 * 128) + (k & 3) * 32) >> 4;
+            mma_bf16_ss(ts, dq + at, db + at, kIdS, k > 0);
           }
-          mma_commit(&bar.sfull[x]);
+          mma_commit(&bar.sfull[x][place]);
         }
         __syncwarp();
-      };
-      auto product = [&](int x, int st, bool more) {
-        if (elect_one()) {
-#pragma unroll
-          for (int k = 0; k < kTileKeys / 16; ++k) {
-            const uint32_t at = (k >> 2) * (D * 128) + (k & 3) * 32;
-            mma_ts(tmem + kColO + x * 128, tmem + kColS + x * 128 + k * 8, dv + ((st * S::kKTile + at) >> 4), id_o, more || k > 0);
-          }
-          mma_commit(&bar.pvdone[x]);
+        // the tiles that this warp is done with
+        if (place && alive() && elect_one()) {
+          if (j >= 0) mma_commit(&bar.vempty[g & 1]);
+          if (i < n) mma_commit(&bar.kempty[gk & 1]);
         }
         __syncwarp();
-      };
-      auto release = [&](uint64_t* b) {
-        if (elect_one()) mma_commit(b);
-        __syncwarp();
-      };
-      wait(&bar.qfull, round - 1);
-      if (n > 0) {
-        wait(&bar.kfull[kt & 1], kt >> 1);
-        tc_fence_after();
-        if (!s_dead) {
-          if (0 < na) scores(0, kt & 1);
-          if (0 < ntb) scores(1, kt & 1);
-          release(&bar.kempty[kt & 1]);
-        }
-      }
-      for (int j = 0; j < n; ++j) {
-        const uint32_t g = kt + j;
-        const int st = g & 1, sn = st ^ 1;
-        wait(&bar.vfull[st], g >> 1);
-        if (j == 0) {
-          const int2 e = v_range();
-          if (e.x - e.y > 32) id_o = idesc_16(true, 128, D);
-        }
-        // A's product, A's next S; B's product, B's next S: one tile's softmax
-        // has the time of the other's MMAs
-        if (j < na) {
-          wait(&bar.pfull[0], pa++);
-          tc_fence_after();
-          if (!s_dead) product(0, st, j > 0);
-        }
-        if (j + 1 < n) {
-          wait(&bar.kfull[sn], (g + 1) >> 1);
-          tc_fence_after();
-          if (j + 1 < na && !s_dead) scores(0, sn);
-        }
-        if (j < ntb) {
-          wait(&bar.pfull[1], pb++);
-          tc_fence_after();
-          if (!s_dead) product(1, st, j > 0);
-        }
-        if (!s_dead) release(&bar.vempty[st]);
-        if (j + 1 < n && !s_dead) {
-          if (j + 1 < ntb) scores(1, sn);
-          release(&bar.kempty[sn]);
-        }
       }
     }
   }
   // ---- every MMA has ended before tensor memory goes
-  if (warp == 12) {
+  if (warp == 12 || warp == 13) {
     if (elect_one()) mma_commit(&bar.drain);
     (void)mbar_wait(&bar.drain, 0, a.status);
   }
