@@ -23,8 +23,8 @@
 // probabilities (eight tokens a lane), and nothing is shuffled.
 //
 // Work: units (request, head, tile of query rows), each as many places long
-// as it has blocks and one for its start, laid out in one line that is cut into equal pieces,
-// one a warp, whatever the lengths are; every CTA finds its pieces by
+// as it has blocks and kStart more, laid out in one line that is cut into equal
+// pieces, one a warp, whatever the lengths are; every CTA finds its pieces by
 // summing the lengths itself.  A warp runs through its piece with one ring of
 // cp.async stages that does not stop at a unit's end.  Units that lie in one
 // piece are written by its warp; those cut by a piece's end are joined by the
@@ -40,8 +40,10 @@ namespace {
 constexpr int kMaxWarps = 12;
 constexpr int kMaxRows = 16;             // query rows a unit
 constexpr int kStages = 2;               // blocks a warp has in its ring
-constexpr int kStart = 1;                // places a unit's start takes
-constexpr int kMinPiece = 2;             // places a piece at least
+// Places a unit's start takes: what its rows, their end and the join cost, in
+// blocks (192 unequal requests: 132 us with 1, 126 with 2, 121 with 4, 123 with 10).
+constexpr int kStart = 4;
+constexpr int kMinPiece = 1;             // places a piece at least
 constexpr size_t kPromptUnits = 32;      // units of the prompts' kernel that are worth it
 constexpr float kLn2 = 0.693147180559945f;
 
@@ -604,8 +606,7 @@ __global__ void __launch_bounds__(Tile::kWarps * 32, 1) kv_attn_kernel(AttnArgs 
     return x;
   };
 
-  // ---- places lo + first + lane: the block there and its scales (K | V << 8);
-  // -1: a page that holds no keys, or no block, or one that no row of the tile sees
+  // ---- places pos + lane: the block there and its scales (K | V << 8); -1: a page that holds no keys, or no block, or one that no row of the tile sees
   long place = -1;
   uint32_t place_sc = 0;
   auto look_up = [&](long pos) {
@@ -632,32 +633,56 @@ __global__ void __launch_bounds__(Tile::kWarps * 32, 1) kv_attn_kernel(AttnArgs 
     }
   };
   const int mine = lo < hi ? (int)(hi - lo) : 0;
-  // place i of this piece into its stage: K and V are groups of their own, so
-  // that K's part is refilled while V's is still in use
-  auto fetch = [&](int i, bool is_v) {
-    const long at = __shfl_sync(0xffffffffu, place, i & 31);
-    if (i < mine && at >= 0) {
-      const uint32_t st = ring_s + (i % kStages) * kStage + (is_v ? 32 * D : 0);
-      const int8_t* src = (is_v ? a.c.v : a.c.k) + at * (32 * D);
-#pragma unroll
-      for (int u = 0; u < 2 * D / 32; ++u) {
-        const int ch = u * 32 + lane;
-        cp16(st + (is_v ? Tile::v_place(ch) : Tile::k_place(ch)) * 16, src + ch * 16);
+  // The ring holds the next two blocks (places without one are passed over):
+  // where in the piece they are, their scales, and where in the cache.  K and V
+  // are groups of their own, so that K's part of a stage is refilled while V's
+  // is still in use.
+  int to_see = 0;                        // first place that has not been looked at
+  int q_pos0 = -1, q_pos1 = -1;
+  uint32_t q_sc0 = 0, q_sc1 = 0;
+  long q_at0 = 0, q_at1 = 0;
+  auto fetch_k = [&](int s) {
+    int found = -1;
+    while (to_see < mine) {
+      if ((to_see & 31) == 0 && to_see) look_up(lo + to_see);
+      const uint32_t here = __ballot_sync(0xffffffffu, place >= 0) >> (to_see & 31);
+      if (here) {
+        found = to_see + __ffs((int)here) - 1;
+        to_see = found + 1;
+        break;
       }
+      to_see = (to_see | 31) + 1;
+    }
+    if (s) q_pos1 = found;
+    else q_pos0 = found;
+    if (found >= 0) {
+      const long at = __shfl_sync(0xffffffffu, place, found & 31);
+      const uint32_t sc = __shfl_sync(0xffffffffu, place_sc, found & 31);
+      if (s) q_at1 = at, q_sc1 = sc;
+      else q_at0 = at, q_sc0 = sc;
+      const int8_t* src = a.c.k + at * (32 * D);
+#pragma unroll
+      for (int u = 0; u < 2 * D / 32; ++u)
+        cp16(ring_s + s * kStage + Tile::k_place(u * 32 + lane) * 16, src + (u * 32 + lane) * 16);
     }
     cp_commit();
   };
-  long pl_now = -1;                      // the 32 places that hold the current one
-  uint32_t sc_now = 0;
+  auto fetch_v = [&](int s) {
+    if ((s ? q_pos1 : q_pos0) >= 0) {
+      const int8_t* src = a.c.v + (s ? q_at1 : q_at0) * (32 * D);
+#pragma unroll
+      for (int u = 0; u < 2 * D / 32; ++u)
+        cp16(ring_s + s * kStage + 32 * D + Tile::v_place(u * 32 + lane) * 16, src + (u * 32 + lane) * 16);
+    }
+    cp_commit();
+  };
+  int stage = 0;                         // of the next block
   if (mine) {
     look_up(lo);
-    pl_now = place;
-    sc_now = place_sc;
-#pragma unroll
-    for (int i = 0; i < kStages; ++i) {
-      fetch(i, false);
-      fetch(i, true);
-    }
+    fetch_k(0);
+    fetch_v(0);
+    fetch_k(1);
+    fetch_v(1);
   }
 
   int req = mine ? request_of(lo) : 0;
@@ -681,28 +706,23 @@ __global__ void __launch_bounds__(Tile::kWarps * 32, 1) kv_attn_kernel(AttnArgs 
 
     Tile t;
     if (has) t.start(a, row0, tile, head, nrows, past);
-    for (; i < end; ++i) {
-      const int nx = i + kStages;
-      // place / place_sc: the 32 places that hold nx
-      if ((i & 31) == 0 && i) {
-        pl_now = place;
-        sc_now = place_sc;
-      }
-      if ((nx & 31) == 0) look_up(lo + nx);
-      uint8_t* st = ring + (i % kStages) * kStage;
-      const long at = __shfl_sync(0xffffffffu, pl_now, i & 31);
-      const uint32_t sc = __shfl_sync(0xffffffffu, sc_now, i & 31);
-      cp_wait<2 * kStages - 1>();        // K of place i is there; V of it and what follows may be on the way
+    i = end;
+    for (;;) {
+      const int at = stage ? q_pos1 : q_pos0;
+      if (at < 0 || at >= end) break;
+      uint8_t* st = ring + stage * kStage;
+      const uint32_t sc = stage ? q_sc1 : q_sc0;
+      cp_wait<2 * kStages - 1>();        // K is there; V and what follows may be on the way
       __syncwarp();
-      if (at >= 0)
-        t.keys(st, ((int)(lo + i - unit0) - kStart) * 32, e8m0_to_float(sc & 0xFF), e8m0_to_float(sc >> 8), scratch);
+      t.keys(st, ((int)(lo + at - unit0) - kStart) * 32, e8m0_to_float(sc & 0xFF), e8m0_to_float(sc >> 8), scratch);
       __syncwarp();                      // every lane has read it before it is refilled
-      fetch(nx, false);
-      cp_wait<2 * kStages - 1>();        // V of place i
+      fetch_k(stage);
+      cp_wait<2 * kStages - 1>();        // V
       __syncwarp();
-      if (at >= 0) t.values(st + 32 * D, scratch);
+      t.values(st + 32 * D, scratch);
       __syncwarp();
-      fetch(nx, true);
+      fetch_v(stage);
+      stage ^= 1;
     }
     if (!has) continue;
 
