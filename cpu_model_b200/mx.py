@@ -11,12 +11,13 @@ torch is used only as the device-memory and stream carrier; all arithmetic
 runs in the library's sm_100a kernels.
 """
 import ctypes
+import os
 from dataclasses import dataclass
 
 import torch
 
 from . import _lib
-from ._lib import ACT_NONE, ACT_SILU, DT_BF16, DT_F16, DT_F32, FMT_INT4, FMT_INT8, PATH_AUTO, PATH_GEMM, PATH_GEMV, check
+from ._lib import ACT_NONE, ACT_SILU, FMT_INT4, FMT_INT8, PATH_AUTO, PATH_GEMM, PATH_GEMV, check
 
 __all__ = [
     "MXContext", "MXWeight", "MXActivation", "context",
@@ -733,102 +734,36 @@ def ppo_rollout_forward(states, actions, w_proj, w_policy, w_value=None, ctx=Non
 
 
 # ------------------------------------------------------------------ serving ---
-_DTYPES = {torch.float32: DT_F32, torch.bfloat16: DT_BF16, torch.float16: DT_F16}
+# The arguments of these calls are checked, and their results allocated, by the
+# binding (csrc/mxq_py.cpp): a step's calls take the GPU a few microseconds each.
 KV_BLOCK = _lib.KV_BLOCK
 
 
-# These calls take the GPU a few microseconds, so the checks before them are
-# written to cost less: pointers go to the library as integers, and the words of a
-# refusal are put together only where there is one.
-def _want(t, dtype, name):
-    try:
-        if t.dtype is dtype and t.is_cuda and t.is_contiguous():
-            return
-    except AttributeError:
-        pass
-    _need_cuda(t, dtype, name)
+class _NotBuilt:
+    def __getattr__(self, name):
+        raise ImportError("_serve.so is not built (expected beside %s); run `python -m cpu_model_b200.build`" % _lib.LIB_PATH)
 
 
-def _row_dtype(t, name):
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
-        raise ValueError("%s must be a CUDA tensor" % name)
-    dt = _DTYPES.get(t.dtype)
-    if dt is None:
-        raise ValueError("%s must be float32, bfloat16 or float16, got %s" % (name, t.dtype))
-    return dt
+try:
+    from . import _serve
+except ImportError:
+    if os.path.exists(os.path.join(os.path.dirname(_lib.LIB_PATH), "_serve.so")):
+        raise
+    _serve = _NotBuilt()
+    KVCache = None
+else:
+    KVCache = _serve.KVCache
 
-
-def _row_stride(t, name):
-    """Elements from one row to the next; the dimensions of a row lie side by side."""
-    shape, stride = t.shape, t.stride()
-    if t.is_contiguous():
-        inner = t.numel() // shape[0] if shape[0] else 1
-        return max(inner, stride[0])
-    inner = 1
-    for n, s in zip(reversed(shape[1:]), reversed(stride[1:])):
-        if n != 1 and s != inner:
-            raise ValueError("%s: only rows may have a stride, got %s" % (name, stride))
-        inner *= n
-    return stride[0] if shape[0] > 1 else max(inner, stride[0])
-
-
-def _serve_ctx(ctx, first, *others):
-    """The context of the call, bound to the current stream."""
-    dev = first.get_device()
-    for t in others:
-        if t is not None and t.get_device() != dev:
-            raise ValueError("tensors lie on %s and %s" % (first.device, t.device))
-    if ctx is None:
-        ctx = _contexts.get(dev) or context(dev)
-    ctx._bind()
-    return ctx
-
-
-def _at(t):
-    return 0 if t is None else t.data_ptr()
-
-
-class _KVCacheC(ctypes.Structure):
-    """mxq_kv_cache (include/mxq.h)."""
-    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
-                ("v_scale", ctypes.c_void_p), ("n_pages", ctypes.c_int), ("page_size", ctypes.c_int),
-                ("n_kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int)]
-
-
-class KVCache:
-    """A paged 8-bit K/V cache (mxq_kv_cache): int8 values, one E8M0 scale for
-    each block of 32 tokens and head.  The four tensors are the caller's:
-    k int8 [n_pages][H][page/32][32][D], v int8 [n_pages][H][page/32][D/2][4][2][8],
-    k_scale and v_scale uint8 [n_pages][H][page/32]."""
-
-    def __init__(self, k, v, k_scale, v_scale):
-        _want(k, torch.int8, "k")
-        _want(v, torch.int8, "v")
-        _want(k_scale, torch.uint8, "k_scale")
-        _want(v_scale, torch.uint8, "v_scale")
-        if k.dim() != 5 or k.shape[3] != KV_BLOCK:
-            raise ValueError("k must be [n_pages][heads][blocks][32][head_dim], got %s" % (tuple(k.shape),))
-        n, h, nb, _, d = k.shape
-        if v.shape != (n, h, nb, d // 2, 4, 2, 8):
-            raise ValueError("v must be [n_pages][heads][blocks][head_dim / 2][4][2][8], got %s" % (tuple(v.shape),))
-        if k_scale.shape != (n, h, nb) or v_scale.shape != (n, h, nb):
-            raise ValueError("k_scale and v_scale must be [n_pages][heads][blocks]")
-        if not k.get_device() == v.get_device() == k_scale.get_device() == v_scale.get_device():
-            raise ValueError("the cache's tensors lie on different devices")
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = n, h, nb * KV_BLOCK, d
-        self._c = _KVCacheC(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n, self.page_size, h, d)
-
-    @classmethod
-    def empty(cls, n_pages, page_size, n_kv_heads, head_dim, device="cuda"):
+    def _empty_cache(n_pages, page_size, n_kv_heads, head_dim, device="cuda"):
         """A cache of n_pages pages; every block is written before it is read."""
         if page_size <= 0 or page_size % KV_BLOCK:
             raise ValueError("the page size is a multiple of 32, got %d" % page_size)
-        nb = page_size // KV_BLOCK
-        return cls(torch.zeros((n_pages, n_kv_heads, nb, KV_BLOCK, head_dim), dtype=torch.int8, device=device),
-                   torch.zeros((n_pages, n_kv_heads, nb, head_dim // 2, 4, 2, 8), dtype=torch.int8, device=device),
-                   torch.zeros((n_pages, n_kv_heads, nb), dtype=torch.uint8, device=device),
-                   torch.zeros((n_pages, n_kv_heads, nb), dtype=torch.uint8, device=device))
+        shape = (n_pages, n_kv_heads, page_size // KV_BLOCK)
+        new = lambda *dims, dtype: torch.zeros(shape + dims, dtype=dtype, device=device)
+        return KVCache(new(KV_BLOCK, head_dim, dtype=torch.int8), new(head_dim // 2, 4, 2, 8, dtype=torch.int8),
+                       new(dtype=torch.uint8), new(dtype=torch.uint8))
+
+    KVCache.empty = staticmethod(_empty_cache)
 
 
 @dataclass
@@ -845,10 +780,15 @@ class KVPlan:
     short: torch.Tensor
 
 
-def _table(table, rows):
-    _want(table, torch.int32, "table")
-    if table.dim() != 2 or table.shape[0] != rows:
-        raise ValueError("table must be [n_requests][max_pages], got %s" % (tuple(table.shape),))
+def _address(ctx, tensor):
+    """The address of the call's context: the given one or the default one of
+    the tensor's device."""
+    if ctx is None:
+        dev = tensor.get_device()
+        if dev < 0:
+            raise ValueError("the tensors must lie on a CUDA device")
+        ctx = _contexts.get(dev) or context(dev)
+    return ctx.h.value
 
 
 def kv_plan(past, new, page_size, table, free_pages, free_count, n_tokens, in_place=False, ctx=None):
@@ -857,84 +797,25 @@ def kv_plan(past, new, page_size, table, free_pages, free_count, n_tokens, in_pl
     pages taken from the stack free_pages[:free_count]; n_tokens rows of maps
     are written (the sum of new, or more: the rest are -1).  With in_place,
     `past` becomes ctx_len and free_count is lowered.  Returns a KVPlan."""
-    _want(past, torch.int32, "past")
-    _want(new, torch.int32, "new")
-    _want(free_pages, torch.int32, "free_pages")
-    _want(free_count, torch.int32, "free_count")
-    r = past.numel()
-    if new.numel() != r or free_count.numel() != 1:
-        raise ValueError("kv_plan: past and new must hold one length a request, free_count one number")
-    _table(table, r)
-    n = int(n_tokens)
-    if n < 0:
-        raise ValueError("kv_plan: n_tokens is negative")
-    ctx = _serve_ctx(ctx, past, new, table, free_pages, free_count)
-    # one allocation for the maps and the two numbers
-    sizes = [n, n, n, r + 1, 1] if in_place else [n, n, n, r + 1, 1, 1, r]
-    views = past.new_empty(3 * n + r + 2 + (0 if in_place else 1 + r)).split_with_sizes(sizes)
-    slots, pos, req, cu, short = views[:5]
-    free_out, ctx_len = (free_count, past) if in_place else views[5:]
-    cu_at = cu.data_ptr()
-    at = cu_at - 12 * n
-    rc = ctx.lib.mxq_kv_plan(ctx.h, past.data_ptr(), new.data_ptr(), r, page_size, table.data_ptr(), table.shape[1],
-                             free_pages.data_ptr(), free_pages.numel(), free_count.data_ptr(), ctx_len.data_ptr(), cu_at, at,
-                             at + 4 * n, at + 8 * n, n, free_out.data_ptr(), cu_at + 4 * (r + 1))
-    if rc:
-        check(rc, ctx.h)
-    return KVPlan(ctx_len, cu, slots, pos, req, free_out, short)
+    return KVPlan(*_serve.kv_plan(_address(ctx, past), past, new, page_size, table, free_pages, free_count, n_tokens, in_place))
 
 
 def kv_release(done, lengths, page_size, table, free_pages, free_count, ctx=None):
     """Give the pages of ended requests back (mxq_kv_release): done uint8 or
     bool [R]; lengths, table, free_pages and free_count are updated."""
-    if isinstance(done, torch.Tensor) and done.dtype == torch.bool:
-        done = done.view(torch.uint8)
-    _want(done, torch.uint8, "done")
-    for name, t in (("lengths", lengths), ("free_pages", free_pages), ("free_count", free_count)):
-        _want(t, torch.int32, name)
-    r = lengths.numel()
-    if done.numel() != r or free_count.numel() != 1:
-        raise ValueError("kv_release: done and lengths must hold one value a request, free_count one number")
-    _table(table, r)
-    ctx = _serve_ctx(ctx, lengths, done, table, free_pages, free_count)
-    check(ctx.lib.mxq_kv_release(ctx.h, _at(done), _at(lengths), r, page_size, _at(table), table.shape[1],
-                                 _at(free_pages), free_pages.numel(), _at(free_count)), ctx.h)
+    _serve.kv_release(_address(ctx, lengths), done, lengths, page_size, table, free_pages, free_count)
 
 
 def kv_append(cache, k, v, slots, ctx=None):
     """Quantise new K/V rows into the cache (mxq_kv_append): k, v [N][H][D]
     (float32, bfloat16 or float16; rows may have a stride, as slices of fused
     QKV rows do), slots int32 [N] (-1: not stored)."""
-    dt = _row_dtype(k, "k")
-    _want(slots, torch.int32, "slots")
-    if not isinstance(v, torch.Tensor) or v.dtype != k.dtype or v.shape != k.shape:
-        raise ValueError("kv_append: k and v must have one type and shape")
-    n = slots.numel()
-    if k.shape != (n, cache.n_kv_heads, cache.head_dim):
-        raise ValueError("kv_append: k and v must be [n][%d][%d] with one slot a row" % (cache.n_kv_heads, cache.head_dim))
-    stride = _row_stride(k, "k")
-    if _row_stride(v, "v") != stride:
-        raise ValueError("kv_append: k and v must have the same row stride")
-    ctx = _serve_ctx(ctx, cache.k, k, v, slots)
-    rc = ctx.lib.mxq_kv_append(ctx.h, ctypes.byref(cache._c), dt, k.data_ptr(), v.data_ptr(), stride, slots.data_ptr(), n)
-    if rc:
-        check(rc, ctx.h)
+    _serve.kv_append(_address(ctx, slots), cache, k, v, slots)
 
 
 def kv_read(cache, slots, dtype=torch.float32, ctx=None):
     """Cached tokens as values (mxq_kv_read): (k, v) [N][H][D] of `dtype`."""
-    _want(slots, torch.int32, "slots")
-    if dtype not in _DTYPES:
-        raise ValueError("kv_read: float32, bfloat16 or float16, got %s" % dtype)
-    ctx = _serve_ctx(ctx, cache.k, slots)
-    n = slots.numel()
-    shape = (n, cache.n_kv_heads, cache.head_dim)
-    k = slots.new_empty(shape, dtype=dtype)
-    v = torch.empty_like(k)
-    rc = ctx.lib.mxq_kv_read(ctx.h, ctypes.byref(cache._c), slots.data_ptr(), n, _DTYPES[dtype], k.data_ptr(), v.data_ptr())
-    if rc:
-        check(rc, ctx.h)
-    return k, v
+    return _serve.kv_read(_address(ctx, slots), cache, slots, dtype)
 
 
 def kv_attention(q, cache, table, ctx_len, cu, scale=None, max_new=None, want_lse=True, ctx=None):
@@ -943,29 +824,7 @@ def kv_attention(q, cache, table, ctx_len, cu, scale=None, max_new=None, want_ls
     r's rows are cu[r] .. cu[r + 1] - 1, the last of its ctx_len[r] tokens.
     scale defaults to 1 / sqrt(D); max_new bounds the new rows of a request.
     Returns (out [N][Hq][D] of q's type, lse fp32 [N][Hq] or None)."""
-    dt = _row_dtype(q, "q")
-    _want(ctx_len, torch.int32, "ctx_len")
-    _want(cu, torch.int32, "cu")
-    r = ctx_len.numel()
-    _table(table, r)
-    if q.dim() != 3 or q.shape[2] != cache.head_dim or q.shape[1] % cache.n_kv_heads:
-        raise ValueError("kv_attention: q must be [n][heads][%d] with heads a multiple of %d, got %s"
-                         % (cache.head_dim, cache.n_kv_heads, tuple(q.shape)))
-    if cu.numel() != r + 1:
-        raise ValueError("kv_attention: cu must hold n_requests + 1 offsets")
-    n, hq, d = q.shape
-    if max_new is not None and max_new < 1:
-        raise ValueError("kv_attention: max_new must be positive")
-    ctx = _serve_ctx(ctx, cache.k, q, table, ctx_len, cu)
-    out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((n, hq, d))
-    lse = q.new_empty((n, hq), dtype=torch.float32) if want_lse else None
-    rc = ctx.lib.mxq_kv_attention(ctx.h, ctypes.byref(cache._c), dt, q.data_ptr(), _row_stride(q, "q"), n, hq,
-                                  table.data_ptr(), table.shape[1], ctx_len.data_ptr(), cu.data_ptr(), r,
-                                  max(1, n if max_new is None else max_new), d ** -0.5 if scale is None else scale,
-                                  out.data_ptr(), _at(lse))
-    if rc:
-        check(rc, ctx.h)
-    return out, lse
+    return _serve.kv_attention(_address(ctx, q), q, cache, table, ctx_len, cu, scale, max_new, want_lse)
 
 
 @dataclass
@@ -979,58 +838,18 @@ class TokenLogprobs:
     top_ids: torch.Tensor = None
 
 
-def _logits_rows(logits, targets):
-    dt = _row_dtype(logits, "logits")
-    _want(targets, torch.int32, "targets")
-    if logits.dim() != 2 or targets.numel() != logits.shape[0]:
-        raise ValueError("logits must be [rows][vocab] with one target a row")
-    return dt, _row_stride(logits, "logits")
-
-
 def token_logprobs(logits, targets, top_k=0, ctx=None):
     """Log probabilities of given tokens with entropy and the top_k largest
     alternatives (mxq_token_logprobs): logits [N][V] (float32, bfloat16 or
     float16; rows may have a stride), targets int32 [N] (outside [0, V): 0).
     Returns a TokenLogprobs; no autograd (see token_logp)."""
-    dt, stride = _logits_rows(logits, targets)
-    n, v = logits.shape
-    if not 0 <= top_k <= min(v, _lib.TOPK_MAX):
-        raise ValueError("token_logprobs: top_k (%d) must be in [0, min(32, vocab=%d)]" % (top_k, v))
-    ctx = _serve_ctx(ctx, logits, targets)
-    logp, entropy, lse = logits.new_empty((3, n), dtype=torch.float32).unbind(0)
-    top = logits.new_empty((n, top_k), dtype=torch.float32) if top_k else None
-    ids = targets.new_empty((n, top_k)) if top_k else None
-    rc = ctx.lib.mxq_token_logprobs(ctx.h, dt, logits.data_ptr(), stride, n, v, targets.data_ptr(), top_k, logp.data_ptr(),
-                                    entropy.data_ptr(), lse.data_ptr(), _at(top), _at(ids))
-    if rc:
-        check(rc, ctx.h)
-    return TokenLogprobs(logp, entropy, lse, top, ids)
+    return TokenLogprobs(*_serve.token_logprobs(_address(ctx, logits), logits, targets, top_k))
 
 
 def token_logprobs_grad(logits, targets, lse, entropy, dlogp=None, dentropy=None, out=None, ctx=None):
     """The gradient of token_logprobs's logp and entropy to the logits
     (mxq_token_logprobs_grad), of the logits' type; out may be logits."""
-    dt, stride = _logits_rows(logits, targets)
-    n, v = logits.shape
-    for name, t in (("lse", lse), ("entropy", entropy), ("dlogp", dlogp), ("dentropy", dentropy)):
-        if t is not None:
-            _want(t, torch.float32, name)
-            if t.numel() != n:
-                raise ValueError("token_logprobs_grad: %s must hold one value a row" % name)
-    if lse is None or (dentropy is not None and entropy is None):
-        raise ValueError("token_logprobs_grad: lse is needed, and entropy for dentropy")
-    if out is None:
-        out = torch.empty((n, v), dtype=logits.dtype, device=logits.device)
-    elif out.dtype != logits.dtype or out.shape != logits.shape:
-        raise ValueError("token_logprobs_grad: out must have the logits' type and shape")
-    elif not out.is_cuda:
-        raise ValueError("token_logprobs_grad: out must be a CUDA tensor")
-    ctx = _serve_ctx(ctx, logits, targets, lse, entropy, dlogp, dentropy, out)
-    rc = ctx.lib.mxq_token_logprobs_grad(ctx.h, dt, logits.data_ptr(), stride, n, v, targets.data_ptr(), lse.data_ptr(),
-                                         _at(entropy), _at(dlogp), _at(dentropy), out.data_ptr(), _row_stride(out, "out"))
-    if rc:
-        check(rc, ctx.h)
-    return out
+    return _serve.token_logprobs_grad(_address(ctx, logits), logits, targets, lse, entropy, dlogp, dentropy, out)
 
 
 class _TokenLogp(torch.autograd.Function):
