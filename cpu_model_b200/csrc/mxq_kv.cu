@@ -246,7 +246,21 @@ template <typename T, int V> struct Raw {
     for (int i = 0; i < V * (int)sizeof(T) / 4; ++i) w[i] = 0;
   }
   __device__ __forceinline__ float get(int i) const;
+  // The largest |value| so far, in whatever order-keeping bits the type has; f32_bits() of it at the end.
+  __device__ __forceinline__ uint32_t top(uint32_t so_far) const {
+#pragma unroll
+    for (int i = 0; i < V * (int)sizeof(T) / 4; ++i)
+      so_far = sizeof(T) == 4 ? max(so_far, w[i] & 0x7fffffffu) : __vmaxu2(so_far, w[i] & 0x7fff7fffu);
+    return so_far;
+  }
 };
+// What Raw::top left, as the bits of an fp32 number.
+template <typename T> __device__ __forceinline__ uint32_t f32_bits(uint32_t top);
+template <> __device__ __forceinline__ uint32_t f32_bits<float>(uint32_t top) { return top; }
+template <> __device__ __forceinline__ uint32_t f32_bits<__nv_bfloat16>(uint32_t top) { return max(top & 0xffffu, top >> 16) << 16; }
+template <> __device__ __forceinline__ uint32_t f32_bits<__half>(uint32_t top) {
+  return __float_as_uint(__half2float(__ushort_as_half((unsigned short)max(top & 0xffffu, top >> 16))));
+}
 template <> __device__ __forceinline__ float Raw<float, 4>::get(int i) const { return __uint_as_float(w[i]); }
 template <> __device__ __forceinline__ float Raw<float, 2>::get(int i) const { return __uint_as_float(w[i]); }
 __device__ __forceinline__ float bf16_at(uint32_t w, int i) { return __uint_as_float(i & 1 ? w & 0xFFFF0000u : w << 16); }
@@ -326,10 +340,9 @@ __global__ void __launch_bounds__(kCopyWarps * 32)
       Raw<T, V> x;
       for (int r = 0; r < len; ++r) {
         x.load(rows + (long)r * stride);
-#pragma unroll
-        for (int e = 0; e < V; ++e) top = max(top, __float_as_uint(x.get(e)) & 0x7fffffffu);
+        top = x.top(top);
       }
-      top = __reduce_max_sync(0xffffffffu, top);
+      top = __reduce_max_sync(0xffffffffu, f32_bits<T>(top));
       const int byte = max(scale_byte(top), was);
       if (o && byte > was && byte != 255) {
         const float down = step_down(was, byte);
@@ -368,10 +381,8 @@ __global__ void __launch_bounds__(kCopyWarps * 32)
     }
     uint32_t top = 0;
 #pragma unroll
-    for (int t = 0; t < 32; ++t)
-#pragma unroll
-      for (int e = 0; e < V; ++e) top = max(top, __float_as_uint(x[t].get(e)) & 0x7fffffffu);
-    top = __reduce_max_sync(0xffffffffu, top);
+    for (int t = 0; t < 32; ++t) top = x[t].top(top);
+    top = __reduce_max_sync(0xffffffffu, f32_bits<T>(top));
     const int byte = max(scale_byte(top), was);
     const bool grew = o && byte > was && byte != 255;
     const float down = grew ? step_down(was, byte) : 1.0f;
@@ -431,6 +442,11 @@ __global__ void __launch_bounds__(kCopyWarps * 32)
 
 // ------------------------------------------------------------------ read --
 
+// Byte b of a word of int8 as a float: 2^23 + 128 + x from its bits, less 2^23 + 128.
+__device__ __forceinline__ float int8_value(uint32_t flipped, int b) {   // flipped: w ^ 0x80808080
+  return __uint_as_float(__byte_perm(flipped, 0x4B000000u, 0x7540 | b)) - 8388736.0f;
+}
+
 // N consecutive values, N * sizeof(T) bytes aligned.
 __device__ __forceinline__ void put2(float* p, float a, float b) { *reinterpret_cast<float2*>(p) = make_float2(a, b); }
 __device__ __forceinline__ void put2(__nv_bfloat16* p, float a, float b) {
@@ -476,7 +492,7 @@ __global__ void __launch_bounds__(kCopyWarps * 32)
       for (int e = 0; e < 4; ++e) {
         float y[4];
 #pragma unroll
-        for (int b = 0; b < 4; ++b) y[b] = (float)(int8_t)(q[e] >> (8 * b)) * sc;
+        for (int b = 0; b < 4; ++b) y[b] = int8_value(q[e] ^ 0x80808080u, b) * sc;
         store4(to + 4 * e, y);
       }
     }
@@ -495,7 +511,10 @@ __global__ void __launch_bounds__(kCopyWarps * 32)
     const int cc = lane & 3;
     uint4 w[D / 16];
 #pragma unroll
-    for (int u = 0; u < D / 16; ++u) w[u] = __ldg(src + u * 32 + lane);
+    for (int u = 0; u < D / 16; ++u) {
+      w[u] = __ldg(src + u * 32 + lane);
+      w[u].x ^= 0x80808080u; w[u].y ^= 0x80808080u; w[u].z ^= 0x80808080u; w[u].w ^= 0x80808080u;
+    }
 #pragma unroll
     for (int jb = 0; jb < 8; ++jb) {
       const int r = (jb >> 1) * 8 + 2 * cc + (jb & 1) - o;   // the token's entry in the run
@@ -504,7 +523,7 @@ __global__ void __launch_bounds__(kCopyWarps * 32)
 #pragma unroll
       for (int u = 0; u < D / 16; ++u) {
         const uint32_t a = jb < 4 ? w[u].x : w[u].y, b = jb < 4 ? w[u].z : w[u].w;
-        put2(to + u * 16, (float)(int8_t)(a >> (8 * (jb & 3))) * sc, (float)(int8_t)(b >> (8 * (jb & 3))) * sc);
+        put2(to + u * 16, int8_value(a, jb & 3) * sc, int8_value(b, jb & 3) * sc);
       }
     }
   }

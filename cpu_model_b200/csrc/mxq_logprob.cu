@@ -171,6 +171,28 @@ __device__ __forceinline__ void place_entries(const uint64_t* in, int n, int k, 
   }
 }
 
+// The same for `lists` ordered lists of MXQ_TOPK_MAX entries (0 beyond their
+// ends): an entry's place is its own in its list and, from each other list, the
+// entries above it.
+__device__ __forceinline__ void merge_entries(const uint64_t* in, int lists, int k, uint64_t* out, int threads) {
+  static_assert(MXQ_TOPK_MAX == 32, "five steps");
+  for (int i = threadIdx.x; i < lists * MXQ_TOPK_MAX; i += threads) {
+    const uint64_t e = in[i];
+    if (!e) continue;
+    int above = i % MXQ_TOPK_MAX;
+    for (int l = 0; l < lists; ++l) {
+      if (l == i / MXQ_TOPK_MAX) continue;
+      const uint64_t* p = in + l * MXQ_TOPK_MAX;
+      int n = 0;                   // entries of the list known to be above
+#pragma unroll
+      for (int step = 16; step > 0; step >>= 1)
+        if (p[n + step - 1] > e) n += step;
+      above += n + (p[n] > e);
+    }
+    if (above < k) out[above] = e;
+  }
+}
+
 // One row, `slices` CTAs (a cluster when there are several: few rows leave
 // SMs idle, and a row is long).  The top alternatives need no second pass
 // over the row: every group of THREADS / 32 threads knows its largest logit, so the
@@ -332,7 +354,7 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(LogprobArgs a) 
           sh.cand[e] = v;
         }
         __syncthreads();
-        place_entries(sh.cand, slices * MXQ_TOPK_MAX, a.k, sh.best, THREADS);
+        merge_entries(sh.cand, slices, a.k, sh.best, THREADS);
         __syncthreads();
       }
     }
@@ -499,8 +521,11 @@ cudaError_t launch_logprobs(const LogprobArgs& a, cudaStream_t st) {
 
 template <typename T>
 cudaError_t run_logprobs(const LogprobArgs& a, cudaStream_t st) {
-  // 512 threads only where each of them has two vectors of the row or more
-  return a.vocab / Vec<T>::kN < 1024 ? launch_logprobs<T, 128>(a, st) : launch_logprobs<T, 256>(a, st);
+  // a row that gives 512 threads less than two vectors each goes to 128; few rows
+  // to 512 (one row of 32000 fp32: 6.3 us, with 256 threads 8.3), many to 256, eight
+  // rows an SM at a time (8192 rows: 185 us, with 512 threads 226)
+  if (a.vocab / Vec<T>::kN < 1024) return launch_logprobs<T, 128>(a, st);
+  return a.rows < 2 * 148 ? launch_logprobs<T, 512>(a, st) : launch_logprobs<T, 256>(a, st);
 }
 
 template <typename T>
@@ -539,9 +564,9 @@ int mxq_token_logprobs(mxq_ctx c, int dtype, const void* logits, size_t row_stri
   ServeDevice g(ctx_device(c));
   LogprobArgs a{logits, (long)row_stride, (int)rows, (int)vocab, (int)top_k, 1,
                 target, logp, entropy, lse, top_logp, top_ids};
-  // a row is cut into slices while the rows alone leave SMs idle and a slice
-  // still has work for its threads
-  while (a.slices < kMaxSlices && rows * (size_t)a.slices < 148 && vocab / (size_t)(2 * a.slices) >= 4096) a.slices *= 2;
+  // a long row is cut into slices while the rows alone leave SMs idle: a cluster
+  // costs 2 us more than one CTA, which reads 256 KB in that time
+  while (a.slices < kMaxSlices && rows * (size_t)a.slices < 148 && vocab * es / (size_t)a.slices > (256u << 10)) a.slices *= 2;
   const cudaStream_t st = ctx_stream(c);
   const cudaError_t e = dtype == MXQ_DT_F32    ? run_logprobs<float>(a, st)
                         : dtype == MXQ_DT_BF16 ? run_logprobs<__nv_bfloat16>(a, st)
