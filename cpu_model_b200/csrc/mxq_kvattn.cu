@@ -44,6 +44,7 @@ constexpr int kStages = 2;               // blocks a warp has in its ring
 // blocks (192 unequal requests: 132 us with 1, 126 with 2, 121 with 4, 123 with 10).
 constexpr int kStart = 4;
 constexpr int kMinPiece = 1;             // places a piece at least
+constexpr int kWholeBlocks = 3;          // blocks a warp of a unit that a CTA keeps to itself, at most
 constexpr size_t kPromptUnits = 32;      // units of the prompts' kernel that are worth it
 constexpr float kLn2 = 0.693147180559945f;
 
@@ -563,23 +564,73 @@ __global__ void __launch_bounds__(Tile::kWarps * 32, 1) kv_attn_kernel(AttnArgs 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int Hkv = a.c.heads, G = a.G, nb = a.c.nb;
 
-  // ---- the line of work: units * places of every request, summed
-  {
+  // ---- the line of work: units * places of every request, summed.  A warp's
+  // worth of requests is summed by every warp for itself, without a barrier.
+  auto units_of = [&](int r, int* blocks) {
+    *blocks = 0;
+    if (r >= a.R) return 0;
+    const int rows = (row_start(a, r + 1) - row_start(a, r)) * G, len = a.ctx_len[r];
+    if (rows <= 0 || rows > a.few || len <= 0) return 0;
+    *blocks = (len + 31) >> 5;
+    return (rows + kRows - 1) / kRows * Hkv;
+  };
+  if (lane < 2) s_part[warp * 2 + lane].valid = 0;
+  const int pieces = gridDim.x * kWarps, piece = blockIdx.x * kWarps + warp;
+  long lo, hi, len;
+  int share = 0;                         // a unit a CTA: blocks of it a warp
+  if (a.R <= 32) {
+    int blocks;
+    const int u = units_of(lane, &blocks), most = __reduce_max_sync(0xffffffffu, blocks);
+    const long w = (long)u * (blocks + kStart);
+    long sum = w;
+    int units = u;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long x = __shfl_up_sync(0xffffffffu, sum, o);
+      const int y = __shfl_up_sync(0xffffffffu, units, o);
+      if (lane >= o) sum += x, units += y;
+    }
+    if (lane < a.R) s_sum[lane] = sum - w;           // every warp writes the same
+    const long total = __shfl_sync(0xffffffffu, sum, 31);
+    if (lane == 0) s_sum[a.R] = total;
+    __syncwarp();
+    // Few short units: a CTA each, its blocks shared out over the warps, and
+    // nothing to join outside it.  (At 36 blocks the SM that has them all takes as
+    // long as several would with the join through workspace, 4500 cycles.)
+    if (__shfl_sync(0xffffffffu, units, 31) <= (int)gridDim.x && most <= kWholeBlocks * kWarps) {
+      const uint32_t before = __ballot_sync(0xffffffffu, units <= (int)blockIdx.x);
+      const int r = __popc(before);                  // the request of this CTA's unit
+      if (r >= 32) {
+        lo = hi = 0;
+        len = 1;
+      } else {
+        const int nblk = __shfl_sync(0xffffffffu, blocks, r);
+        const int in = (int)blockIdx.x - __shfl_sync(0xffffffffu, units - u, r);
+        const long unit0 = __shfl_sync(0xffffffffu, sum - w, r) + (long)in * (nblk + kStart);
+        share = max(1, (nblk + kWarps - 1) / kWarps);
+        lo = unit0 + kStart + warp * share;
+        hi = min(lo + share, unit0 + kStart + nblk);
+        len = 1;
+      }
+    } else {
+      len = max(div_long(total + pieces - 1, pieces), (long)kMinPiece);
+      lo = piece * len;
+      hi = min(lo + len, total);
+    }
+  } else {
     long base = 0;
     for (int r0 = 0; r0 < a.R; r0 += kThreads) {
-      const int r = r0 + tid;
-      long w = 0;
-      if (r < a.R) {
-        const int rows = (row_start(a, r + 1) - row_start(a, r)) * G, len = a.ctx_len[r];
-        if (rows > 0 && rows <= a.few && len > 0) w = (long)((rows + kRows - 1) / kRows) * (((len + 31) >> 5) + kStart) * Hkv;
-      }
-      long s = w;
+      int blocks;
+      const int u = units_of(r0 + tid, &blocks);
+      const long w = (long)u * (blocks + kStart);
+      long sum = w;
+#pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const long u = __shfl_up_sync(0xffffffffu, s, o);
-        if (lane >= o) s += u;
+        const long x = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += x;
       }
       __syncthreads();
-      if (lane == 31) s_warp[warp] = s;
+      if (lane == 31) s_warp[warp] = sum;
       __syncthreads();
       long before = base;
 #pragma unroll
@@ -587,18 +638,14 @@ __global__ void __launch_bounds__(Tile::kWarps * 32, 1) kv_attn_kernel(AttnArgs 
         if (i < warp) before += s_warp[i];
         base += s_warp[i];
       }
-      if (r < a.R) s_sum[r] = before + s - w;
+      if (r0 + tid < a.R) s_sum[r0 + tid] = before + sum - w;
     }
     if (tid == 0) s_sum[a.R] = base;
-    if (tid < kWarps * 2) s_part[tid].valid = 0;
     __syncthreads();
+    len = max(div_long(base + pieces - 1, pieces), (long)kMinPiece);
+    lo = piece * len;
+    hi = min(lo + len, base);
   }
-  const long total = s_sum[a.R];
-  const int pieces = gridDim.x * kWarps;
-  long len = div_long(total + pieces - 1, pieces);
-  if (len < kMinPiece) len = kMinPiece;
-  const int piece = blockIdx.x * kWarps + warp;
-  const long lo = piece * len, hi = min(lo + len, total);
 
   uint8_t* ring = sm + warp * (kStages * kStage);
   const uint32_t ring_s = smem_u32(ring);
@@ -613,13 +660,14 @@ __global__ void __launch_bounds__(Tile::kWarps * 32, 1) kv_attn_kernel(AttnArgs 
     return x;
   };
 
-  // ---- places pos + lane: the block there and its scales (K | V << 8); -1: a page that holds no keys, or no block, or one that no row of the tile sees
+  // ---- places pos + lane: the page of the block there (look), and then where
+  // it is in the cache (seen; -1: a page that holds no keys, no block, or one that no
+  // row of the tile sees)
   long place = -1;
-  uint32_t place_sc = 0;
-  auto look_up = [&](long pos) {
+  int page = -1, page_head = 0, page_sub = 0;
+  auto look = [&](long pos) {
     pos += lane;
-    place = -1;
-    place_sc = 0;
+    page = -1;
     if (pos < hi) {
       const int r = request_of(pos);
       const int row0 = row_start(a, r), rows = (row_start(a, r + 1) - row0) * G, ctx = a.ctx_len[r];
@@ -628,17 +676,14 @@ __global__ void __launch_bounds__(Tile::kWarps * 32, 1) kv_attn_kernel(AttnArgs 
       const int unit = (int)div_long(in, per), b = (int)(in - (long)unit * per) - kStart;
       const int head = unit / tiles, tile = unit - head * tiles;
       const int last_row = min((tile + 1) * kRows, rows) - 1;
-      const int seen = ctx - rows / G + last_row / G + 1;
-      if (b >= 0 && b * 32 < seen) {
-        const int pg = b / nb;
-        const int page = pg < a.max_pages ? a.table[(long)r * a.max_pages + pg] : -1;
-        if (page >= 0 && page < a.c.n_pages) {
-          place = kv_block(a.c, page, head, b - pg * nb);
-          place_sc = (uint32_t)a.c.ks[place] | (uint32_t)a.c.vs[place] << 8;
-        }
-      }
+      const int sees = ctx - rows / G + last_row / G + 1;
+      const int pg = b / nb;
+      page_head = head;
+      page_sub = b - pg * nb;
+      if (b >= 0 && b * 32 < sees && pg < a.max_pages) page = a.table[(long)r * a.max_pages + pg];
     }
   };
+  auto seen = [&]() { place = page >= 0 && page < a.c.n_pages ? kv_block(a.c, page, page_head, page_sub) : -1; };
   const int mine = lo < hi ? (int)(hi - lo) : 0;
   // The ring holds the next two blocks (places without one are passed over):
   // where in the piece they are, their scales, and where in the cache.  K and V
@@ -646,12 +691,15 @@ __global__ void __launch_bounds__(Tile::kWarps * 32, 1) kv_attn_kernel(AttnArgs 
   // is still in use.
   int to_see = 0;                        // first place that has not been looked at
   int q_pos0 = -1, q_pos1 = -1;
-  uint32_t q_sc0 = 0, q_sc1 = 0;
+  uint32_t q_ks0 = 0, q_ks1 = 0, q_vs0 = 0, q_vs1 = 0;
   long q_at0 = 0, q_at1 = 0;
   auto fetch_k = [&](int s) {
     int found = -1;
     while (to_see < mine) {
-      if ((to_see & 31) == 0 && to_see) look_up(lo + to_see);
+      if ((to_see & 31) == 0 && to_see) {
+        look(lo + to_see);
+        seen();
+      }
       const uint32_t here = __ballot_sync(0xffffffffu, place >= 0) >> (to_see & 31);
       if (here) {
         found = to_see + __ffs((int)here) - 1;
@@ -664,9 +712,8 @@ __global__ void __launch_bounds__(Tile::kWarps * 32, 1) kv_attn_kernel(AttnArgs 
     else q_pos0 = found;
     if (found >= 0) {
       const long at = __shfl_sync(0xffffffffu, place, found & 31);
-      const uint32_t sc = __shfl_sync(0xffffffffu, place_sc, found & 31);
-      if (s) q_at1 = at, q_sc1 = sc;
-      else q_at0 = at, q_sc0 = sc;
+      if (s) q_at1 = at, q_ks1 = a.c.ks[at], q_vs1 = a.c.vs[at];
+      else q_at0 = at, q_ks0 = a.c.ks[at], q_vs0 = a.c.vs[at];
       const int8_t* src = a.c.k + at * (32 * D);
 #pragma unroll
       for (int u = 0; u < 2 * D / 32; ++u)
@@ -684,33 +731,50 @@ __global__ void __launch_bounds__(Tile::kWarps * 32, 1) kv_attn_kernel(AttnArgs 
     cp_commit();
   };
   int stage = 0;                         // of the next block
+
+  // ---- the unit at place i of the piece
+  int req = 0, row0 = 0, tile = 0, head = 0, nrows = 0, past = 0, end = 0, g_first = 0, g_last = 0;
+  long unit0 = 0;
+  bool has = false;                      // the piece has blocks of it to attend to (or all it has: none)
+  auto unit_at = [&](int i) {
+    const long pos = lo + i;
+    while (s_sum[req + 1] <= pos) ++req;
+    row0 = row_start(a, req);
+    const int rows = (row_start(a, req + 1) - row0) * G, ctx = a.ctx_len[req];
+    const int per = ((ctx + 31) >> 5) + kStart, tiles = (rows + kRows - 1) / kRows;
+    const long in = pos - s_sum[req];
+    const int unit = (int)div_long(in, per), skip = (int)(in - (long)unit * per);
+    head = unit / tiles;
+    tile = unit - head * tiles;
+    unit0 = pos - skip;
+    end = (int)min((long)mine, (long)i + per - skip);          // this piece's places of the unit: i .. end - 1
+    nrows = min(kRows, rows - tile * kRows);
+    past = ctx - rows / G;
+    // blocks with keys that the tile's last row sees
+    const int blocks = max(0, (min(ctx, past + (tile * kRows + nrows - 1) / G + 1) + 31) >> 5);
+    // the pieces with blocks of it
+    if (share) {
+      g_first = blockIdx.x * kWarps;
+      g_last = g_first + max(blocks - 1, 0) / share;
+    } else {
+      g_first = (int)div_long(unit0 + kStart, len);
+      g_last = blocks ? (int)div_long(unit0 + kStart + blocks - 1, len) : g_first;
+    }
+    has = blocks ? skip < kStart + blocks && skip + (end - i) > kStart
+                 : skip <= kStart && skip + (end - i) > kStart;   // a unit without keys: whoever has its first place
+  };
   if (mine) {
-    look_up(lo);
+    look(lo);                            // the pages are on their way while the unit is worked out
+    req = request_of(lo);
+    unit_at(0);
+    seen();
     fetch_k(0);
     fetch_v(0);
     fetch_k(1);
     fetch_v(1);
   }
-
-  int req = mine ? request_of(lo) : 0;
   for (int i = 0; i < mine;) {
-    const long pos = lo + i;
-    while (s_sum[req + 1] <= pos) ++req;
-    const int row0 = row_start(a, req), rows = (row_start(a, req + 1) - row0) * G, ctx = a.ctx_len[req];
-    const int per = ((ctx + 31) >> 5) + kStart, tiles = (rows + kRows - 1) / kRows;
-    const long in = pos - s_sum[req];
-    const int unit = (int)div_long(in, per), skip = (int)(in - (long)unit * per);
-    const int head = unit / tiles, tile = unit - head * tiles;
-    const long unit0 = pos - skip;
-    const int end = (int)min((long)mine, (long)i + per - skip);          // this piece's places of the unit: i .. end - 1
-    const int nrows = min(kRows, rows - tile * kRows);
-    const int past = ctx - rows / G;
-    // blocks with keys that the tile's last row sees
-    const int blocks = max(0, (min(ctx, past + (tile * kRows + nrows - 1) / G + 1) + 31) >> 5);
-    const int g_first = (int)div_long(unit0 + kStart, len), g_last = blocks ? (int)div_long(unit0 + kStart + blocks - 1, len) : g_first;
-    const bool has = blocks ? skip < kStart + blocks && skip + (end - i) > kStart
-                            : skip <= kStart && skip + (end - i) > kStart;   // a unit without keys: whoever has its first place
-
+    if (i) unit_at(i);
     Tile t;
     if (has) t.start(a, row0, tile, head, nrows, past);
     i = end;
@@ -718,10 +782,10 @@ __global__ void __launch_bounds__(Tile::kWarps * 32, 1) kv_attn_kernel(AttnArgs 
       const int at = stage ? q_pos1 : q_pos0;
       if (at < 0 || at >= end) break;
       uint8_t* st = ring + stage * kStage;
-      const uint32_t sc = stage ? q_sc1 : q_sc0;
+      const uint32_t ks = stage ? q_ks1 : q_ks0, vs = stage ? q_vs1 : q_vs0;
       cp_wait<2 * kStages - 1>();        // K is there; V and what follows may be on the way
       __syncwarp();
-      t.keys(st, ((int)(lo + at - unit0) - kStart) * 32, e8m0_to_float(sc & 0xFF), e8m0_to_float(sc >> 8), scratch);
+      t.keys(st, ((int)(lo + at - unit0) - kStart) * 32, e8m0_to_float(ks), e8m0_to_float(vs), scratch);
       __syncwarp();                      // every lane has read it before it is refilled
       fetch_k(stage);
       cp_wait<2 * kStages - 1>();        // V
@@ -770,31 +834,59 @@ __global__ void __launch_bounds__(Tile::kWarps * 32, 1) kv_attn_kernel(AttnArgs 
   }
   __syncthreads();                       // every part of this CTA is where its record says
 
-  // ---- the CTA's parts of each cut unit joined, in the order of the pieces
-  int groups = 0;
+  // ---- the CTA's parts of each cut unit joined, in the order of the pieces:
+  // records of one unit follow one another
+  static_assert(kWarps * 2 <= 32, "a record a lane");
+  const bool valid = lane < kWarps * 2 && s_part[lane].valid;
+  const uint32_t all = __ballot_sync(0xffffffffu, valid);
+  uint32_t starts;
+  {
+    const uint32_t below = all & ((1u << lane) - 1);
+    const bool first = !below || s_part[31 - __clz(below)].unit0 != s_part[lane < kWarps * 2 ? lane : 0].unit0;
+    starts = __ballot_sync(0xffffffffu, valid && first);
+  }
   int open[2] = {-1, -1};                // records of the units that go on outside this CTA
-  for (int g = 0; g < kWarps * 2;) {
-    if (!s_part[g].valid) {
-      ++g;
-      continue;
-    }
-    int n = 1;
-    while (g + n < kWarps * 2 && (!s_part[g + n].valid || s_part[g + n].unit0 == s_part[g].unit0)) ++n;
-    const Part p = s_part[g];
-    const int c_first = p.g_first / kWarps, c_last = p.g_last / kWarps;
-    const bool outside = c_first != c_last;
+  int groups = 0;
+  for (; starts; starts &= starts - 1, ++groups) {
+    const int g = __ffs((int)starts) - 1;
+    const uint32_t rest = starts & (starts - 1);     // the next unit's first record
+    const uint32_t group = all & ~((1u << g) - 1) & (rest ? (1u << (__ffs((int)rest) - 1)) - 1 : 0xffffffffu);
+    const Part& p = s_part[g];
+    const int p_nrows = p.nrows, c_first = p.g_first / kWarps;
+    const bool outside = c_first != p.g_last / kWarps;
     const int slot = c_first == (int)blockIdx.x ? 1 : 0;
     if (outside) open[slot] = g;
     float* to = a.cta_part + ((long)blockIdx.x * 2 + slot) * kPart;
     // small units start at different warps
-    for (int w = (tid + kThreads - (groups * 32) % kThreads) % kThreads; w < p.nrows * (D / 4); w += kThreads) {
+    for (int w = (tid + kThreads - (groups * 32) % kThreads) % kThreads; w < p_nrows * (D / 4); w += kThreads) {
       const int row = w / (D / 4), d = (w - row * (D / 4)) * 4;
       float m = neg_inf(), l = 0.0f;
       float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      for (int e = g; e < g + n; ++e) {
-        if (!s_part[e].valid) continue;
-        const float* q = s_part[e].at;
-        join(m, l, y, q[kRows * D + row], q[kRows * (D + 1) + row], *reinterpret_cast<const float4*>(q + row * D + d));
+      for (uint32_t left = group; left;) {           // four parts' loads at a time
+        float pm[4], pl[4];
+        float4 v[4];
+        bool real[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          real[e] = left != 0;
+          const float* q = s_part[left ? __ffs((int)left) - 1 : g].at;
+          pm[e] = real[e] ? q[kRows * D + row] : neg_inf();
+          pl[e] = q[kRows * (D + 1) + row];
+          v[e] = *reinterpret_cast<const float4*>(q + row * D + d);
+          left &= left - 1;
+        }
+        const float top = fmaxf(fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3])), m), ms = top == neg_inf() ? 0.0f : top;
+        const float fa = ex2(m - ms);
+        l *= fa;
+        y[0] *= fa; y[1] *= fa; y[2] *= fa; y[3] *= fa;
+        m = top;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (!real[e]) continue;
+          const float f = ex2(pm[e] - ms);
+          l += f * pl[e];
+          y[0] += f * v[e].x; y[1] += f * v[e].y; y[2] += f * v[e].z; y[3] += f * v[e].w;
+        }
       }
       if (!outside) {
         write_row<D>(a, p.row0, p.tile * kRows, row, p.head, d, y, m, l);
@@ -806,8 +898,6 @@ __global__ void __launch_bounds__(Tile::kWarps * 32, 1) kv_attn_kernel(AttnArgs 
         }
       }
     }
-    ++groups;
-    g += n;
   }
   if (open[0] < 0 && open[1] < 0) return;          // the same in every thread
   __threadfence();
@@ -824,21 +914,25 @@ __global__ void __launch_bounds__(Tile::kWarps * 32, 1) kv_attn_kernel(AttnArgs 
     __syncthreads();
     if (!s_flag) continue;
     __threadfence();
-    for (int w = tid; w < p.nrows * (D / 4); w += kThreads) {
-      const int row = w / (D / 4), d = (w - row * (D / 4)) * 4;
+    // several threads a result where there are few: each takes every crew-th part
+    const int tasks = p.nrows * (D / 4), crew = max(1, min(kThreads / tasks, parts));
+    float* s_join = reinterpret_cast<float*>(sm);  // [crew][tasks][6]
+    for (int w = tid; w < tasks * crew; w += kThreads) {
+      const int who = w / tasks, task = w - who * tasks, row = task / (D / 4), d = (task - row * (D / 4)) * 4;
       float m = neg_inf(), l = 0.0f;
       float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
       constexpr int kAhead = 8;
-      for (int i = 0; i < parts; i += kAhead) {
+      for (int i = who; i < parts; i += kAhead * crew) {
         float pm[kAhead], pl[kAhead];
         float4 v[kAhead];
 #pragma unroll
         for (int e = 0; e < kAhead; ++e) {
+          const int at = i + e * crew;
           pm[e] = neg_inf();
           pl[e] = 0.0f;
           v[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-          if (i + e < parts) {
-            const float* q = a.cta_part + ((long)(c_first + i + e) * 2 + (i + e == 0 ? 1 : 0)) * kPart;
+          if (at < parts) {
+            const float* q = a.cta_part + ((long)(c_first + at) * 2 + (at == 0 ? 1 : 0)) * kPart;
             pm[e] = __ldcg(q + kRows * D + row);
             pl[e] = __ldcg(q + kRows * (D + 1) + row);
             v[e] = __ldcg(reinterpret_cast<const float4*>(q + row * D + d));
@@ -847,7 +941,28 @@ __global__ void __launch_bounds__(Tile::kWarps * 32, 1) kv_attn_kernel(AttnArgs 
 #pragma unroll
         for (int e = 0; e < kAhead; ++e) join(m, l, y, pm[e], pl[e], v[e]);
       }
-      write_row<D>(a, p.row0, p.tile * kRows, row, p.head, d, y, m, l);
+      if (crew == 1) {
+        write_row<D>(a, p.row0, p.tile * kRows, row, p.head, d, y, m, l);
+      } else {
+        float* q = s_join + w * 6;
+        q[0] = m;
+        q[1] = l;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) q[2 + e] = y[e];
+      }
+    }
+    if (crew > 1) {
+      __syncthreads();
+      if (tid < tasks) {
+        const int row = tid / (D / 4), d = (tid - row * (D / 4)) * 4;
+        float m = neg_inf(), l = 0.0f;
+        float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int i = 0; i < crew; ++i) {
+          const float* q = s_join + (i * tasks + tid) * 6;
+          join(m, l, y, q[0], q[1], make_float4(q[2], q[3], q[4], q[5]));
+        }
+        write_row<D>(a, p.row0, p.tile * kRows, row, p.head, d, y, m, l);
+      }
     }
   }
 }
