@@ -261,7 +261,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(KvPromptAr
   const uint32_t tmem = s_tmem;
   const int units = s_sum[a.R];
 
+  // A hand-over comes soon, as a rule: 32 polls that do not put the warp to sleep first
+  // (4 prompts of 900 to 2048 rows: 291 us without, 282 with 8, 280 with 32, 284 with 64).
+  // Lanes may leave at different polls: what needs the warp together says so.
   auto wait = [&](uint64_t* b, uint32_t parity) {
+    for (int i = 0; i < 32; ++i)
+      if (mbar_test_wait(b, parity & 1u)) return;
     if (!s_dead && !mbar_wait(b, parity & 1u, a.status)) s_dead = 1;
   };
 
@@ -372,6 +377,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(KvPromptAr
         const uint32_t tp = ts + place * 64;
         const uint32_t before = place ? taken0 : taken1;               // P left in the other place
         wait(&bar.sfull[x][place], place ? taken1 : taken0);
+        __syncwarp();
         taken0 += place ^ 1;
         taken1 += place;
         tc_fence_after();
@@ -415,6 +421,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(KvPromptAr
           if (j > 0) {
             // the product before this one; the one before that ended before this S began
             wait(&bar.pvdone[x][place ^ 1], before - 1);
+            __syncwarp();
             tc_fence_after();
 #pragma unroll 1
             for (int k = 0; k < D / 16; ++k) {
@@ -484,6 +491,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(KvPromptAr
       if (my > 0) {
         const bool second = !(my & 1);
         wait(&bar.pvdone[x][second], (second ? taken1 : taken0) - 1);   // the last product, and so all
+        __syncwarp();
         tc_fence_after();
       }
       const float inv = l == 0.0f ? 0.0f : unscale / l;
