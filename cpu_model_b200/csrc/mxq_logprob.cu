@@ -8,9 +8,9 @@
 // Forward: one pass over the row; every thread keeps (M, s, u) of what it has
 // read and rescales when its M rises, so the row is read from memory once.
 // Both directions are bound by HBM: a pass has nothing to reuse.  8192 rows of
-// 32000 fp32 logits with 5 alternatives: 186 us, 5.6 TB/s, 86 % of a copy; the
-// gradient of 4096 x 32000 bf16: 87.6 us, 6.0 TB/s, 91 %.  One row of 32000 is
-// bound by latency: 6.5 us.
+// 32000 fp32 logits with 5 alternatives: 167 us, 6.3 TB/s, 96 % of a copy; the
+// gradient of 4096 x 32000 bf16: 82.5 us, 6.35 TB/s, 97 %.  One row of 32000 is
+// bound by latency: 5.9 us.
 #include "mxq_serve.cuh"
 
 namespace mxq {
@@ -61,13 +61,21 @@ __device__ __forceinline__ Stat shfl_xor(const Stat& a, int o) {
           __shfl_xor_sync(0xffffffffu, a.u, o)};
 }
 
-// N values into a thread's statistics.
+// Where a thread's largest value is: its batch, and the largest of its other batches.
+struct Largest {
+  int at;                          // the batch's first vector, -1: the ends of the row
+  float other;
+};
+
+// N values, the batch `at`, into a thread's statistics.
 template <int N>
-__device__ __forceinline__ void add_values(Stat& t, const float (&x)[N]) {
+__device__ __forceinline__ void add_values(Stat& t, Largest& g, int at, const float (&x)[N]) {
   float top = x[0];
 #pragma unroll
   for (int i = 1; i < N; ++i) top = fmaxf(top, x[i]);
+  g.other = fmaxf(g.other, fminf(top, t.m));
   if (top > t.m) {
+    g.at = at;
     const float f = floor_max(top), d = drop(floor_max(t.m) - f), c = exp2_approx(d * kLog2e);
     t.u = c * (t.u + t.s * d);
     t.s *= c;
@@ -199,23 +207,27 @@ __device__ __forceinline__ void merge_entries(const uint64_t* in, int lists, int
 // One row, `slices` CTAs (a cluster when there are several: few rows leave
 // SMs idle, and a row is long).  The top alternatives need no second pass
 // over the row: every group of THREADS / 32 threads knows its largest logit, so the
-// k-th largest of these 32 is a bound that at least k logits reach; only the parts
-// of threads whose own maximum reaches it are looked through again.
+// k-th largest of these 32 is a bound that at least k logits reach.  A thread whose
+// own maximum reaches it reads the batch of 8 that has it again, and all of its part
+// only where another of its batches reaches the bound too.
 template <typename T, int THREADS>
 __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(LogprobArgs a) {
   __shared__ LogprobShared<THREADS> sh;
-  constexpr int kN = Vec<T>::kN, kAhead = 4;
+  // vectors a thread has on the way: 8 where many rows share an SM (8192 rows: 167 us,
+  // with 4 173, with 12 186), 4 where one row's latency counts (5.9 us, with 8 6.3)
+  constexpr int kN = Vec<T>::kN, kAhead = THREADS == 256 ? 8 : 4;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int slices = a.slices, rank = slices > 1 ? (int)cluster_ctarank() : 0;
   const long row = blockIdx.x / slices;
   const RowView<T> rv(static_cast<const T*>(a.logits) + row * a.stride, a.vocab);
 
   Stat t{-__int_as_float(0x7f800000), 0.0f, 0.0f};
+  Largest g{-1, t.m};
   bool any = false;
   if (rank == 0) {
     for (int i = tid; i < rv.head + rv.tail; i += THREADS) {
       const float v[1] = {to_f32(rv.x[rv.end(i)])};
-      add_values(t, v);
+      add_values(t, g, -1, v);
       any = true;
     }
   }
@@ -238,7 +250,7 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(LogprobArgs a) 
         const int nx = i + (kAhead + u + q) * step;
         if (nx < rv.nv) w[u + q] = __ldcs(rv.body + nx);
       }
-      add_values(t, v);
+      add_values(t, g, i + u * step, v);
     }
   }
 #pragma unroll
@@ -246,7 +258,7 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(LogprobArgs a) 
     if (i + u * step < rv.nv) {
       float v[kN];
       unpack16<T>(w[u], v);
-      add_values(t, v);
+      add_values(t, g, i + u * step, v);
     }
   const uint32_t mine = any ? order_key(t.m) : 0u;
 
@@ -256,11 +268,11 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(LogprobArgs a) 
   for (int o = 16; o > 0; o >>= 1) r = merge(r, shfl_xor(r, o));
   if (lane == 0) sh.warp[warp] = r;
   if (a.k > 0) {
-    uint32_t g = mine;
+    uint32_t top = mine;
     constexpr int kGroup = THREADS / 32;
 #pragma unroll
-    for (int o = kGroup / 2; o > 0; o >>= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, o));
-    if (tid % kGroup == 0) sh.group[tid / kGroup] = g;
+    for (int o = kGroup / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (tid % kGroup == 0) sh.group[tid / kGroup] = top;
   }
   if (tid == 0) sh.count = 0;
   if (tid < MXQ_TOPK_MAX) sh.best[tid] = 0;
@@ -287,7 +299,6 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(LogprobArgs a) 
     const uint32_t least = sh.threshold;
     const bool odd = !(sh.all.s == sh.all.s);     // a NaN or +inf among them: the maxima are not to be trusted
     if (!odd) {
-      // a warp looks through the part of each of its lanes in turn, a vector a lane
       const float bound = key_value(least);       // least 0: a group without logits, every logit counts
       auto test = [&](float x, int id) {
         if (least == 0u || x >= bound) {
@@ -295,7 +306,22 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(LogprobArgs a) 
           if (at < kCandidates) sh.cand[at] = order_entry(x, id);
         }
       };
-      for (uint32_t left = __ballot_sync(0xffffffffu, any && mine >= least); left; left &= left - 1) {
+      const bool reaches = any && mine >= least;
+      const bool many = reaches && (least == 0u || g.other >= bound);
+      if (reaches && !many) {
+        // one batch: its second vector is a batch of its own near the row's end, and below the bound
+        if (g.at < 0)
+          test(to_f32(rv.x[rv.end(tid)]), rv.end(tid));
+        else
+          for (int q = 0; q < kPair && g.at + q * step < rv.nv; ++q) {
+            float v[kN];
+            unpack16<T>(__ldg(rv.body + g.at + q * step), v);
+#pragma unroll
+            for (int e = 0; e < kN; ++e) test(v[e], rv.head + (g.at + q * step) * kN + e);
+          }
+      }
+      // several: a warp looks through the part of each such lane in turn, a vector a lane
+      for (uint32_t left = __ballot_sync(0xffffffffu, many); left; left &= left - 1) {
         const int who = warp * 32 + __ffs((int)left) - 1;
         if (rank == 0 && lane == 0 && who < rv.head + rv.tail) test(to_f32(rv.x[rv.end(who)]), rv.end(who));
         for (int j = rank * THREADS + who + lane * step; j < rv.nv; j += 32 * step) {
@@ -418,8 +444,10 @@ template <> __device__ __forceinline__ void store16(__half* p, const float* v) {
 }
 
 constexpr int kGradThreads = 256;
-constexpr int kGradBatch = 4;      // vectors a thread has on the way
-constexpr int kGradLoops = 4;      // times that, a CTA
+// vectors a thread has on the way, and times that, a CTA (4096 rows of 32000 bf16:
+// 82.5 us with 2 and 2, 85.2 with 4 and 2, 88.2 with 4 and 4)
+constexpr int kGradBatch = 2;
+constexpr int kGradLoops = 2;
 
 // dx_j = dlogp (1[j = t] - p_j) - dentropy p_j (log p_j + H): 16-byte stores at
 // the gradient's alignment, the logits in 16 bytes where they share it.  The
@@ -525,8 +553,8 @@ cudaError_t launch_logprobs(const LogprobArgs& a, cudaStream_t st) {
 template <typename T>
 cudaError_t run_logprobs(const LogprobArgs& a, cudaStream_t st) {
   // a row that gives 512 threads less than two vectors each goes to 128; few rows
-  // to 512 (one row of 32000 fp32: 6.3 us, with 256 threads 8.3), many to 256, eight
-  // rows an SM at a time (8192 rows: 185 us, with 512 threads 226)
+  // to 512 (one row of 32000 fp32: 5.9 us, with 256 threads 7.0), many to 256, several
+  // rows an SM at a time (8192 rows: 167 us, with 512 threads 227)
   if (a.vocab / Vec<T>::kN < 1024) return launch_logprobs<T, 128>(a, st);
   return a.rows < 2 * 148 ? launch_logprobs<T, 512>(a, st) : launch_logprobs<T, 256>(a, st);
 }
