@@ -8,9 +8,9 @@
 // Forward: one pass over the row; every thread keeps (M, s, u) of what it has
 // read and rescales when its M rises, so the row is read from memory once.
 // Both directions are bound by HBM: a pass has nothing to reuse.  8192 rows of
-// 32000 fp32 logits with 5 alternatives: 167 us, 6.3 TB/s, 96 % of a copy; the
-// gradient of 4096 x 32000 bf16: 82.5 us, 6.35 TB/s, 97 %.  One row of 32000 is
-// bound by latency: 5.9 us.
+// 32000 fp32 logits with 5 alternatives: 167 us launch after launch, 173 with cold
+// caches, 6.1 TB/s, 93 % of a copy; the gradient of 4096 x 32000 bf16: 82.5 us, 6.35
+// TB/s.  One row of 32000 is bound by latency: 5.9 us.
 #include "mxq_serve.cuh"
 
 namespace mxq {
