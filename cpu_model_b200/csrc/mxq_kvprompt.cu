@@ -268,7 +268,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(KvPromptAr
 
   // A hand-over comes soon, as a rule: 32 polls that do not put the warp to sleep first
   // (4 prompts of 900 to 2048 rows: 291 us without, 282 with 8, 280 with 32, 284 with 64).
-  // Lanes may leave at different polls: what needs the warp together says so.
+  // Lanes may leave at different polls: a wait that an instruction of the whole warp
+  // (tcgen05.ld, .st and .wait, bar.sync) follows has a __syncwarp behind it.
   auto wait = [&](uint64_t* b, uint32_t parity) {
     for (int i = 0; i < 32; ++i)
       if (mbar_test_wait(b, parity & 1u)) return;
@@ -443,6 +444,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(KvPromptAr
         const float base = m == neg_inf() ? 0.0f : m - kLift;
         if (j == 0) {
           wait(&bar.vfull[kt & 1], kt >> 1);     // the unit's V exponents are known
+          __syncwarp();
           const int2 e = v_range();
           half = e.x - e.y <= 32;
           unscale = pow2_exact(e.x - 127 - 8);
@@ -522,6 +524,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(KvPromptAr
             dst[c / 8] = make_uint4(w[0], w[1], w[2], w[3]);
           }
         }
+        __syncwarp();                            // rows that are not there are back for the next load
       }
       if (valid && a.lse) a.lse[at] = l == 0.0f ? neg_inf() : (m - kLift) * kLn2 + logf(l);
       tc_fence_before();                         // O may be written over after the next unit's barrier
@@ -606,6 +609,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(KvPromptAr
         top = __reduce_max_sync(0xffffffffu, top);
         low = __reduce_min_sync(0xffffffffu, low);
         if (lane == 0) s_top[w] = top, s_low[w] = low;
+        __syncwarp();
         asm volatile("bar.sync 2, 128;" ::: "memory");
       }
       const int2 range = v_range();
@@ -759,6 +763,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(KvPromptAr
   if (warp == 12 || warp == 13) {
     if (elect_one()) mma_commit(&bar.drain);
     (void)mbar_wait(&bar.drain, 0, a.status);
+    __syncwarp();
   }
   __syncthreads();
   if (warp == 12) tmem_dealloc(tmem, 512);

@@ -437,3 +437,11 @@ def test_refusals(ctx):
             mx.kv_attention(**{**ok, **change})
     out, lse = mx.kv_attention(c.q[:0], c.cache(), c.table, c.ctx_len, torch.zeros(2, dtype=torch.int32, device="cuda"))
     assert out.shape == (0, 4, 64) and lse.shape == (0, 4)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [64, 128])
+def test_prompts_behind_a_long_prefix(ctx, D, dtype):
+    """V's exponents of a whole prefix are searched before a unit's first
+    probabilities: the softmax's wait for them is a long one, and ends the sleeping way."""
+    Case([(20000, 300), (15001, 33)], 8, 4, D, 64, dtype, seed=51).check(ctx)
