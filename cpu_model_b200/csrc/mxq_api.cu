@@ -7,6 +7,7 @@
 #include <cstdio>
 #include <cstring>
 #include <cstdarg>
+#include <memory>
 #include <new>
 #include <string>
 #include <vector>
@@ -72,12 +73,17 @@ struct mxq_context {
   static constexpr size_t kMaxHostGraphs = 64;
   std::vector<HostGraph> graphs;
   uint64_t graph_clock = 0;
-  // serving operators: one workspace for each stream they ran on
-  struct StreamWs {
-    cudaStream_t stream;
+  // serving operators: one workspace for each stream they ran on, and one for
+  // each stream of a capture (a graph keeps its addresses and may be replayed
+  // on any stream, beside calls on the one it was captured on)
+  struct ServeSlot {
     uint8_t* base;
+    cudaStream_t stream;
+    unsigned long long stream_id;   // another stream may get the handle later, none the id (unused in captures)
+    unsigned long long capture_id;  // 0: calls that run at once
+    std::shared_ptr<std::atomic<bool>> held;   // by a graph; false once every graph that has it is gone
   };
-  std::vector<StreamWs> serve_ws;
+  std::vector<ServeSlot> serve_ws;
   int sms = 0;
 };
 
@@ -134,6 +140,49 @@ int ensure(mxq_context* c, T*& p, size_t& cap, size_t bytes, const char* what) {
   p = static_cast<T*>(q);
   cap = bytes;
   return MXQ_OK;
+}
+
+// A serving workspace with its counters at zero, while a stream of this thread may
+// be capturing: the calls are not the capture's, and no stream waits for them.
+cudaError_t serve_alloc(uint8_t** out) {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  cudaError_t e = cudaThreadExchangeStreamCaptureMode(&mode);
+  if (e != cudaSuccess) return e;
+  void* p = nullptr;
+  cudaStream_t st = nullptr;
+  e = cudaMalloc(&p, kServeCounters * 4 + kServeScratch);
+  if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking);
+  if (e == cudaSuccess) e = cudaMemsetAsync(p, 0, kServeCounters * 4, st);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  if (st) cudaStreamDestroy(st);
+  if (e != cudaSuccess) cudaFree(p);
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  if (e == cudaSuccess) *out = static_cast<uint8_t*>(p);
+  return e;
+}
+
+// The slot stays with the graph, its copies and what is instantiated of them.
+cudaError_t serve_hold(mxq_context::ServeSlot& s, cudaGraph_t graph) {
+  using Flag = std::shared_ptr<std::atomic<bool>>;
+  s.held = std::make_shared<std::atomic<bool>>(true);
+  Flag* f = new Flag(s.held);
+  cudaUserObject_t obj;
+  cudaError_t e = cudaUserObjectCreate(
+      &obj, f,
+      [](void* p) {
+        Flag* flag = static_cast<Flag*>(p);
+        (*flag)->store(false);
+        delete flag;
+      },
+      1, cudaUserObjectNoDestructorSync);
+  if (e != cudaSuccess) {
+    s.held->store(false);
+    delete f;
+    return e;
+  }
+  e = cudaGraphRetainUserObject(graph, obj, 1, cudaGraphUserObjectMove);
+  if (e != cudaSuccess) cudaUserObjectRelease(obj, 1);
+  return e;
 }
 
 // A workspace of counters that the kernels using it leave zero: zeroed once
@@ -2339,28 +2388,54 @@ uint64_t ctx_ws_gen(mxq_context* c) { return c->ws_gen; }
 uint64_t ctx_launches(mxq_context* c) { return c->launches; }
 
 int ctx_serve_ws(mxq_context* c, ServeWs* out) {
+  auto broken = [&](cudaError_t e) {
+    cudaGetLastError();
+    return cuda_fail(c, e, "serving workspace");
+  };
   try {
-    uint8_t* base = nullptr;
-    for (auto& w : c->serve_ws)
-      if (w.stream == c->stream) base = w.base;
-    if (!base) {
-      if (c->sms == 0) {
-        const cudaError_t e = cudaDeviceGetAttribute(&c->sms, cudaDevAttrMultiProcessorCount, c->device);
-        if (e != cudaSuccess) return cuda_fail(c, e, "multiprocessor count");
-      }
-      c->serve_ws.reserve(c->serve_ws.size() + 1);
-      void* p = nullptr;
-      cudaError_t e = cudaMalloc(&p, kServeCounters * 4 + kServeScratch);
-      if (e == cudaSuccess) e = cudaMemsetAsync(p, 0, kServeCounters * 4, c->stream);
-      if (e != cudaSuccess) {
-        cudaFree(p);
-        return cuda_fail(c, e, "serving workspace");
-      }
-      base = static_cast<uint8_t*>(p);
-      c->serve_ws.push_back({c->stream, base});
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    unsigned long long id = 0, capture = 0;
+    cudaGraph_t graph = nullptr;
+    cudaError_t e = cudaStreamGetCaptureInfo(c->stream, &status, &capture, &graph);
+    const bool capturing = e == cudaSuccess && status != cudaStreamCaptureStatusNone;
+    if (!capturing) capture = 0;
+    if (e == cudaSuccess && !capturing) e = cudaStreamGetId(c->stream, &id);   // which a capture does not allow
+    if (e != cudaSuccess) return broken(e);
+    mxq_context::ServeSlot *mine = nullptr, *spare = nullptr, *gone = nullptr;
+    for (auto& s : c->serve_ws) {
+      const bool held = !s.held || s.held->load();
+      if (!held) spare = &s;                         // every graph that had it is gone, and has ended
+      else if (s.stream != c->stream || s.capture_id != capture) continue;
+      else if (capturing || s.stream_id == id) mine = &s;
+      else gone = &s;                                // of a stream that is no more
     }
-    out->counters = reinterpret_cast<uint32_t*>(base);
-    out->scratch = base + kServeCounters * 4;
+    if (!mine) {
+      if (c->sms == 0) {
+        e = cudaDeviceGetAttribute(&c->sms, cudaDevAttrMultiProcessorCount, c->device);
+        if (e != cudaSuccess) return broken(e);
+      }
+      if (!spare && gone && cudaDeviceSynchronize() == cudaSuccess) spare = gone;   // its last calls have ended
+      if (!spare) {
+        c->serve_ws.reserve(c->serve_ws.size() + 1);
+        uint8_t* base = nullptr;
+        e = serve_alloc(&base);
+        if (e != cudaSuccess) return broken(e);
+        c->serve_ws.push_back({base, nullptr, 0, 0, std::make_shared<std::atomic<bool>>(false)});
+        spare = &c->serve_ws.back();
+      }
+      if (capturing) {
+        e = serve_hold(*spare, graph);
+        if (e != cudaSuccess) return broken(e);
+      } else {
+        spare->held = nullptr;
+      }
+      spare->stream = c->stream;
+      spare->stream_id = id;
+      spare->capture_id = capture;
+      mine = spare;
+    }
+    out->counters = reinterpret_cast<uint32_t*>(mine->base);
+    out->scratch = mine->base + kServeCounters * 4;
     out->sms = c->sms;
     return MXQ_OK;
   } catch (...) {

@@ -236,12 +236,14 @@ uint64_t ctx_launches(mxq_context* c);
 void ctx_set_launches(mxq_context* c, uint64_t n);
 const WeightView* weight_view(mxq_weight w);
 
-// Workspace of the serving operators (mxq_kv.cu, mxq_kvattn.cu), one for each
-// stream that a context has used them on, so that calls on two streams do not
-// meet in it: counters that every kernel leaves zero, then bytes that hold
-// nothing from one call to the next.
+// Workspace of the serving operators (mxq_kv.cu, mxq_kvattn.cu): counters that
+// every kernel leaves zero, then bytes that hold nothing from one call to the
+// next.  There is one for each stream that a context has used them on, and one
+// for each stream of a capture, which its graph keeps: calls on two streams
+// and replays of two graphs do not meet in it, on whatever streams they run.
+// (One graph's replays that run at once would meet, as they would in its outputs.)
 constexpr size_t kServeCounters = 2048;                  // uint32
-constexpr size_t kServeScratch = 24u << 20;              // bytes
+constexpr size_t kServeScratch = 13u << 20;              // bytes
 struct ServeWs {
   uint32_t* counters;
   uint8_t* scratch;

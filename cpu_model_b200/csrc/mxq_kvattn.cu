@@ -45,7 +45,6 @@ namespace mxq {
 
 namespace {
 
-constexpr int kMaxWarps = 12;
 constexpr int kMaxRows = 16;             // query rows a unit
 constexpr int kStages = 2;               // blocks a warp has in its ring
 // Places a unit's start takes: what its rows, their end and the join cost, in
@@ -564,6 +563,7 @@ __global__ void __launch_bounds__(Tile::kWarps * 32, 1) kv_attn_kernel(AttnArgs 
   constexpr int kPart = (kRows * (D + 2) + 3) / 4 * 4;   // floats of a part, whole 16-byte pieces
   constexpr int kStage = 64 * D;                   // one block's K and V
   static_assert(kPart * 4 <= kStages * kStage, "a part takes its warp's ring");
+  static_assert(kWarps * kPart <= 8 * kMaxRows * (D + 2) && kPart <= kMaxRows * (D + 2), "parts take their place in the workspace");
   extern __shared__ __align__(16) uint8_t sm[];
   uint8_t* scratch = sm + kWarps * kStages * kStage + (threadIdx.x >> 5) * 128;   // a tile's own
   long* s_sum = reinterpret_cast<long*>(sm + kWarps * (kStages * kStage + 128));  // [R + 1]
@@ -1043,14 +1043,14 @@ int mxq_kv_attention(mxq_ctx c, const mxq_kv_cache* cache, int dtype, const void
   a.max_pages = (int)max_pages;
   a.scale2 = scale * 1.44269504088896341f;
   a.counters = ws.counters + 1;
-  // a part for each warp and two for each CTA
-  const size_t per = kMaxRows * (size_t)(kv.dim + 2) * 4;
+  // a part for each warp (12 of up to 8 rows, or 8 of 16) and two for each CTA
+  const size_t row = (size_t)(kv.dim + 2) * 4, warp_parts = 8 * kMaxRows * row;
   int ctas = ws.sms;
-  const int fit = (int)(kServeScratch / ((kMaxWarps + 2) * per));
+  const int fit = (int)(kServeScratch / (warp_parts + 2 * kMaxRows * row));
   if (ctas > fit) ctas = fit;
   if (ctas > (int)kServeCounters - 3) ctas = (int)kServeCounters - 3;
   a.warp_part = reinterpret_cast<float*>(ws.scratch);
-  a.cta_part = reinterpret_cast<float*>(ws.scratch + (size_t)ctas * kMaxWarps * per);
+  a.cta_part = reinterpret_cast<float*>(ws.scratch + (size_t)ctas * warp_parts);
   const size_t rows = max_new * (size_t)a.G;
   a.few = 1 << 30;
   // Prompts' 16-bit rows go to the tensor cores' kernel where they fill at

@@ -624,7 +624,15 @@ typedef struct mxq_kv_cache {
  *                    the slots of their rows, and the entries of the table
  *                    that it has for them, are -1
  * ctx_len may be past and free_out may be free_count (in place).  n_req <=
- * MXQ_KV_MAX_REQUESTS; lengths and their sums fit int32. */
+ * MXQ_KV_MAX_REQUESTS; lengths and their sums fit int32.
+ *
+ * This call and mxq_kv_attention work in a workspace that the context keeps:
+ * one for each stream, and one for each stream of a capture, which belongs to
+ * the graph that is made (and is used again when the graph and all that was
+ * instantiated of it are gone).  So calls on different streams, and replays of
+ * different graphs on any streams, run beside one another.  The first call
+ * on a stream or in a capture may allocate it; graphs must go before the
+ * context does. */
 MXQ_API int mxq_kv_plan(mxq_ctx ctx, const int32_t* past, const int32_t* add,
                         size_t n_req, size_t page_size, int32_t* table,
                         size_t max_pages, const int32_t* free_pages,
@@ -668,9 +676,7 @@ MXQ_API int mxq_kv_read(mxq_ctx ctx, const mxq_kv_cache* cache,
  * logarithm of the softmax's denominator.  A row that sees no key, or that
  * belongs to no request (rows from cu[n_req] on), gets 0 and -inf.  Pages
  * outside the pool hold no keys.  max_new >= every request's number of new rows (more is safe; it only
- * chooses the kernel).  The call works in a workspace that the context
- * keeps for each stream (made by the first call there, which therefore must
- * not be one that is being captured). */
+ * chooses the kernel).  Its workspace: see mxq_kv_plan. */
 MXQ_API int mxq_kv_attention(mxq_ctx ctx, const mxq_kv_cache* cache, int dtype,
                              const void* q, size_t q_stride, size_t n,
                              size_t n_heads, const int32_t* table,

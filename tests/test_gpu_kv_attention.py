@@ -9,6 +9,8 @@ bound of the other fp32 results.  bf16 / fp16 rows: the result's own rounding is
 query's 15 bits an error of s below 2^-16 max|q| sum|k| scale, about 1e-4 here:
 2^-9 + 2e-4 and 2^-12 + 4e-4.  lse: 2e-6 |lse| + 2e-6 in fp32, that error
 of s (5e-4 bounds it) in 16 bits."""
+import ctypes
+
 import numpy as np
 import pytest
 import torch
@@ -445,3 +447,97 @@ def test_prompts_behind_a_long_prefix(ctx, D, dtype):
     """V's exponents of a whole prefix are searched before a unit's first
     probabilities: the softmax's wait for them is a long one, and ends the sleeping way."""
     Case([(20000, 300), (15001, 33)], 8, 4, D, 64, dtype, seed=51).check(ctx)
+
+
+def capture(stream, f):
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=stream):
+        out = f()
+    return g, out
+
+
+SHARED = {
+    "joined": lambda i: Case([(9000 + 500 * i, 1), (40, 1)], 2, 2, 128, 64, torch.bfloat16, seed=60 + i),
+    "prompts": lambda i: Case([(900, 700), (1300, 1000 + i)], 8, 2, 128, 64, torch.bfloat16, seed=64 + i)}
+
+
+@pytest.mark.parametrize("kind", sorted(SHARED))
+def test_graphs_of_one_stream_replayed_on_two(ctx, kind):
+    """Graphs captured on one stream run at the same time on others, and beside
+    calls on the stream that they were captured on."""
+    cs = [SHARED[kind](i) for i in range(3)]
+    want = [c.run(ctx) for c in cs]
+    s = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    graphs = [capture(s[0], lambda c=c: c.run(ctx)) for c in cs[:2]]
+    for _ in range(3):
+        eager = []
+        for i in range(2):
+            graphs[i][1][0].zero_()
+            graphs[i][1][1].zero_()
+        torch.cuda.synchronize()
+        for _ in range(15):
+            for i in range(2):
+                with torch.cuda.stream(s[1 + i]):
+                    graphs[i][0].replay()
+            with torch.cuda.stream(s[0]):
+                eager.append(cs[2].run(ctx))
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert torch.equal(graphs[i][1][0], want[i][0]) and torch.equal(graphs[i][1][1], want[i][1])
+        for o, l in eager:
+            assert torch.equal(o, want[2][0]) and torch.equal(l, want[2][1])
+
+
+def test_first_call_in_a_capture():
+    """A capture on a stream that has not been used before, by a context that has no workspace yet."""
+    c = Case([(3000, 1), (200, 1)], 2, 4, 128, 64, torch.float32, seed=67)
+    want, _ = c.ref()
+    fresh = mx.MXContext(0)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out, _ = c.run(fresh)
+    g.replay()
+    torch.cuda.synchronize()
+    assert float((out.double() - want).norm() / want.norm()) <= TOL[torch.float32]
+    a = c.run(fresh)[0]
+    assert torch.equal(a, out)
+    del g
+    torch.cuda.synchronize()
+    fresh.close()
+
+
+def test_workspaces_of_graphs_and_streams_that_are_gone_are_used_again(ctx):
+    """Forty graphs, and forty streams, one after another, do not keep a workspace each (13 MB)."""
+    c = Case([(3000, 1), (200, 1)], 2, 4, 128, 64, torch.bfloat16, seed=68)
+    want = c.run(ctx)[0]
+    s = torch.cuda.Stream()
+
+    def once():
+        g, (out, _) = capture(s, lambda: c.run(ctx))
+        with torch.cuda.stream(s):
+            g.replay()
+        s.synchronize()
+        assert torch.equal(out, want)
+        del g, out
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+
+    def own_stream():
+        rt, h = torch.cuda.cudart(), ctypes.c_void_p()
+        assert int(rt.cudaStreamCreate(ctypes.addressof(h))) == 0
+        with torch.cuda.stream(torch.cuda.ExternalStream(h.value)):
+            out = c.run(ctx)[0]
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        ctx._bind()                                  # a context's stream outlives its use there
+        assert int(rt.cudaStreamDestroy(h.value)) == 0
+        return h.value
+
+    for f in (once, own_stream):
+        f()
+        f()
+        before = torch.cuda.mem_get_info()[0]
+        handles = {f() for _ in range(40)}
+        used = (before - torch.cuda.mem_get_info()[0]) / 2 ** 20
+        assert used <= 13 * (len(handles) + 4), (f.__name__, used, len(handles))

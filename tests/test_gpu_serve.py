@@ -446,3 +446,31 @@ def test_two_streams_share_no_workspace(ctx):
     for p in out:
         np.testing.assert_array_equal(p.slots.cpu().numpy(), ref[3])
         assert int(p.free_count) == ref[6] and p.ctx_len.tolist() == ref[1]
+
+
+def test_plans_captured_on_one_stream_run_on_two(ctx):
+    """Plans of many CTAs, captured on one stream, replayed on two at once."""
+    cases = [plan_case(5000, 200, 20, 32, 77 + i) for i in range(2)]
+    s = [torch.cuda.Stream() for _ in range(3)]
+    graphs = []
+    for past, add, table, stack, n_pages in cases:
+        n = int(add.sum())
+        free = cuda(np.concatenate([stack, np.full(n_pages - len(stack), -1)]), torch.int32)
+        args = [cuda(past), cuda(add), 32, cuda(table), free, cuda([len(stack)], torch.int32), n]
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s[0]):
+            p = mx.kv_plan(*args, ctx=ctx)
+        graphs.append((g, p, args, plan_ref(past, add, 32, table, stack, n)))
+    torch.cuda.synchronize()
+    for _ in range(30):
+        for i, (g, p, args, ref) in enumerate(graphs):
+            with torch.cuda.stream(s[1 + i]):
+                p.slots.zero_()
+                p.ctx_len.zero_()
+                g.replay()
+    torch.cuda.synchronize()
+    for g, p, args, ref in graphs:
+        np.testing.assert_array_equal(p.slots.cpu().numpy(), ref[3])
+        np.testing.assert_array_equal(args[3].cpu().numpy(), ref[0])
+        assert int(p.free_count) == ref[6] and p.ctx_len.tolist() == ref[1]
