@@ -84,7 +84,7 @@ __global__ void __launch_bounds__(1024) kv_plan_kernel(PlanArgs a) {
   int over = 0;
   int2 mine = make_int2(0, 0);
   for (int r = r0; r < r1; ++r) {
-    const int have = (len[r] + a.P - 1) / a.P, full = (len[r] + cu[r] + a.P - 1) / a.P;
+    const int have = ceil_div(len[r], a.P), full = ceil_div(len[r] + cu[r], a.P);
     const int w = min(full, a.max_pages) - min(have, a.max_pages);
     over += full - have - w;       // pages beyond the table's width
     pf[r] = w;
@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(1024) kv_plan_kernel(PlanArgs a) {
 
   for (int j = t0; j < wanted; j += step) {
     const int r = last_not_above(pf, a.R, j);
-    const int have = (len[r] + a.P - 1) / a.P, from = height - 1 - j;
+    const int have = ceil_div(len[r], a.P), from = height - 1 - j;
     a.table[(long)r * a.max_pages + have + (j - pf[r])] = from >= 0 ? a.free_pages[from] : -1;
   }
   for (int i = t0; i < a.N; i += step) {
@@ -121,8 +121,8 @@ __global__ void __launch_bounds__(1024) kv_plan_kernel(PlanArgs a) {
       req = last_not_above(cu, a.R, i);
       const int p = len[req];
       pos = p + (i - cu[req]);
-      const int have = (p + a.P - 1) / a.P, pi = pos / a.P;
-      if (pi < a.max_pages) {
+      const int have = ceil_div(p, a.P), pi = pos / a.P;
+      if (pos >= 0 && pi < a.max_pages) {
         const int from = height - 1 - (pf[req] + pi - have);
         const int page = pi < have ? a.table[(long)req * a.max_pages + pi] : from >= 0 ? a.free_pages[from] : -1;
         if (page >= 0 && page < a.n_pages) slot = page * a.P + (pos - pi * a.P);
@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(1024) kv_release_kernel(const uint8_t* done, i
   int base = 0;
   for (int r0 = 0; r0 < R; r0 += nt) {
     const int r = r0 + tid;
-    const int w = r < R && done[r] ? min((at_least_0(len[r]) + P - 1) / P, max_pages) : 0;
+    const int w = r < R && done[r] ? min(ceil_div(len[r], P), max_pages) : 0;
     int2 total;
     const int s = block_scan(make_int2(w, 0), sums, &total).x;
     if (r < R) pf[r] = base + s - w;

@@ -575,12 +575,13 @@ __global__ void __launch_bounds__(Tile::kWarps * 32, 1) kv_attn_kernel(AttnArgs 
 
   // ---- the line of work: units * places of every request, summed.  A warp's
   // worth of requests is summed by every warp for itself, without a barrier.
+  auto blocks_of = [&](int ctx) { return ceil_div(table_keys(a.c, a.max_pages, ctx), 32); };
   auto units_of = [&](int r, int* blocks) {
     *blocks = 0;
     if (r >= a.R) return 0;
     const int rows = (row_start(a, r + 1) - row_start(a, r)) * G, len = a.ctx_len[r];
     if (rows <= 0 || rows > a.few || len <= 0) return 0;
-    *blocks = (len + 31) >> 5;
+    *blocks = blocks_of(len);
     return (rows + kRows - 1) / kRows * Hkv;
   };
   if (lane < 2) s_part[warp * 2 + lane].valid = 0;
@@ -680,7 +681,7 @@ __global__ void __launch_bounds__(Tile::kWarps * 32, 1) kv_attn_kernel(AttnArgs 
     if (pos < hi) {
       const int r = request_of(pos);
       const int row0 = row_start(a, r), rows = (row_start(a, r + 1) - row0) * G, ctx = a.ctx_len[r];
-      const int per = ((ctx + 31) >> 5) + kStart, tiles = (rows + kRows - 1) / kRows;
+      const int per = blocks_of(ctx) + kStart, tiles = (rows + kRows - 1) / kRows;
       const long in = pos - s_sum[r];
       const int unit = (int)div_long(in, per), b = (int)(in - (long)unit * per) - kStart;
       const int head = unit / tiles, tile = unit - head * tiles;
@@ -750,7 +751,7 @@ __global__ void __launch_bounds__(Tile::kWarps * 32, 1) kv_attn_kernel(AttnArgs 
     while (s_sum[req + 1] <= pos) ++req;
     row0 = row_start(a, req);
     const int rows = (row_start(a, req + 1) - row0) * G, ctx = a.ctx_len[req];
-    const int per = ((ctx + 31) >> 5) + kStart, tiles = (rows + kRows - 1) / kRows;
+    const int per = blocks_of(ctx) + kStart, tiles = (rows + kRows - 1) / kRows;
     const long in = pos - s_sum[req];
     const int unit = (int)div_long(in, per), skip = (int)(in - (long)unit * per);
     head = unit / tiles;
@@ -760,7 +761,7 @@ __global__ void __launch_bounds__(Tile::kWarps * 32, 1) kv_attn_kernel(AttnArgs 
     nrows = min(kRows, rows - tile * kRows);
     past = ctx - rows / G;
     // blocks with keys that the tile's last row sees
-    const int blocks = max(0, (min(ctx, past + (tile * kRows + nrows - 1) / G + 1) + 31) >> 5);
+    const int blocks = blocks_of(min(ctx, past + (tile * kRows + nrows - 1) / G + 1));
     // the pieces with blocks of it
     if (share) {
       g_first = blockIdx.x * kWarps;

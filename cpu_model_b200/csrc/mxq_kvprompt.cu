@@ -309,10 +309,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(KvPromptAr
     u.first = (tiles - 1 - in / Hkv) * 256;
     u.past = u.ctx - u.rows / G;
     const int end_a = min(u.first + 128, u.rows), end_b = min(u.first + 256, u.rows);
-    u.see_a = max(0, min(u.ctx, u.past + (end_a - 1) / G + 1));
-    u.see_b = end_b > u.first + 128 ? max(0, min(u.ctx, u.past + (end_b - 1) / G + 1)) : 0;
-    u.na = (u.see_a + kStepKeys - 1) / kStepKeys;
-    u.nb = (u.see_b + kStepKeys - 1) / kStepKeys;
+    u.see_a = table_keys(a.c, a.max_pages, min(u.ctx, u.past + (end_a - 1) / G + 1));
+    u.see_b = end_b > u.first + 128 ? table_keys(a.c, a.max_pages, min(u.ctx, u.past + (end_b - 1) / G + 1)) : 0;
+    u.na = ceil_div(u.see_a, kStepKeys);
+    u.nb = ceil_div(u.see_b, kStepKeys);
     u.n = (max(u.na, u.nb) + 1) >> 1;
     return true;
   };
@@ -534,7 +534,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(KvPromptAr
     asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
     for (; next(un); kt += un.n) {
       const int w = warp - 8, ct = tid - 256, req = un.req, head = un.head, n = un.n;
-      const int nblk = (max(un.see_a, un.see_b) + 31) >> 5;
+      const int nblk = ceil_div(max(un.see_a, un.see_b), 32);
       // lanes 0-3: block 4 j + lane of tile j and its scales
       auto look = [&](int j, long& pl, uint32_t& sc) {
         pl = -1;

@@ -45,6 +45,17 @@ __host__ __device__ __forceinline__ int v_offset(int t, int d) {
   return ((d >> 1) * 4 + ((t >> 1) & 3)) * 16 + (d & 1) * 8 + (t >> 3) * 2 + (t & 1);
 }
 
+// ceil(x / d), 0 for x < 0: for every int x (x + d - 1 may not be one).
+__host__ __device__ __forceinline__ int ceil_div(int x, int d) {
+  return x > 0 ? (int)(((unsigned)x + (unsigned)d - 1) / (unsigned)d) : 0;
+}
+
+// Keys and blocks of a request that its block table has places for: no more is
+// looked at, however long the request says it is.
+__device__ __forceinline__ int table_keys(const KvView& c, int max_pages, int len) {
+  return (int)min((long)max_pages * c.page, (long)max(len, 0));
+}
+
 // ------------------------------------------------------------- row types --
 template <typename T> __device__ __forceinline__ float to_f32(T x);
 template <> __device__ __forceinline__ float to_f32(float x) { return x; }

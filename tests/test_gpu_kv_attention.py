@@ -541,3 +541,24 @@ def test_workspaces_of_graphs_and_streams_that_are_gone_are_used_again(ctx):
         handles = {f() for _ in range(40)}
         used = (before - torch.cuda.mem_get_info()[0]) / 2 ** 20
         assert used <= 13 * (len(handles) + 4), (f.__name__, used, len(handles))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("new", [1, 3, 300])
+def test_lengths_near_the_end_of_int32(ctx, new, dtype):
+    """A request that says it is 2^31 - 1 tokens long, with pages for 96 of them: each of its rows sees those."""
+    c = Case([(96, 96)] * 2, 8, 4, 64, 32, dtype, seed=53, extra_rows=2 * new)
+    q = c.q[:2 * new]
+    cu = torch.tensor([0, new, 2 * new], dtype=torch.int32, device="cuda")
+    for length in (2 ** 31 - 1, 2 ** 31 - 31, 2 ** 31 - 65):
+        lens = torch.tensor([length, 2 ** 31 - 1], dtype=torch.int32, device="cuda")
+        out, lse = mx.kv_attention(q, c.cache(), c.table, lens, cu, max_new=new, ctx=ctx)
+        ctx.synchronize()
+        for r in range(2):
+            for h in range(8):
+                k, v, _ = c.dense(r, h, 96)
+                rows = slice(r * new, r * new + new)
+                s = torch.einsum("tgd,ld->tgl", q[rows, 4 * h:4 * h + 4].double(), k) / 8
+                want, got = torch.softmax(s, -1) @ v, out[rows, 4 * h:4 * h + 4].double()
+                assert float((got - want).norm() / want.norm()) <= TOL[dtype]
+                assert float((lse[rows, 4 * h:4 * h + 4].double() - torch.logsumexp(s, -1)).abs().max()) <= 5e-4

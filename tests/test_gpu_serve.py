@@ -474,3 +474,30 @@ def test_plans_captured_on_one_stream_run_on_two(ctx):
         np.testing.assert_array_equal(p.slots.cpu().numpy(), ref[3])
         np.testing.assert_array_equal(args[3].cpu().numpy(), ref[0])
         assert int(p.free_count) == ref[6] and p.ctx_len.tolist() == ref[1]
+
+
+@pytest.mark.parametrize("P", [32, 1024])
+def test_lengths_near_the_end_of_int32(ctx, P):
+    """Lengths whose next page's end is no int32: pages and slots as page by page, and their pages come back."""
+    top = 2 ** 31 - 1
+    past, add = np.array([5, top - 40, 0, top, 33], np.int32), np.array([3, 40, 40, 0, 7], np.int32)
+    table = np.full((5, 3), -1, np.int32)
+    held = iter(range(20))
+    for r in range(5):
+        for j in range(min(3, -(-int(past[r]) // P))):
+            table[r, j] = next(held)
+    stack = np.arange(20, 27, dtype=np.int32)
+    free = np.concatenate([stack, np.full(23, -1, np.int32)])
+    n = 92
+    ref = plan_ref([int(x) for x in past], [int(x) for x in add], P, table, stack, n)
+    d = [cuda(past), cuda(table), cuda(free), cuda([7], torch.int32)]
+    p = mx.kv_plan(d[0], cuda(add), P, d[1], d[2], d[3], n, in_place=True, ctx=ctx)
+    ctx.synchronize()
+    for got, want in ((d[1], ref[0]), (p.ctx_len, ref[1]), (p.cu, ref[2]), (p.slots, ref[3]), (p.positions, ref[4]), (p.requests, ref[5]),
+                      (p.free_count, [ref[6]]), (p.short, [ref[7]])):
+        np.testing.assert_array_equal(got.cpu().numpy(), np.asarray(want, np.int32))
+    mx.kv_release(cuda(np.ones(5, np.uint8)), d[0], P, d[1], d[2], d[3], ctx=ctx)
+    assert (d[1] == -1).all() and (d[0] == 0).all()
+    owned = int((ref[0] >= 0).sum())
+    assert int(d[3]) == ref[6] + owned
+    assert d[2][ref[6]:ref[6] + owned].tolist() == [int(x) for x in ref[0].flatten() if x >= 0]
