@@ -89,6 +89,7 @@ struct KVCache {
     want(v_scale, at::kByte, "v_scale");
     if (k.dim() != 5 || k.size(3) != kBlock) refuse("k must be [n_pages][heads][blocks][32][head_dim]");
     const int64_t n = k.size(0), h = k.size(1), nb = k.size(2), d = k.size(4);
+    if (k.numel() == 0) refuse("kv cache: no pages, heads, blocks or dimensions");
     if (v.sizes() != at::IntArrayRef({n, h, nb, d / 2, 4, 2, 8}))
       refuse("v must be [n_pages][heads][blocks][head_dim / 2][4][2][8]");
     if (k_scale.sizes() != at::IntArrayRef({n, h, nb}) || v_scale.sizes() != at::IntArrayRef({n, h, nb}))

@@ -501,3 +501,11 @@ def test_lengths_near_the_end_of_int32(ctx, P):
     owned = int((ref[0] >= 0).sum())
     assert int(d[3]) == ref[6] + owned
     assert d[2][ref[6]:ref[6] + owned].tolist() == [int(x) for x in ref[0].flatten() if x >= 0]
+
+
+@pytest.mark.parametrize("n,h,nb,d", [(2, 0, 1, 64), (0, 2, 1, 64), (2, 2, 0, 64), (2, 2, 1, 0)])
+def test_caches_of_nothing_are_refused(n, h, nb, d):
+    i8 = lambda *s: torch.zeros(s, dtype=torch.int8, device="cuda")
+    u8 = lambda: torch.zeros((n, h, nb), dtype=torch.uint8, device="cuda")
+    with pytest.raises(ValueError):
+        mx.KVCache(i8(n, h, nb, 32, d), i8(n, h, nb, d // 2, 4, 2, 8), u8(), u8())
