@@ -170,11 +170,11 @@ struct Top {                             // what probability 1 is in fixed point
 
 // Rows of a unit in the MMA's layout: 8 or 16 of them (16 where a unit has more
 // than 8, so that a block is read half as often).
-template <int D_, int MT, int NP>
+template <int D_, int MT, int NP, int W>
 struct MmaTile {
   static constexpr int D = D_;
   static constexpr int kRows = 8 * MT;
-  static constexpr int kWarps = MT == 1 ? 12 : 8;
+  static constexpr int kWarps = W;
   static constexpr int kJ = D / 64;                       // 64-dimension halves
   static constexpr int kU = D / 16;                       // V words of 16 dimensions
   static constexpr int kTiles = MT == 1 ? 2 : 3;          // MMA row tiles of S: upper digits of 8 rows each, then the lowest
@@ -387,11 +387,11 @@ struct MmaTile {
 // seven of its eight rows empty; dp4a takes the same digits with a lane for each
 // token (S, no sums across lanes) and a lane for every D / 32 dimensions (O): under half
 // the instructions.
-template <int D_, int NP>
+template <int D_, int NP, int W>
 struct DotTile {
   static constexpr int D = D_;
   static constexpr int kRows = 1;
-  static constexpr int kWarps = 12;
+  static constexpr int kWarps = W;
   static constexpr int kW = D / 4;                        // words of a K row
   static constexpr int kPairs = D / 64;                   // dimension pairs a lane: lane, lane + 32
 
@@ -977,23 +977,52 @@ __global__ void __launch_bounds__(Tile::kWarps * 32, 1) kv_attn_kernel(AttnArgs 
   }
 }
 
+// A ring a warp, and the requests' sums.
+template <typename Tile>
+constexpr size_t attn_smem(size_t requests) {
+  return (size_t)Tile::kWarps * (kStages * 64 * Tile::D + 128) + (requests + 1) * 8;
+}
+constexpr size_t kSmemLimit = 227u << 10, kSmemStatic = 1536;   // of a CTA; what the kernel's own variables may take of it
+
 template <typename Tile>
 cudaError_t launch(const AttnArgs& a, int ctas, cudaStream_t st) {
   static SmemAttr attr;
-  const size_t smem = (size_t)Tile::kWarps * (kStages * 64 * Tile::D + 128) + ((size_t)a.R + 1) * 8;
+  const size_t smem = attn_smem<Tile>(a.R);
   const cudaError_t e = attr.ensure(kv_attn_kernel<Tile>, smem);
   if (e != cudaSuccess) return e;
   kv_attn_kernel<Tile><<<(unsigned)ctas, Tile::kWarps * 32, smem, st>>>(a);
   return cudaGetLastError();
 }
 
+// A tile with 12 warps a CTA, or with 10 where the sums of thousands of
+// requests would not fit beside 12 rings (D = 128, from 4096 requests on; 8
+// K/V heads, 150 to 350 tokens each, one fp32 row: 4095 requests 426 us, 4096
+// 462; four bf16 rows: 455 and 453).
+template <template <int> class Tile>
+cudaError_t launch_warps(const AttnArgs& a, int ctas, cudaStream_t st) {
+  static_assert(attn_smem<Tile<10>>(MXQ_KV_MAX_REQUESTS) + kSmemStatic <= kSmemLimit, "every number of requests fits");
+  if constexpr (attn_smem<Tile<12>>(MXQ_KV_MAX_REQUESTS) + kSmemStatic > kSmemLimit)
+    if (attn_smem<Tile<12>>(a.R) + kSmemStatic > kSmemLimit) return launch<Tile<10>>(a, ctas, st);
+  return launch<Tile<12>>(a, ctas, st);
+}
+template <int D, int NP> struct Rows {
+  template <int W> using One = DotTile<D, NP, W>;
+  template <int W> using Eight = MmaTile<D, 1, NP, W>;
+  using Sixteen = MmaTile<D, 2, NP, 8>;
+  static_assert(attn_smem<Sixteen>(MXQ_KV_MAX_REQUESTS) + kSmemStatic <= kSmemLimit, "every number of requests fits");
+};
+
 // One row a unit, eight while no request has more (16-row tiles spend twice the
 // registers on them), else sixteen.
+template <int D, int NP>
+cudaError_t launch_rows(const AttnArgs& a, size_t rows, int ctas, cudaStream_t st) {
+  if (rows == 1) return launch_warps<Rows<D, NP>::template One>(a, ctas, st);
+  if (rows <= 8) return launch_warps<Rows<D, NP>::template Eight>(a, ctas, st);
+  return launch<typename Rows<D, NP>::Sixteen>(a, ctas, st);
+}
 template <int D>
 cudaError_t launch_rows(const AttnArgs& a, size_t rows, bool f32, int ctas, cudaStream_t st) {
-  if (rows == 1) return f32 ? launch<DotTile<D, 3>>(a, ctas, st) : launch<DotTile<D, 2>>(a, ctas, st);
-  if (rows <= 8) return f32 ? launch<MmaTile<D, 1, 3>>(a, ctas, st) : launch<MmaTile<D, 1, 2>>(a, ctas, st);
-  return f32 ? launch<MmaTile<D, 2, 3>>(a, ctas, st) : launch<MmaTile<D, 2, 2>>(a, ctas, st);
+  return f32 ? launch_rows<D, 3>(a, rows, ctas, st) : launch_rows<D, 2>(a, rows, ctas, st);
 }
 
 int bad(mxq_context* c, const char* msg) { return ctx_fail(c, MXQ_ERR_INVALID_ARGUMENT, msg); }

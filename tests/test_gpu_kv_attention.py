@@ -562,3 +562,33 @@ def test_lengths_near_the_end_of_int32(ctx, new, dtype):
                 want, got = torch.softmax(s, -1) @ v, out[rows, 4 * h:4 * h + 4].double()
                 assert float((got - want).norm() / want.norm()) <= TOL[dtype]
                 assert float((lse[rows, 4 * h:4 * h + 4].double() - torch.logsumexp(s, -1)).abs().max()) <= 5e-4
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("G", [1, 4])
+@pytest.mark.parametrize("R", [500, 4095, 4096, 4130, 8192])
+def test_thousands_of_requests(ctx, R, G, dtype):
+    """As many requests as kv_plan takes, short ones and a few long enough to be cut."""
+    g = synth.rng(R)
+    lens = g.integers(1, 70, R)
+    far = g.integers(0, R, 5)
+    lens[far] = g.integers(2000, 6000, 5)
+    c = Case([(int(n), 1) for n in lens], 1, G, 128, 32, dtype, seed=54)
+    out, lse = c.run(ctx)
+    ctx.synchronize()
+    # the first 96 keys of every request at once, then the long ones by themselves
+    ids = c.table[:, :3].long().clamp(min=0)
+    two = lambda x: torch.exp2(x.double() - 127)[..., None, None]
+    k = (c.k[ids, 0, 0].double() * two(c.ks[ids, 0, 0])).reshape(R, 96, 128)
+    v = (c.v[ids, 0, 0].flatten(2)[:, :, v_index(128).cuda()].double() * two(c.vs[ids, 0, 0])).reshape(R, 96, 128)
+    s = torch.einsum("rgd,rld->rgl", c.q.double(), k) * 128 ** -0.5
+    s.masked_fill_(torch.arange(96, device="cuda") >= c.ctx_len[:, None, None], -float("inf"))
+    want, wl = torch.softmax(s, -1) @ v, torch.logsumexp(s, -1)
+    for r in set(far.tolist()):
+        k, v, _ = c.dense(r, 0, int(lens[r]))
+        s = torch.einsum("gd,ld->gl", c.q[r].double(), k) * 128 ** -0.5
+        want[r], wl[r] = torch.softmax(s, -1) @ v, torch.logsumexp(s, -1)
+    err = (out.double() - want).norm(dim=2) / want.norm(dim=2)
+    assert float(err.max()) <= 4 * TOL[dtype] and float((out.double() - want).norm() / want.norm()) <= TOL[dtype]
+    tol = 2e-6 * wl.abs() + 2e-6 if dtype == torch.float32 else 5e-4
+    assert ((lse.double() - wl).abs() <= tol).all()
