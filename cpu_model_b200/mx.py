@@ -852,6 +852,18 @@ def token_logprobs_grad(logits, targets, lse, entropy, dlogp=None, dentropy=None
     return _serve.token_logprobs_grad(_address(ctx, logits), logits, targets, lse, entropy, dlogp, dentropy, out)
 
 
+class _TokenLogpGrad(torch.autograd.Function):
+    """token_logprobs_grad where a graph of the backward pass is recorded: its
+    own derivative is refused instead of taken for 0."""
+    @staticmethod
+    def forward(ctx, logits, targets, lse, entropy, dlogp, dentropy):
+        return token_logprobs_grad(logits, targets, lse, entropy, dlogp, dentropy)
+
+    @staticmethod
+    def backward(ctx, _):
+        raise RuntimeError("token_logp has no second derivative")
+
+
 class _TokenLogp(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets):
@@ -863,12 +875,13 @@ class _TokenLogp(torch.autograd.Function):
     def backward(ctx, dlogp, dentropy):
         logits, targets, lse, entropy = ctx.saved_tensors
         flat = lambda g: None if g is None else g.contiguous()
-        return token_logprobs_grad(logits, targets, lse, entropy, flat(dlogp), flat(dentropy)), None
+        return _TokenLogpGrad.apply(logits, targets, lse, entropy, flat(dlogp), flat(dentropy)), None
 
 
 def token_logp(logits, targets):
     """(logp [N], entropy [N]) of given tokens, differentiable in the logits
-    (the policy-gradient and entropy terms of a rollout update)."""
+    (the policy-gradient and entropy terms of a rollout update), once: a second
+    derivative is refused."""
     return _TokenLogp.apply(logits, targets)
 
 
