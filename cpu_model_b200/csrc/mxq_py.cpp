@@ -54,6 +54,12 @@ void same_device(const Tensor& first, std::initializer_list<const Tensor*> other
 // The outputs and their views are made below autograd: nothing here is recorded.
 using Below = at::AutoDispatchBelowADInplaceOrView;
 
+// Tensors that a call has written into: a graph that saved one is told.
+void written(std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
 // The context, bound to the current stream of the tensors' device.
 mxq_ctx bind(uintptr_t ctx, const Tensor& on) {
   mxq_ctx c = reinterpret_cast<mxq_ctx>(ctx);
@@ -131,6 +137,8 @@ py::tuple kv_plan(uintptr_t ctx, const Tensor& past, const Tensor& add, int64_t 
                     in_place ? ptr<int32_t>(past) : at + rest + 2, at + 3 * n, at, at + n, at + 2 * n, n,
                     in_place ? ptr<int32_t>(free_count) : at + rest + 1, at + rest),
         ctx);
+  written({&table});
+  if (in_place) written({&past, &free_count});
   return py::make_tuple(len, buf.narrow(0, 3 * n, r + 1), buf.narrow(0, 0, n), buf.narrow(0, n, n), buf.narrow(0, 2 * n, n),
                         left, buf.narrow(0, rest, 1));
 }
@@ -151,6 +159,7 @@ void kv_release(uintptr_t ctx, const Tensor& done, const Tensor& lengths, int64_
   check(mxq_kv_release(bind(ctx, lengths), ptr<uint8_t>(done), ptr<int32_t>(lengths), r, page_size, ptr<int32_t>(table),
                        table.size(1), ptr<int32_t>(free_pages), free_pages.numel(), ptr<int32_t>(free_count)),
         ctx);
+  written({&lengths, &table, &free_pages, &free_count});
 }
 
 void kv_append(uintptr_t ctx, const KVCache& cache, const Tensor& k, const Tensor& v, const Tensor& slots) {
@@ -165,6 +174,7 @@ void kv_append(uintptr_t ctx, const KVCache& cache, const Tensor& k, const Tenso
   if (row_stride(v, "v") != stride) refuse("kv_append: k and v must have the same row stride");
   same_device(cache.k, {&k, &v, &slots});
   check(mxq_kv_append(bind(ctx, k), &cache.c, dt, k.data_ptr(), v.data_ptr(), stride, ptr<int32_t>(slots), n), ctx);
+  written({&cache.k, &cache.v, &cache.k_scale, &cache.v_scale});
 }
 
 py::tuple kv_read(uintptr_t ctx, const KVCache& cache, const Tensor& slots, at::ScalarType type) {
@@ -258,6 +268,7 @@ Tensor token_logprobs_grad(uintptr_t ctx, const Tensor& logits, const Tensor& ta
                                 ptr<int32_t>(targets), ptr<float>(lse), ptr<float>(entropy), ptr<float>(dlogp),
                                 ptr<float>(dentropy), g.data_ptr(), row_stride(g, "out")),
         ctx);
+  if (out) written({&g});
   return g;
 }
 

@@ -264,3 +264,18 @@ def test_refusals(ctx):
         with pytest.raises(ValueError):
             f()
     assert mx.token_logprobs(x[:0], t[:0], 2).top_ids.shape == (0, 2)
+
+
+def test_gradient_into_the_logits_raises_their_version(ctx):
+    """A graph that has saved the logits does not go on with what was written over them."""
+    x, t = rows_of(4, 300, torch.float32, 9)
+    r = mx.token_logprobs(x, t, ctx=ctx)
+    w = torch.ones(4, 300, device="cuda", requires_grad=True)
+    y = (x * w).sum()                                 # saves x
+    mx.token_logprobs_grad(x, t, r.lse, r.entropy, torch.ones(4, device="cuda"), out=x, ctx=ctx)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    out = torch.empty_like(x)
+    before = out._version
+    assert mx.token_logprobs_grad(x, t, r.lse, r.entropy, torch.ones(4, device="cuda"), out=out, ctx=ctx) is out
+    assert out._version > before

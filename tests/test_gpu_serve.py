@@ -509,3 +509,26 @@ def test_caches_of_nothing_are_refused(n, h, nb, d):
     u8 = lambda: torch.zeros((n, h, nb), dtype=torch.uint8, device="cuda")
     with pytest.raises(ValueError):
         mx.KVCache(i8(n, h, nb, 32, d), i8(n, h, nb, d // 2, 4, 2, 8), u8(), u8())
+
+
+def test_versions_of_what_is_written(ctx):
+    """Every tensor that a call writes into says so to autograd."""
+    P, H, D = 32, 1, 64
+    cache = mx.KVCache.empty(4, P, H, D)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    lens, table, free, count = i32(0, 0), i32([-1, -1], [-1, -1]), i32(0, 1, 2, 3), i32(4)
+
+    def raised(tensors, f):
+        before = [t._version for t in tensors]
+        r = f()
+        assert all(t._version > b for t, b in zip(tensors, before))
+        return r
+    p = raised([table], lambda: mx.kv_plan(lens, i32(3, 1), P, table, free, count, 4, ctx=ctx))
+    raised([table, lens, count], lambda: mx.kv_plan(lens, i32(3, 1), P, table, free, count, 4, in_place=True, ctx=ctx))
+    x = torch.randn((4, H, D), device="cuda")
+    raised([cache.k, cache.v, cache.k_scale, cache.v_scale], lambda: mx.kv_append(cache, x, x, p.slots, ctx=ctx))
+    raised([lens, table, free, count], lambda: mx.kv_release(i32(1, 1).bool(), lens, P, table, free, count, ctx=ctx))
+    with torch.inference_mode():
+        y = torch.zeros((2, 5), device="cuda")
+        r = mx.token_logprobs(y, i32(0, 1), ctx=ctx)
+        mx.token_logprobs_grad(y, i32(0, 1), r.lse, r.entropy, torch.ones(2, device="cuda"), out=y, ctx=ctx)
