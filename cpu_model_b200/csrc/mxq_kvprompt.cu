@@ -342,30 +342,29 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(KvPromptAr
           w[ch] = make_uint4(0, 0, 0, 0);
           if (valid) w[ch] = __ldg(reinterpret_cast<const uint4*>(from) + ch);
         }
-        float lift = 1.0f;
-        if (kBf16) {
-          uint32_t top = 0;                      // the largest |q|, as bf16 bits
+        uint32_t top = 0;                        // the largest |q|, as its type's bits
 #pragma unroll
-          for (int ch = 0; ch < D / 8; ++ch) {
-            const uint32_t m0 = __vmaxu2(w[ch].x & 0x7FFF7FFFu, w[ch].y & 0x7FFF7FFFu);
-            top = __vmaxu2(top, __vmaxu2(m0, __vmaxu2(w[ch].z & 0x7FFF7FFFu, w[ch].w & 0x7FFF7FFFu)));
-          }
-          top = max(top & 0xFFFFu, top >> 16);
-          const int e = (int)(top >> 7);         // its exponent field; 255: inf or NaN
-          // 2^(14 - exponent): |q| below 2^15
-          const int up = min(14 - (e - 127), 126);
-          lift = e == 255 ? 0.0f : __int_as_float((up + 127) << 23);
-          qs = e == 255 ? __int_as_float(0x7fc00000) : qs * __int_as_float((127 - up) << 23);
+        for (int ch = 0; ch < D / 8; ++ch) {
+          const uint32_t m0 = __vmaxu2(w[ch].x & 0x7FFF7FFFu, w[ch].y & 0x7FFF7FFFu);
+          top = __vmaxu2(top, __vmaxu2(m0, __vmaxu2(w[ch].z & 0x7FFF7FFFu, w[ch].w & 0x7FFF7FFFu)));
         }
+        top = max(top & 0xFFFFu, top >> 16);
+        const bool finite = top < (kBf16 ? 0x7F80u : 0x7C00u);
+        float lift = 1.0f;
+        if (kBf16 && finite) {
+          // 2^(14 - exponent): |q| below 2^15
+          const int up = min(14 - ((int)(top >> 7) - 127), 126);
+          lift = __int_as_float((up + 127) << 23);
+          qs *= __int_as_float((127 - up) << 23);
+        }
+        if (!finite) qs = __int_as_float(0x7fc00000);      // a row with an inf or a NaN is NaN by its scale
 #pragma unroll
         for (int ch = 0; ch < D / 8; ++ch) {
           uint32_t v[4] = {w[ch].x ^ flip, w[ch].y ^ flip, w[ch].z ^ flip, w[ch].w ^ flip};
           if (kBf16)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              v[e] = pack_f16(__uint_as_float(v[e] << 16) * lift, __uint_as_float(v[e] & 0xFFFF0000u) * lift);
-              if (lift == 0.0f) v[e] = 0;        // inf or NaN: the row is NaN by its scale
-            }
+            for (int e = 0; e < 4; ++e) v[e] = pack_f16(__uint_as_float(v[e] << 16) * lift, __uint_as_float(v[e] & 0xFFFF0000u) * lift);
+          if (!finite) v[0] = v[1] = v[2] = v[3] = 0;
           *reinterpret_cast<uint4*>(to + (ch >> 3) * (128 * 128) + sw128_offset(tid & 127, ch & 7)) = make_uint4(v[0], v[1], v[2], v[3]);
         }
         fence_proxy_async_smem();

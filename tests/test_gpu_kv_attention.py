@@ -592,3 +592,20 @@ def test_thousands_of_requests(ctx, R, G, dtype):
     assert float(err.max()) <= 4 * TOL[dtype] and float((out.double() - want).norm() / want.norm()) <= TOL[dtype]
     tol = 2e-6 * wl.abs() + 2e-6 if dtype == torch.float32 else 5e-4
     assert ((lse.double() - wl).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("value", [float("inf"), -float("inf"), float("nan")])
+def test_prompt_rows_with_an_infinity_or_nan(ctx, value, dtype):
+    """Such a row is NaN, whatever the sign of the keys it sees: the first rows see one or two."""
+    c = Case([(512, 512), (300, 300)], 8, 4, 128, 64, dtype, seed=55)
+    want, wl = c.ref()
+    bad = torch.zeros(want.shape[:2], dtype=torch.bool)
+    for row, head, d in ((0, 0, 7), (0, 5, 100), (1, 3, 0), (2, 31, 127), (512, 9, 64), (513, 14, 1), (400, 2, 3)):
+        c.q[row, head, d] = value
+        bad[row, head] = True
+    out, lse = c.run(ctx)
+    assert torch.isnan(out[bad]).all() and torch.isnan(lse[bad]).all()
+    keep = ~bad
+    assert float((out[keep].double() - want[keep]).norm() / want[keep].norm()) <= TOL[dtype]
+    assert ((lse[keep].double() - wl[keep]).abs() <= 5e-4).all()
