@@ -484,8 +484,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(KvPromptAr
             p[c / 2] = half ? pack_f16(p0, p1) : pack_bf16(p0, p1);
             p[16 + c / 2] = half ? pack_f16(q0, q1) : pack_bf16(q0, q1);
           }
-          if ((flags & 0x10u) && part0 > 0.0f) part0 = __int_as_float(0x7fc00000);
-          if ((flags & 0x20u) && part1 > 0.0f) part1 = __int_as_float(0x7fc00000);
+          // a NaN block of V makes NaN of every row that sees a key of it
+          if (((flags & 0x10u) && below0 > 0) || ((flags & 0x20u) && below1 > 0)) unscale = __int_as_float(0x7fc00000);
           l += part0 + part1;
         }
         tmem_st32(tp, p);                        // over S, which has been read
@@ -645,7 +645,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(KvPromptAr
         if (j + 1 < n) load_k(pl_next);
         if (g >= 2) wait(&bar.vempty[st], (g >> 1) - 1);
         uint8_t* vd = sv + st * S::kKTile;
-        // the blocks' steps as pairs; a NaN block's values count as 0 (its rows' sums become NaN instead)
+        // the blocks' steps as pairs; a NaN block's values count as 0 (its rows become NaN at their end instead)
         uint32_t step[2];
 #pragma unroll
         for (int q = 0; q < 2; ++q) {

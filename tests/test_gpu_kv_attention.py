@@ -609,3 +609,25 @@ def test_prompt_rows_with_an_infinity_or_nan(ctx, value, dtype):
     keep = ~bad
     assert float((out[keep].double() - want[keep]).norm() / want[keep].norm()) <= TOL[dtype]
     assert ((lse[keep].double() - wl[keep]).abs() <= 5e-4).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_v_blocks_that_are_nan(ctx, dtype):
+    """Rows that see such a block are NaN, also those whose probabilities there are 0; their log-sum-exp knows nothing of V."""
+    c = Case([(512, 512), (200, 200)], 8, 4, 128, 64, dtype, seed=56)
+    pg = int(c.table[0, 3])                          # keys 192 .. 255
+    c.k[pg, 2, 0] = 0                                # head 2: keys 192 .. 223 have scores far below the others'
+    c.ks[:, 2] = 140
+    c.k[int(c.table[0, 0]), 2, 0, 0] = 100
+    c.q[:512, 8:12] = c.q[:512, 8:12].abs()
+    want, wl = c.ref()                               # of the values without the NaN: what the other rows are
+    c.vs[pg, 1, 1] = 255                             # head 1: keys 224 .. 255
+    c.vs[pg, 2, 0] = 255
+    assert float(torch.exp(wl[300:512, 8:12].neg()).max()) == 0.0
+    out, lse = c.run(ctx)
+    nan = torch.zeros(want.shape[:2], dtype=torch.bool)
+    nan[224:512, 4:8] = True
+    nan[192:512, 8:12] = True
+    assert torch.isnan(out[nan]).all() and torch.isfinite(out[~nan]).all()
+    assert float((out[~nan].double() - want[~nan]).norm() / want[~nan].norm()) <= TOL[dtype]
+    assert ((lse.double() - wl).abs() <= 5e-4 + 2e-6 * wl.abs()).all()
