@@ -12,7 +12,7 @@
 // runs in fp16 too: P keeps 11 bits, and V' = q_v 2^(e_v - e + 8), e the unit's
 // largest V exponent, is exact while the unit's exponents lie within 2^32 of
 // each other.  Where they do not, that unit's P and V are bf16, which takes any
-// exponent (and leaves P 8 bits).
+// exponent, and P is the sum of two terms of 8 bits, each with a product of its own.
 //
 // Warps: 0-3 and 4-7 softmax of tile A and of B, a row a thread; 8-11 bring K
 // and V from their pages, int8 -> 16 bits, into two-stage rings in the 128-byte
@@ -164,6 +164,10 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
+}
+// What rounding to bf16 took off a pair.
+__device__ __forceinline__ uint32_t rest_bf16(uint32_t rounded, float lo, float hi) {
+  return pack_bf16(lo - __uint_as_float(rounded << 16), hi - __uint_as_float(rounded & 0xFFFF0000u));
 }
 // 2^e in fp16 (0 below its smallest), e <= 8.
 __device__ __forceinline__ uint32_t f16_pow2(int e) {
@@ -471,18 +475,36 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(KvPromptAr
           l += p0 + p1;
         } else {
           float part0 = 0.0f, part1 = 0.0f;
+          auto four = [&](int c, float (&y)[4]) {  // columns c, c + 1 of both blocks
+            y[0] = ex2(fmaf(__uint_as_float(s0[c]), f0, -base)), y[1] = ex2(fmaf(__uint_as_float(s0[c + 1]), f0, -base));
+            y[2] = ex2(fmaf(__uint_as_float(s1[c]), f1, -base)), y[3] = ex2(fmaf(__uint_as_float(s1[c + 1]), f1, -base));
+            if (key_token(c) >= below0) y[0] = 0.0f;
+            if (key_token(c + 1) >= below0) y[1] = 0.0f;
+            if (key_token(c) >= below1) y[2] = 0.0f;
+            if (key_token(c + 1) >= below1) y[3] = 0.0f;
+            part0 += y[0] + y[1];
+            part1 += y[2] + y[3];
+          };
+          if (half) {
 #pragma unroll
-          for (int c = 0; c < 32; c += 2) {
-            float p0 = ex2(fmaf(__uint_as_float(s0[c]), f0, -base)), p1 = ex2(fmaf(__uint_as_float(s0[c + 1]), f0, -base));
-            float q0 = ex2(fmaf(__uint_as_float(s1[c]), f1, -base)), q1 = ex2(fmaf(__uint_as_float(s1[c + 1]), f1, -base));
-            if (key_token(c) >= below0) p0 = 0.0f;
-            if (key_token(c + 1) >= below0) p1 = 0.0f;
-            if (key_token(c) >= below1) q0 = 0.0f;
-            if (key_token(c + 1) >= below1) q1 = 0.0f;
-            part0 += p0 + p1;
-            part1 += q0 + q1;
-            p[c / 2] = half ? pack_f16(p0, p1) : pack_bf16(p0, p1);
-            p[16 + c / 2] = half ? pack_f16(q0, q1) : pack_bf16(q0, q1);
+            for (int c = 0; c < 32; c += 2) {
+              float y[4];
+              four(c, y);
+              p[c / 2] = pack_f16(y[0], y[1]);
+              p[16 + c / 2] = pack_f16(y[2], y[3]);
+            }
+          } else {
+            uint32_t rest[32];                   // what bf16 rounds off P
+#pragma unroll
+            for (int c = 0; c < 32; c += 2) {
+              float y[4];
+              four(c, y);
+              p[c / 2] = pack_bf16(y[0], y[1]);
+              p[16 + c / 2] = pack_bf16(y[2], y[3]);
+              rest[c / 2] = rest_bf16(p[c / 2], y[0], y[1]);
+              rest[16 + c / 2] = rest_bf16(p[16 + c / 2], y[2], y[3]);
+            }
+            tmem_st32(tp + 32, rest);            // beside P: the step's S had 64 columns, P has 32
           }
           // a NaN block of V makes NaN of every row that sees a key of it
           if (((flags & 0x10u) && below0 > 0) || ((flags & 0x20u) && below1 > 0)) unscale = __int_as_float(0x7fc00000);
@@ -702,6 +724,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(KvPromptAr
       const int my = uniform(x ? un.nb : un.na), n = uniform(un.n) * 2;   // steps of this tile; of the unit, in whole K/V tiles
       const uint32_t kt0 = uniform(kt), tm = uniform(tmem);
       constexpr uint32_t kIdS = idesc_16(false, 128, kStepKeys);
+      constexpr uint32_t kIdWide = idesc_16(true, 128, D);
       uint32_t id_o = idesc_16(false, 128, D);
       const uint64_t dq = sw128_kmajor_desc(smem_u32(sq + x * S::kQTile)), dk = sw128_kmajor_desc(smem_u32(sk)),
                      dv = sw128_kmajor_desc(smem_u32(sv));
@@ -717,7 +740,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(KvPromptAr
         if (j >= 0 && !place) {
           wait(&bar.vfull[g & 1], g >> 1);
           const int2 e = v_range();
-          id_o = idesc_16(e.x - e.y > 32, 128, D);
+          id_o = e.x - e.y > 32 ? kIdWide : idesc_16(false, 128, D);
         }
         if (j >= 0 && j < my) {
           wait(&bar.pfull[x][place], place ? np1 : np0);
@@ -729,6 +752,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(KvPromptAr
             const uint64_t db = dv + (((g & 1) * S::kKTile + place * (D * 128)) >> 4);
 #pragma unroll
             for (int k = 0; k < kStepKeys / 16; ++k) mma_ts(to, ts + k * 8, db + k * 2, id_o, j > 0 || k > 0);
+            if (id_o == kIdWide)         // P's second term
+#pragma unroll 1
+              for (int k = 0; k < kStepKeys / 16; ++k) mma_ts(to, ts + 32 + k * 8, db + k * 2, kIdWide, 1);
             mma_commit(&bar.pvdone[x][place]);
           }
           __syncwarp();

@@ -631,3 +631,28 @@ def test_v_blocks_that_are_nan(ctx, dtype):
     assert torch.isnan(out[nan]).all() and torch.isfinite(out[~nan]).all()
     assert float((out[~nan].double() - want[~nan]).norm() / want[~nan].norm()) <= TOL[dtype]
     assert ((lse.double() - wl).abs() <= 5e-4 + 2e-6 * wl.abs()).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [64, 128])
+def test_prompts_keep_their_bits_where_v_scales_are_far_apart(ctx, D, dtype):
+    """Exponents of V more than 2^32 apart: P in two terms of 8 bits (2^-17 of
+    an element), beside which the usual bound holds."""
+    c = Case([(600, 600), (300, 200), (1000, 77)], 8, 4, D, 64, dtype, seed=57)
+    c.vs[:, 1, 1] -= 70                              # head 1: every other block tiny
+    c.vs[int(c.table[1, 0]), 2, 0] = 1               # head 2 of request 1: one block tiny
+    c.vs[int(c.table[2, 9]), 3, :] -= 40             # head 3 of request 2: a page small
+    c.vs[int(c.table[2, 3]), 5, 1] = 255             # head 5 of request 2: a NaN block and a tiny one
+    c.vs[int(c.table[2, 4]), 5, 1] = 1
+    want, wl = c.ref()
+    out, lse = c.run(ctx)
+    assert ((lse.double() - wl).abs() <= 5e-4).all()
+    for a, b, r in ((0, 600, 0), (600, 800, 1), (800, 877, 2)):
+        for h in range(8):
+            g, w = out[a:b, 4 * h:4 * h + 4].double(), want[a:b, 4 * h:4 * h + 4]
+            if (r, h) == (2, 5):
+                assert torch.isnan(g).all()
+                continue
+            assert float((g - w).norm() / w.norm()) <= TOL[dtype], (h, a)
+            by_row = (g - w).flatten(0, 1).norm(dim=1) / w.flatten(0, 1).norm(dim=1)
+            assert float(by_row.max()) <= 4 * TOL[dtype], (h, a)
