@@ -739,18 +739,30 @@ def ppo_rollout_forward(states, actions, w_proj, w_policy, w_value=None, ctx=Non
 KV_BLOCK = _lib.KV_BLOCK
 
 
-class _NotBuilt:
+class _NoBinding:
+    """In the binding's place where it cannot be loaded: its calls say why, the
+    others do not need it."""
+
+    def __init__(self, why):
+        self.why = str(why)
+
     def __getattr__(self, name):
-        raise ImportError("_serve.so is not built (expected beside %s); run `python -m cpu_model_b200.build`" % _lib.LIB_PATH)
+        raise ImportError("the serving calls need _serve.so beside %s: %s; run `python -m cpu_model_b200.build`"
+                          % (_lib.LIB_PATH, self.why))
 
 
 try:
     from . import _serve
-except ImportError:
-    if os.path.exists(os.path.join(os.path.dirname(_lib.LIB_PATH), "_serve.so")):
-        raise
-    _serve = _NotBuilt()
-    KVCache = None
+except ImportError as e:
+    _serve = _NoBinding(e if os.path.exists(os.path.join(os.path.dirname(_lib.LIB_PATH), "_serve.so")) else "it is not built")
+
+    class KVCache:
+        def __init__(self, *args):
+            _serve.KVCache
+
+        @staticmethod
+        def empty(*args):
+            _serve.KVCache
 else:
     KVCache = _serve.KVCache
 

@@ -1,4 +1,10 @@
-"""The serving calls' host side, without a GPU: what autograd is told."""
+"""The serving calls' host side, without a GPU: what autograd is told, the
+binding's build and what goes on without it."""
+import os
+import shutil
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -37,3 +43,38 @@ def test_second_derivatives_are_refused(on_cpu):
     with pytest.raises(RuntimeError, match="second derivative"):
         (g.square().sum() + logp.sum()).backward()
     mx.token_logp(x, t)[0].sum().backward()          # the first still goes
+
+
+def a_package(tmp_path, serve):
+    """The package's files with another _serve.so."""
+    here = os.path.dirname(os.path.abspath(mx.__file__))
+    pkg = tmp_path / "cpu_model_b200"
+    pkg.mkdir()
+    for f in os.listdir(here):
+        if f.endswith(".py"):
+            shutil.copy(os.path.join(here, f), pkg / f)
+    os.symlink(os.path.join(here, "libmxq.so"), pkg / "libmxq.so")
+    if serve is not None:
+        (pkg / "_serve.so").write_bytes(serve)
+    return tmp_path
+
+
+@pytest.mark.parametrize("serve", [None, b"built against another torch"])
+def test_without_the_binding_the_rest_works(tmp_path, serve):
+    """A binding that is not there or does not load is missed by its own calls, with the reason, and by nobody else."""
+    code = """
+import torch
+from cpu_model_b200 import mx
+mx.MXContext, mx.mx_linear, mx.MXWeight
+calls = [lambda: mx.kv_plan(*[torch.zeros(1)] * 3, None, None, None, 1), lambda: mx.token_logprobs(torch.zeros(1, 1), None),
+         lambda: mx.KVCache(None, None, None, None), lambda: mx.KVCache.empty(1, 32, 1, 64)]
+for f in calls:
+    try:
+        f()
+    except ImportError as e:
+        assert "_serve.so" in str(e) and "cpu_model_b200.build" in str(e), e
+    else:
+        raise AssertionError("did not say that the binding is missing")
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=a_package(tmp_path, serve), capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
