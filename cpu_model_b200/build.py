@@ -28,20 +28,34 @@ FLAGS = [
 ]
 
 
+def newer(files, target):
+    return not os.path.exists(target) or any(os.path.getmtime(f) > os.path.getmtime(target) for f in files)
+
+
 def needs_build():
-    if not os.path.exists(LIB) or not os.path.exists(BINDING):
+    csrc = [os.path.join(HERE, "csrc", f) for f in os.listdir(os.path.join(HERE, "csrc")) if f != "mxq_py.cpp"]
+    return newer(csrc + [os.path.join(ROOT, "include", "mxq.h")], LIB)
+
+
+def binding_tag(torch):
+    """What a binding was built against: torch's C++ interface and Python's are their versions' own."""
+    return "torch %s python %s" % (torch.__version__, sys.version.split()[0])
+
+
+def binding_is_old(torch):
+    if newer([os.path.join(HERE, "csrc", "mxq_py.cpp"), os.path.join(ROOT, "include", "mxq.h")], BINDING):
         return True
-    t = min(os.path.getmtime(LIB), os.path.getmtime(BINDING))
-    deps = [os.path.join(HERE, "csrc", f) for f in os.listdir(os.path.join(HERE, "csrc"))]
-    deps.append(os.path.join(ROOT, "include", "mxq.h"))
-    return any(os.path.getmtime(d) > t for d in deps)
+    try:
+        with open(BINDING + ".tag") as f:
+            return f.read() != binding_tag(torch)
+    except OSError:
+        return True
 
 
-def build_binding(verbose=False):
+def build_binding(torch, verbose=False):
     """_serve.so: csrc/mxq_py.cpp against the installed torch and libmxq.so."""
     import sysconfig
 
-    import torch
     from torch.utils import cpp_extension as ext
     inc = ext.include_paths() + [sysconfig.get_paths()["include"], "/usr/local/cuda/include", os.path.join(ROOT, "include")]
     cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", "-DTORCH_EXTENSION_NAME=_serve",
@@ -53,12 +67,12 @@ def build_binding(verbose=False):
         print(" ".join(cmd))
     subprocess.check_call(cmd)
     os.replace(BINDING + ".tmp", BINDING)
+    with open(BINDING + ".tag", "w") as f:
+        f.write(binding_tag(torch))
     return BINDING
 
 
-def build(force=False, verbose=False, ptxas_v=False):
-    if not force and not needs_build():
-        return LIB
+def build_library(verbose=False, ptxas_v=False):
     objs = []
     for src in SOURCES:
         obj = os.path.join(HERE, "csrc", src.replace(".cu", ".o"))
@@ -74,7 +88,23 @@ def build(force=False, verbose=False, ptxas_v=False):
     os.replace(tmp, LIB)
     for o in objs:
         os.remove(o)
-    build_binding(verbose)
+
+
+def build(force=False, verbose=False, ptxas_v=False):
+    """The library, which needs nvcc, and the binding, which needs torch with
+    its headers: without them it is left out, and only its calls are missing."""
+    if force or needs_build():
+        build_library(verbose, ptxas_v)
+    try:
+        import torch
+        from torch.utils import cpp_extension
+        if not any(os.path.exists(os.path.join(i, "torch", "extension.h")) for i in cpp_extension.include_paths()):
+            raise ImportError("torch has no headers")
+    except (ImportError, OSError) as e:
+        print("_serve.so (the serving calls' binding) is not built: %s" % e, file=sys.stderr)
+        return LIB
+    if force or binding_is_old(torch):
+        build_binding(torch, verbose)
     return LIB
 
 

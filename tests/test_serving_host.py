@@ -78,3 +78,31 @@ for f in calls:
 """
     r = subprocess.run([sys.executable, "-c", code], cwd=a_package(tmp_path, serve), capture_output=True, text=True)
     assert r.returncode == 0, r.stderr
+
+
+def test_library_builds_without_torch(monkeypatch, capfd):
+    """nvcc is enough for the library; the binding is left out, with a word."""
+    from cpu_model_b200 import build
+    done = []
+    monkeypatch.setattr(build, "build_library", lambda *a, **k: done.append("library"))
+    monkeypatch.setattr(build.subprocess, "check_call", lambda cmd: done.append(cmd[0]))
+    monkeypatch.setitem(sys.modules, "torch", None)
+    assert build.build(force=True) == build.LIB
+    assert done == ["library"] and "_serve.so" in capfd.readouterr().err
+
+
+def test_binding_of_another_torch_is_built_again(monkeypatch, tmp_path):
+    from cpu_model_b200 import build
+    so = tmp_path / "_serve.so"
+    monkeypatch.setattr(build, "BINDING", str(so))
+    done = []
+    monkeypatch.setattr(build, "build_library", lambda *a, **k: done.append("library"))
+    monkeypatch.setattr(build, "needs_build", lambda: False)
+    monkeypatch.setattr(build.subprocess, "check_call", lambda cmd: (done.append("binding"), open(cmd[cmd.index("-o") + 1], "w").close()))
+    build.build()
+    assert done == ["binding"] and os.path.exists(so)
+    build.build()
+    assert done == ["binding"]
+    monkeypatch.setattr(torch, "__version__", "0.0.1")
+    build.build()
+    assert done == ["binding"] * 2
