@@ -106,3 +106,23 @@ def test_binding_of_another_torch_is_built_again(monkeypatch, tmp_path):
     monkeypatch.setattr(torch, "__version__", "0.0.1")
     build.build()
     assert done == ["binding"] * 2
+
+
+def test_calls_in_the_documents_have_the_library_s_arguments(tmp_path):
+    """The documented serving step, compiled with every device array a pointer: an address of one would not do."""
+    import glob
+    import re
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    calls = []
+    for doc in glob.glob(os.path.join(root, "*.md")):
+        for block in re.findall(r"```c\n(.*?)```", open(doc).read(), re.S):
+            calls += re.findall(r"mxq_(?:kv|token)_\w+\([^;]*\);", block)
+    assert len(calls) >= 5
+    ints = "past add len table free_pages free_count free_count_dev cu slot position request short_dev chosen top_ids".split()
+    src = '#include "mxq.h"\nvoid f(mxq_ctx ctx, mxq_kv_cache* cache, int l, size_t R, size_t page, size_t max_pages, size_t n_pages, size_t n_tokens,\n' \
+          '  size_t row_stride, size_t n_heads, size_t max_new, size_t rows, size_t vocab, size_t top_k, float scale, const uint8_t* done,\n' \
+          '  const float* q, const float* k, const float* v, const float* logits, float* out, float* lse, float* logp, float* entropy,\n' \
+          '  float* top_logp, %s) {\n%s\n}\n' % (", ".join("int32_t* " + n for n in ints), "\n".join(calls))
+    (tmp_path / "doc.cpp").write_text(src)
+    r = subprocess.run(["g++", "-fsyntax-only", "-I" + os.path.join(root, "include"), str(tmp_path / "doc.cpp")], capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
