@@ -357,7 +357,7 @@ __global__ void __launch_bounds__(kCopyWarps * 32)
         }
         __syncwarp();
       }
-      const float inv = byte == 255 ? 0.0f : __int_as_float((254 - byte) << 23);
+      const float inv = byte == 255 ? 0.0f : pow2_exact(127 - byte);
       for (int r = 0; r < len; ++r) {
         if (len > 1) x.load(rows + (long)r * stride);
         uint32_t w = 0;
@@ -390,7 +390,7 @@ __global__ void __launch_bounds__(kCopyWarps * 32)
     const int byte = max(scale_byte(top), was);
     const bool grew = o && byte > was && byte != 255;
     const float down = grew ? step_down(was, byte) : 1.0f;
-    const float inv = byte == 255 ? 0.0f : __int_as_float((254 - byte) << 23);
+    const float inv = byte == 255 ? 0.0f : pow2_exact(127 - byte);
     const uint32_t tokens = (len == 32 ? 0xffffffffu : (1u << len) - 1) << o;
     if (byte == 255) {
 #pragma unroll

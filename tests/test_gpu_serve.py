@@ -532,3 +532,21 @@ def test_versions_of_what_is_written(ctx):
         y = torch.zeros((2, 5), device="cuda")
         r = mx.token_logprobs(y, i32(0, 1), ctx=ctx)
         mx.token_logprobs_grad(y, i32(0, 1), r.lse, r.entropy, torch.ones(2, device="cuda"), out=y, ctx=ctx)
+
+
+@pytest.mark.parametrize("n", [1, 12])
+def test_append_to_a_block_with_the_largest_scale(ctx, n):
+    """A block whose scale is 2^127 already: new rows are rounded to that step, not lost."""
+    P, H, D = 32, 1, 64
+    cache = mx.KVCache.empty(1, P, H, D)
+    cache.k_scale.fill_(254)
+    cache.v_scale.fill_(254)
+    x = torch.zeros((n, H, D), device="cuda")
+    x[:, 0, 0], x[:, 0, 1], x[:, 0, 2], x[:, 0, 3] = 3e38, -2e38, 1e38, 8e37
+    mx.kv_append(cache, x, x, cuda(np.arange(1, n + 1), torch.int32), ctx=ctx)
+    want = torch.round(x.double() * 2.0 ** -127)
+    assert want[0, 0, :4].tolist() == [2, -1, 1, 0]
+    assert torch.equal(cache.k[0, 0, 0, 1:n + 1].double(), want[:, 0])
+    for i in range(n):
+        for d in range(4):
+            assert int(cache.v.flatten()[v_place(i + 1, d)]) == int(want[i, 0, d])
