@@ -795,11 +795,13 @@ class KVPlan:
 def _address(ctx, tensor):
     """The address of the call's context: the given one or the default one of
     the tensor's device."""
+    dev = tensor.get_device()
     if ctx is None:
-        dev = tensor.get_device()
         if dev < 0:
             raise ValueError("the tensors must lie on a CUDA device")
         ctx = _contexts.get(dev) or context(dev)
+    elif dev != ctx.device:
+        raise ValueError("the tensors lie on device %d, the context is one of device %d" % (dev, ctx.device))
     return ctx.h.value
 
 

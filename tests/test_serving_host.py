@@ -1,5 +1,6 @@
 """The serving calls' host side, without a GPU: what autograd is told, the
 binding's build and what goes on without it."""
+import ctypes
 import os
 import shutil
 import subprocess
@@ -126,3 +127,18 @@ def test_calls_in_the_documents_have_the_library_s_arguments(tmp_path):
     (tmp_path / "doc.cpp").write_text(src)
     r = subprocess.run(["g++", "-fsyntax-only", "-I" + os.path.join(root, "include"), str(tmp_path / "doc.cpp")], capture_output=True, text=True)
     assert r.returncode == 0, r.stderr
+
+
+def test_a_context_of_another_device_is_refused(monkeypatch):
+    """Its kernels would run there, on a stream of the tensors' device."""
+    class Context:
+        device = 1
+        h = ctypes.c_void_p(1)
+
+    class OnDevice0:
+        def get_device(self):
+            return 0
+    with pytest.raises(ValueError, match="device"):
+        mx._address(Context(), OnDevice0())
+    Context.device = 0
+    assert mx._address(Context(), OnDevice0()) == 1
