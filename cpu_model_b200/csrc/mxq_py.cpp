@@ -102,8 +102,21 @@ struct KVCache {
       refuse("k_scale and v_scale must be [n_pages][heads][blocks]");
     same_device(k, {&v, &k_scale, &v_scale});
     if (n > INT32_MAX || h > INT32_MAX || nb > INT32_MAX / kBlock || d > INT32_MAX) refuse("kv cache: too large");
-    c = mxq_kv_cache{k.data_ptr(), v.data_ptr(), ptr<uint8_t>(k_scale), ptr<uint8_t>(v_scale),
-                     (int)n, (int)(nb * kBlock), (int)h, (int)d};
+    c = mxq_kv_cache{nullptr, nullptr, nullptr, nullptr, (int)n, (int)(nb * kBlock), (int)h, (int)d};
+  }
+  // Where the tensors' memory is now: they are the caller's, who may have given them another.
+  mxq_kv_cache now() const {
+    const int64_t blocks = (int64_t)c.n_pages * c.n_kv_heads * (c.page_size / kBlock), values = blocks * kBlock * c.head_dim;
+    const std::pair<const Tensor*, int64_t> all[] = {{&k, values}, {&v, values}, {&k_scale, blocks}, {&v_scale, blocks}};
+    for (const auto& [t, n] : all)
+      if (t->numel() != n || !t->is_cuda() || !t->is_contiguous() || t->element_size() != 1)
+        refuse("kv cache: a tensor is not what the cache was made of");
+    mxq_kv_cache at = c;
+    at.k = k.data_ptr();
+    at.v = v.data_ptr();
+    at.k_scale = ptr<uint8_t>(k_scale);
+    at.v_scale = ptr<uint8_t>(v_scale);
+    return at;
   }
 };
 
@@ -172,8 +185,9 @@ void kv_append(uintptr_t ctx, const KVCache& cache, const Tensor& k, const Tenso
     refuse("kv_append: k and v must be [n][heads][head_dim] of the cache with one slot a row");
   const int64_t stride = row_stride(k, "k");
   if (row_stride(v, "v") != stride) refuse("kv_append: k and v must have the same row stride");
-  same_device(cache.k, {&k, &v, &slots});
-  check(mxq_kv_append(bind(ctx, k), &cache.c, dt, k.data_ptr(), v.data_ptr(), stride, ptr<int32_t>(slots), n), ctx);
+  same_device(cache.k, {&cache.v, &cache.k_scale, &cache.v_scale, &k, &v, &slots});
+  const mxq_kv_cache c = cache.now();
+  check(mxq_kv_append(bind(ctx, k), &c, dt, k.data_ptr(), v.data_ptr(), stride, ptr<int32_t>(slots), n), ctx);
   written({&cache.k, &cache.v, &cache.k_scale, &cache.v_scale});
 }
 
@@ -182,11 +196,12 @@ py::tuple kv_read(uintptr_t ctx, const KVCache& cache, const Tensor& slots, at::
   want(slots, at::kInt, "slots");
   if (type != at::kFloat && type != at::kBFloat16 && type != at::kHalf)
     refuse(std::string("kv_read: float32, bfloat16 or float16, got ") + type_name(type));
-  same_device(cache.k, {&slots});
+  same_device(cache.k, {&cache.v, &cache.k_scale, &cache.v_scale, &slots});
+  const mxq_kv_cache c = cache.now();
   const int64_t n = slots.numel();
   const Tensor k = at::empty({n, cache.c.n_kv_heads, cache.c.head_dim}, slots.options().dtype(type));
   const Tensor v = at::empty_like(k);
-  check(mxq_kv_read(bind(ctx, slots), &cache.c, ptr<int32_t>(slots), n, row_type(k, "k"), k.data_ptr(), v.data_ptr()), ctx);
+  check(mxq_kv_read(bind(ctx, slots), &c, ptr<int32_t>(slots), n, row_type(k, "k"), k.data_ptr(), v.data_ptr()), ctx);
   return py::make_tuple(k, v);
 }
 
@@ -203,12 +218,13 @@ py::tuple kv_attention(uintptr_t ctx, const Tensor& q, const KVCache& cache, con
     refuse("kv_attention: q must be [n][heads][head_dim] with heads a multiple of the cache's");
   if (cu.numel() != r + 1) refuse("kv_attention: cu must hold n_requests + 1 offsets");
   if (max_new && *max_new < 1) refuse("kv_attention: max_new must be positive");
-  same_device(cache.k, {&q, &table, &ctx_len, &cu});
+  same_device(cache.k, {&cache.v, &cache.k_scale, &cache.v_scale, &q, &table, &ctx_len, &cu});
+  const mxq_kv_cache c = cache.now();
   const int64_t n = q.size(0), hq = q.size(1);
   const Tensor out = at::empty({n, hq, d}, q.options());
   optional<Tensor> lse;
   if (want_lse) lse = at::empty({n, hq}, q.options().dtype(at::kFloat));
-  check(mxq_kv_attention(bind(ctx, q), &cache.c, dt, q.data_ptr(), row_stride(q, "q"), n, hq, ptr<int32_t>(table),
+  check(mxq_kv_attention(bind(ctx, q), &c, dt, q.data_ptr(), row_stride(q, "q"), n, hq, ptr<int32_t>(table),
                          table.size(1), ptr<int32_t>(ctx_len), ptr<int32_t>(cu), r,
                          max_new ? *max_new : std::max<int64_t>(n, 1),
                          (float)(scale ? *scale : 1.0 / std::sqrt((double)d)), out.data_ptr(), ptr<float>(lse)),

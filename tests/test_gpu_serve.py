@@ -550,3 +550,25 @@ def test_append_to_a_block_with_the_largest_scale(ctx, n):
     for i in range(n):
         for d in range(4):
             assert int(cache.v.flatten()[v_place(i + 1, d)]) == int(want[i, 0, d])
+
+
+def test_a_cache_follows_its_tensors(ctx):
+    """The cache's tensors are the caller's: other memory given to one is what the next call uses, another shape is refused."""
+    P, H, D = 32, 2, 64
+    cache = mx.KVCache.empty(2, P, H, D)
+    x = torch.randn((3, H, D), device="cuda")
+    slots = cuda([0, 1, 2], torch.int32)
+    mx.kv_append(cache, x, x, slots, ctx=ctx)
+    want = mx.kv_read(cache, slots, ctx=ctx)
+    old = cache.k.clone(), cache.k_scale.clone()
+    cache.k.set_(torch.zeros_like(cache.k))
+    cache.k_scale.set_(torch.zeros_like(cache.k_scale))
+    assert (mx.kv_read(cache, slots, ctx=ctx)[0] == 0).all()
+    mx.kv_append(cache, x, x, slots, ctx=ctx)
+    assert all(torch.equal(a, b) for a, b in zip(mx.kv_read(cache, slots, ctx=ctx), want))
+    assert torch.equal(cache.k, old[0]) and torch.equal(cache.k_scale, old[1])
+    cache.v_scale.set_(torch.zeros(1, dtype=torch.uint8, device="cuda"))
+    for f in (lambda: mx.kv_append(cache, x, x, slots), lambda: mx.kv_read(cache, slots),
+              lambda: mx.kv_attention(x, cache, slots[None, :1].contiguous(), slots[:1], slots[:2])):
+        with pytest.raises(ValueError):
+            f()
