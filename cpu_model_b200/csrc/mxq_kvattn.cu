@@ -53,7 +53,6 @@ constexpr int kStart = 4;
 constexpr int kMinPiece = 1;             // places a piece at least
 constexpr int kWholeBlocks = 3;          // blocks a warp of a unit that a CTA keeps to itself, at most
 constexpr size_t kPromptUnits = 32;      // units of the prompts' kernel that are worth it
-constexpr float kLn2 = 0.693147180559945f;
 
 struct AttnArgs {
   KvView c;
@@ -69,13 +68,6 @@ struct AttnArgs {
   float* warp_part;                      // [CTAs * warps][rows][D + 2]
   float* cta_part;                       // [CTAs][2][rows][D + 2]
 };
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ float neg_inf() { return -__int_as_float(0x7f800000); }
 
 __device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                        uint32_t b1) {
@@ -1071,7 +1063,7 @@ int mxq_kv_attention(mxq_ctx c, const mxq_kv_cache* cache, int dtype, const void
   a.Hq = (int)n_heads;
   a.G = (int)(n_heads / kv.heads);
   a.max_pages = (int)max_pages;
-  a.scale2 = scale * 1.44269504088896341f;
+  a.scale2 = scale * kLog2e;
   a.counters = ws.counters + 1;
   // a part for each warp (12 of up to 8 rows, or 8 of 16) and two for each CTA
   const size_t row = (size_t)(kv.dim + 2) * 4, warp_parts = 8 * kMaxRows * row;

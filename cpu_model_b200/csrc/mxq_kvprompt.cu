@@ -45,14 +45,6 @@ constexpr int kStepKeys = 64;                     // keys of an S
 constexpr uint32_t kColS = 0, kColO = 256;        // TMEM columns: S of A, S of B, O of A, O of B
 constexpr float kRise = 8.0f;                     // log2 of what P may grow by before O is rescaled
 constexpr float kLift = 7.0f;                     // P starts at 2^7: fp16 has it normal down to 2^-21 of the maximum
-constexpr float kLn2 = 0.693147180559945f;
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ float neg_inf() { return -__int_as_float(0x7f800000); }
 
 #define MXQ_R4(a, i) "=r"(a[i]), "=r"(a[i + 1]), "=r"(a[i + 2]), "=r"(a[i + 3])
 #define MXQ_W4(a, i) "r"(a[i]), "r"(a[i + 1]), "r"(a[i + 2]), "r"(a[i + 3])

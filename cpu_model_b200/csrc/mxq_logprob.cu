@@ -17,15 +17,8 @@ namespace mxq {
 
 namespace {
 
-constexpr float kLog2e = 1.44269504088896341f;
 constexpr int kMaxSlices = 8;      // CTAs a row (a portable cluster)
 constexpr int kCandidates = 1024;
-
-__device__ __forceinline__ float exp2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 // Order of the top alternatives as one integer: descending logit (NaN above
 // all, -0 equal to 0), then ascending id.  0 is below every real entry.
@@ -53,7 +46,7 @@ __device__ __forceinline__ float drop(float d) { return fmaxf(d, -1000.0f); }
 __device__ __forceinline__ Stat merge(const Stat& a, const Stat& b) {
   const float m = fmaxf(a.m, b.m), f = floor_max(m);
   const float da = drop(floor_max(a.m) - f), db = drop(floor_max(b.m) - f);
-  const float ca = exp2_approx(da * kLog2e), cb = exp2_approx(db * kLog2e);
+  const float ca = ex2(da * kLog2e), cb = ex2(db * kLog2e);
   return {m, a.s * ca + b.s * cb, ca * (a.u + a.s * da) + cb * (b.u + b.s * db)};
 }
 __device__ __forceinline__ Stat shfl_xor(const Stat& a, int o) {
@@ -76,7 +69,7 @@ __device__ __forceinline__ void add_values(Stat& t, Largest& g, int at, const fl
   g.other = fmaxf(g.other, fminf(top, t.m));
   if (top > t.m) {
     g.at = at;
-    const float f = floor_max(top), d = drop(floor_max(t.m) - f), c = exp2_approx(d * kLog2e);
+    const float f = floor_max(top), d = drop(floor_max(t.m) - f), c = ex2(d * kLog2e);
     t.u = c * (t.u + t.s * d);
     t.s *= c;
     t.m = top;
@@ -85,7 +78,7 @@ __device__ __forceinline__ void add_values(Stat& t, Largest& g, int at, const fl
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const float d = x[i] - f;
-    const float e = exp2_approx(d * kLog2e);
+    const float e = ex2(d * kLog2e);
     t.s += e;
     t.u = fmaf(e, drop(d), t.u);
   }
@@ -221,7 +214,7 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(LogprobArgs a) 
   const long row = blockIdx.x / slices;
   const RowView<T> rv(static_cast<const T*>(a.logits) + row * a.stride, a.vocab);
 
-  Stat t{-__int_as_float(0x7f800000), 0.0f, 0.0f};
+  Stat t{neg_inf(), 0.0f, 0.0f};
   Largest g{-1, t.m};
   bool any = false;
   if (rank == 0) {
@@ -278,7 +271,7 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(LogprobArgs a) 
   if (tid < MXQ_TOPK_MAX) sh.best[tid] = 0;
   __syncthreads();
   if (warp == 0) {
-    Stat w = lane < THREADS / 32 ? sh.warp[lane] : Stat{-__int_as_float(0x7f800000), 0.0f, 0.0f};
+    Stat w = lane < THREADS / 32 ? sh.warp[lane] : Stat{neg_inf(), 0.0f, 0.0f};
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) w = merge(w, shfl_xor(w, o));
     if (lane == 0) sh.all = w;
@@ -387,21 +380,20 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(LogprobArgs a) 
         __syncthreads();
       }
     }
-    const float neg_inf = -__int_as_float(0x7f800000);
     const float logs = logf(all.s);               // -inf where nothing is left
     const bool empty = all.s == 0.0f;
     if (tid == 0) {
       const int tgt = a.target[row];
       float lp = 0.0f;
-      if (tgt >= 0 && tgt < a.vocab) lp = empty ? neg_inf : (to_f32(rv.x[tgt]) - all.m) - logs;
+      if (tgt >= 0 && tgt < a.vocab) lp = empty ? neg_inf() : (to_f32(rv.x[tgt]) - all.m) - logs;
       if (a.logp) a.logp[row] = lp;
-      if (a.lse) a.lse[row] = empty ? neg_inf : all.m + logs;
+      if (a.lse) a.lse[row] = empty ? neg_inf() : all.m + logs;
       if (a.entropy) a.entropy[row] = empty ? 0.0f : logs - all.u / all.s;
     }
     if (tid < a.k) {
       const uint64_t e = sh.best[tid];
       const float x = key_value((uint32_t)(e >> 32));
-      a.top_logp[row * a.k + tid] = empty ? neg_inf : (x - all.m) - logs;
+      a.top_logp[row * a.k + tid] = empty ? neg_inf() : (x - all.m) - logs;
       a.top_ids[row * a.k + tid] = (int32_t)(0xFFFFFFFFu - (uint32_t)e);
     }
   }
@@ -495,7 +487,7 @@ __global__ void __launch_bounds__(kGradThreads) token_logprobs_grad_kernel(Logpr
   auto one = [&](float y) {
     const float lp = empty ? -1000.0f : y - lse;
     // p (c - de log p), with a finite log p where p is 0
-    return exp2_approx(lp * kLog2e) * fmaf(-de, drop(lp), c);
+    return ex2(lp * kLog2e) * fmaf(-de, drop(lp), c);
   };
   if (part == 0) {
     for (int i = tid; i < head; i += kGradThreads) {

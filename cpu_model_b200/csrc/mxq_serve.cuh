@@ -34,6 +34,14 @@ struct KvPromptArgs {
 constexpr int kPromptMaxRequests = 4096;
 cudaError_t launch_kv_prompt(const KvPromptArgs& a, int ctas, cudaStream_t st);
 
+constexpr float kLn2 = 0.693147180559945f, kLog2e = 1.44269504088896341f;
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float neg_inf() { return -__int_as_float(0x7f800000); }
+
 // Index of (page, head, block of the page): its scale's place; its values
 // start at 32 * dim times it.
 __device__ __forceinline__ long kv_block(const KvView& c, int page, int head, int b) {
