@@ -1080,7 +1080,7 @@ int mxq_kv_attention(mxq_ctx c, const mxq_kv_cache* cache, int dtype, const void
   // one, but its units are not cut along the keys.
   const bool f32 = dtype == MXQ_DT_F32;
   const size_t units = (n * (size_t)a.G + 255) / 256 * kv.heads;
-  if (!f32 && rows > kMaxRows && n_req <= (size_t)kPromptMaxRequests && units >= kPromptUnits) {
+  if (!f32 && rows > kMaxRows && units >= kPromptUnits) {
     a.few = kMaxRows;
     KvPromptArgs p{kv, q, out, lse, table, ctx_len, cu, (long)q_stride, (int)n_req, (int)n, a.Hq, a.G, a.max_pages,
                    kMaxRows, dtype == MXQ_DT_BF16, a.scale2, ws.counters + kServeCounters - 2, ctx_status_word(c)};

@@ -794,7 +794,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(KvPromptAr
 template <int D, bool kBf16>
 cudaError_t launch(const KvPromptArgs& a, int ctas, cudaStream_t st) {
   static SmemAttr attr;
-  const size_t smem = 1024 + PromptShared<D>::kBytes + ((size_t)a.R + 1) * 4;
+  constexpr size_t kTiles = 1024 + PromptShared<D>::kBytes;
+  static_assert(kTiles + (MXQ_KV_MAX_REQUESTS + 1) * 4 + 1536 <= 227 << 10, "every number of requests fits");
+  const size_t smem = kTiles + ((size_t)a.R + 1) * 4;
   const cudaError_t e = attr.ensure(kv_prompt_kernel<D, kBf16>, smem);
   if (e != cudaSuccess) return e;
   kv_prompt_kernel<D, kBf16><<<(unsigned)ctas, kPromptThreads, smem, st>>>(a);

@@ -31,7 +31,6 @@ struct KvPromptArgs {
   uint32_t* next;                        // two words, zero
   uint32_t* status;
 };
-constexpr int kPromptMaxRequests = 4096;
 cudaError_t launch_kv_prompt(const KvPromptArgs& a, int ctas, cudaStream_t st);
 
 constexpr float kLn2 = 0.693147180559945f, kLog2e = 1.44269504088896341f;

@@ -656,3 +656,22 @@ def test_prompts_keep_their_bits_where_v_scales_are_far_apart(ctx, D, dtype):
             assert float((g - w).norm() / w.norm()) <= TOL[dtype], (h, a)
             by_row = (g - w).flatten(0, 1).norm(dim=1) / w.flatten(0, 1).norm(dim=1)
             assert float(by_row.max()) <= 4 * TOL[dtype], (h, a)
+
+
+def test_prompts_among_thousands_of_requests(ctx):
+    g = synth.rng(58)
+    spans = [(int(c), 1) for c in g.integers(1, 40, 8192)]
+    for r, s in ((0, (300, 290)), (4096, (700, 257)), (8191, (500, 40))):
+        spans[r] = s
+    c = Case(spans, 8, 2, 64, 32, torch.float16, seed=58)
+    out, lse = c.run(ctx)
+    few = [0, 1, 2, 4095, 4096, 4097, 8190, 8191]
+    rows = [i for r in few for i in range(int(c.cu[r]), int(c.cu[r + 1]))]
+    d = Case.__new__(Case)
+    d.__dict__.update(c.__dict__)
+    d.ctx, d.new = [c.ctx[r] for r in few], [c.new[r] for r in few]
+    d.table, d.q = c.table[few], c.q[rows]
+    d.cu = torch.tensor([0] + list(np.cumsum(d.new)), dtype=torch.int32)
+    want, wl = d.ref()
+    assert float((out[rows].double() - want).norm() / want.norm()) <= TOL[torch.float16]
+    assert ((lse[rows].double() - wl).abs() <= 5e-4).all() and torch.isfinite(out).all()
