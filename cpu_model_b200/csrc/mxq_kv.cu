@@ -62,7 +62,7 @@ __device__ __forceinline__ int2 block_scan(int2 v, int2* warp_sums, int2* total)
 // threads with a few requests each, and then writes its share of the rows and
 // of the new table entries.  What may be updated in place (the lengths, the
 // stack's height) is written by the last CTA to finish, when the others have
-// read it.  Bound by latency: 3.1 us for 32 requests of one token each, 9.8 us for
+// read it.  Bound by latency: 3.6 us for 32 requests of one token each, 10.4 us for
 // 4096 requests with 88.7k rows, of which the sums are most.
 __global__ void __launch_bounds__(1024) kv_plan_kernel(PlanArgs a) {
   extern __shared__ int sh[];
@@ -155,6 +155,7 @@ __global__ void __launch_bounds__(1024) kv_plan_kernel(PlanArgs a) {
 
 // One CTA, bound by latency: ending requests are few and their pages a few
 // thousand; the order on the stack is fixed by a scan, not by which thread came first.
+// 64 of 4096 requests with 20 pages each: 9 us.
 __global__ void __launch_bounds__(1024) kv_release_kernel(const uint8_t* done, int32_t* len, int R, int P,
                                                           int32_t* table, int max_pages, int32_t* free_pages,
                                                           int n_pages, int32_t* free_count) {
@@ -315,9 +316,10 @@ struct Runs {
 // bytes a lane, and V needs no exchange between lanes, since the 16-byte pieces of
 // its layout (two dimensions, eight tokens) each lie with one lane.  A decode step's runs
 // are one row each: V's bytes go out one by one, less than a block's way in and out.
-// Bound by HBM, two or four bytes in for one out: 17.4k bf16 rows of 8
-// heads of 128 in 20.1 us, 4.5 TB/s, 68 % of a copy (the grid's last wave is the
-// rest); 32 fp32 rows of 32 heads in 5.0 us, a launch and two dependent reads.
+// Bound by HBM, two or four bytes in for one out: 14.6k bf16 rows of 8
+// heads of 128 in 20.1 us, 4.5 TB/s, 68 % of a copy, fp32 rows in 32.2 us, 71 % (of
+// the rest most is the last wave of these 1824 CTAs, 3.1 of four an SM); 32
+// fp32 rows of 32 heads in 5.2 us, a launch and two dependent reads.
 template <typename T, int D>
 __global__ void __launch_bounds__(kCopyWarps * 32)
     kv_append_kernel(KvView c, const T* __restrict__ k, const T* __restrict__ v, long stride,
@@ -463,8 +465,8 @@ __device__ __forceinline__ void put2(__half* p, float a, float b) {
 // A warp: `chunk` consecutive entries, of one head, of K or V.  K rows are read
 // four at a time.  V is read a run at a time, whole blocks in 16-byte pieces: a
 // lane has two dimensions of eight tokens, and four lanes' stores reach
-// four rows in whole sectors.  Bound by HBM: 17.4k rows of 8 heads to bf16 in
-// 20.2 us, 4.5 TB/s; 32 x 32 heads to fp32 in 5.6 us.
+// four rows in whole sectors.  Bound by HBM: 14.7k rows of 8 heads to bf16 in
+// 20.2 us, 4.5 TB/s; 444 rows of 32 heads to bf16 in 5.8 us.
 template <typename T, int D>
 __global__ void __launch_bounds__(kCopyWarps * 32)
     kv_read_kernel(KvView c, const int32_t* __restrict__ slot, int n, int chunk, T* __restrict__ k_out,
@@ -598,7 +600,8 @@ int mxq_kv_plan(mxq_ctx c, const int32_t* past, const int32_t* add, size_t n_req
   if (int rc = ctx_serve_ws(c, &ws)) return rc;
   PlanArgs a{past, add, free_pages, free_count, table, ctx_len, cu, slot, position, request, free_out, short_out,
              (int)n_req, (int)page_size, (int)max_pages, (int)n_pages, (int)n_tokens, ws.counters};
-  // a thread a new row up to 4 CTAs an SM; small steps in one CTA of 256
+  // a thread a new row (or request) up to one CTA an SM, in CTAs of 256 while
+  // 16 of them will do; up to 256 rows are one CTA's
   const size_t most = n_tokens > n_req ? n_tokens : n_req;
   const int threads = most <= 4096 ? 256 : 1024;
   size_t ctas = (most + threads - 1) / threads;

@@ -36,9 +36,11 @@
 // tokens, 32 heads of 128, fp32 rows: 117 us, 4.85 TB/s of cache (74 % of a copy).
 // 192 requests of 16 to 8191 tokens, 32 heads over 8, bf16: 123 us, 4.6 TB/s; the
 // starts of so many units are the rest.  Two requests of 100k to 131k tokens, 16
-// heads over 2 of 64, fp16: 21 us, 2.7 TB/s; the chain length -> page -> scale and K
+// heads over 2 of 64, fp16: 22 us, 2.6 TB/s; the chain length -> page -> scale and K
 // before a piece's first block, and the join, take two thirds of it.  One request of
-// 517 tokens, 32 heads, fp32: 9.1 us, that chain and nothing else.
+// 517 tokens, 32 heads, fp32: 9.3 us, that chain and nothing else.  At D = 128 the
+// tiles of one and of eight rows spill 42 to 226 bytes a thread at the 168
+// registers that 12 warps leave them; what that costs has not been measured.
 #include "mxq_serve.cuh"
 
 namespace mxq {
@@ -1075,9 +1077,14 @@ int mxq_kv_attention(mxq_ctx c, const mxq_kv_cache* cache, int dtype, const void
   a.cta_part = reinterpret_cast<float*>(ws.scratch + (size_t)ctas * warp_parts);
   const size_t rows = max_new * (size_t)a.G;
   a.few = 1 << 30;
-  // Prompts' 16-bit rows go to the tensor cores' kernel where they fill at
-  // least kPromptUnits of its units: one SM with it is as fast as 6 with this
-  // one, but its units are not cut along the keys.
+  // Prompts' 16-bit rows go to the tensor cores' kernel where the call's rows would
+  // fill at least kPromptUnits of its units: one SM with it is as fast as 6 with this
+  // one, but its units are not cut along the keys.  The rows of the whole call
+  // are counted, since the host does not know whose they are, so a prompt among many
+  // single tokens goes there with few units too.  250 decoding requests of 16 to
+  // 8191 tokens, 32 heads over 8, bf16: 146 us; with a prompt of 40 rows behind 4000
+  // tokens beside them, 8 units, 274 us (fp32 rows, all on this kernel: 207); of 300
+  // rows, 40 units, 286 us (321).
   const bool f32 = dtype == MXQ_DT_F32;
   const size_t units = (n * (size_t)a.G + 255) / 256 * kv.heads;
   if (!f32 && rows > kMaxRows && units >= kPromptUnits) {

@@ -30,9 +30,10 @@
 // run to the end without waiting.
 //
 // 4 prompts of 1142 to 1570 rows after 599 to 2839 tokens, 32 heads over 8 of 128,
-// bf16: 280 us, 707 TFLOP/s, 43 % of cuBLAS's bf16 rate.  Latency bounds it: a
-// softmax step's chain (S, maximum, exp, P, hand-over; without the exp 260 us), and
-// 15 us of each unit's start and end, about 4.6 units a CTA.
+// bf16: 285 us, 695 TFLOP/s, 42 % of cuBLAS's bf16 rate.  Latency bounds it: a
+// softmax step's chain (S, maximum, exp, P, hand-over; without the exp 20 us less), and
+// 15 us of each unit's start and end, about 4.6 units a CTA.  Units are not cut along
+// the keys: 512 rows behind 32k tokens, 64 units, take 664 us, 4 times their operations'.
 #include "mxq_serve.cuh"
 
 namespace mxq {

@@ -7,10 +7,12 @@
 //   lse = M + log s,  logp = (x_t - M) - log s,  entropy = log s - u / s.
 // Forward: one pass over the row; every thread keeps (M, s, u) of what it has
 // read and rescales when its M rises, so the row is read from memory once.
-// Both directions are bound by HBM: a pass has nothing to reuse.  8192 rows of
-// 32000 fp32 logits with 5 alternatives: 167 us launch after launch, 173 with cold
-// caches, 6.1 TB/s, 93 % of a copy; the gradient of 4096 x 32000 bf16: 82.5 us, 6.35
-// TB/s.  One row of 32000 is bound by latency: 5.9 us.
+// A pass has nothing to reuse, and HBM bounds fp32 rows and the gradient: 8192
+// rows of 32000 fp32 logits with 5 alternatives take 167 to 170 us launch after
+// launch, 175 with cold caches, 6.1 TB/s, 92 % of a copy; the gradient of 4096 x
+// 32000 bf16 82 us, 6.4 TB/s, of fp32 157 us.  16-bit rows do the same work
+// for each logit in half the bytes and are bound by its instructions: 8192 x 32000
+// bf16 158 us, twice their bytes' time.  One row of 32000 is bound by latency: 5.9 us.
 #include "mxq_serve.cuh"
 
 namespace mxq {

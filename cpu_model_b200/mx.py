@@ -836,7 +836,8 @@ def kv_attention(q, cache, table, ctx_len, cu, scale=None, max_new=None, want_ls
     """Causal attention of the new rows over the cache (mxq_kv_attention): q
     [N][Hq][D] (float32, bfloat16 or float16; rows may have a stride); request
     r's rows are cu[r] .. cu[r + 1] - 1, the last of its ctx_len[r] tokens.
-    scale defaults to 1 / sqrt(D); max_new bounds the new rows of a request.
+    scale defaults to 1 / sqrt(D); max_new bounds the new rows of a request (N
+    when left out, which is slow for one-token steps).
     Returns (out [N][Hq][D] of q's type, lse fp32 [N][Hq] or None)."""
     return _serve.kv_attention(_address(ctx, q), q, cache, table, ctx_len, cu, scale, max_new, want_lse)
 

@@ -675,8 +675,11 @@ MXQ_API int mxq_kv_read(mxq_ctx ctx, const mxq_kv_cache* cache,
  * softmax(scale * q k^T) v; lse [n][n_heads] fp32 (may be null) the natural
  * logarithm of the softmax's denominator.  A row that sees no key, or that
  * belongs to no request (rows from cu[n_req] on), gets 0 and -inf.  Pages
- * outside the pool hold no keys.  max_new >= every request's number of new rows (more is safe; it only
- * chooses the kernel).  Its workspace: see mxq_kv_plan. */
+ * outside the pool, and places beyond the table, hold no keys.  A row of q with
+ * an infinity or NaN is NaN; a NaN block of K makes rows that see a key of it
+ * NaN, one of V their out alone.  max_new >= every request's number of new
+ * rows; it only chooses the kernel, so more is safe, and slower: one-token
+ * steps want 1.  Its workspace: see mxq_kv_plan. */
 MXQ_API int mxq_kv_attention(mxq_ctx ctx, const mxq_kv_cache* cache, int dtype,
                              const void* q, size_t q_stride, size_t n,
                              size_t n_heads, const int32_t* table,
