@@ -2414,7 +2414,10 @@ int ctx_serve_ws(mxq_context* c, ServeWs* out) {
         e = cudaDeviceGetAttribute(&c->sms, cudaDevAttrMultiProcessorCount, c->device);
         if (e != cudaSuccess) return broken(e);
       }
-      if (!spare && gone && cudaDeviceSynchronize() == cudaSuccess) spare = gone;   // its last calls have ended
+      if (!spare && gone) {
+        if (cudaDeviceSynchronize() == cudaSuccess) spare = gone;   // its last calls have ended
+        else cudaGetLastError();                                    // not while a stream is capturing: another one then
+      }
       if (!spare) {
         c->serve_ws.reserve(c->serve_ws.size() + 1);
         uint8_t* base = nullptr;

@@ -241,7 +241,7 @@ const WeightView* weight_view(mxq_weight w);
 // next.  There is one for each stream that a context has used them on, and one
 // for each stream of a capture, which its graph keeps: calls on two streams
 // and replays of two graphs do not meet in it, on whatever streams they run.
-// (One graph's replays that run at once would meet, as they would in its outputs.)
+// (What is instantiated of one graph would, run at once, as it would in the outputs.)
 constexpr size_t kServeCounters = 2048;                  // uint32
 constexpr size_t kServeScratch = 13u << 20;              // bytes
 struct ServeWs {

@@ -631,7 +631,8 @@ typedef struct mxq_kv_cache {
  * the graph that is made (and is used again when the graph and all that was
  * instantiated of it are gone).  So calls on different streams, and replays of
  * different graphs on any streams, run beside one another.  The first call
- * on a stream or in a capture may allocate it; graphs must go before the
+ * on a stream or in a capture may allocate it; the first on a stream that came
+ * after one was destroyed may wait for the device.  Graphs must go before the
  * context does. */
 MXQ_API int mxq_kv_plan(mxq_ctx ctx, const int32_t* past, const int32_t* add,
                         size_t n_req, size_t page_size, int32_t* table,
