@@ -88,6 +88,7 @@ SIGNATURES = {
     "mxq_kv_plan": [_vp, _vp, _vp, _sz, _sz, _vp, _sz, _vp, _sz, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _vp],
     "mxq_kv_release": [_vp, _vp, _vp, _sz, _sz, _vp, _sz, _vp, _sz, _vp],
     "mxq_kv_append": [_vp, _vp, _i, _vp, _vp, _sz, _vp, _sz],
+    "mxq_kv_append_strided": [_vp, _vp, _i, _vp, _sz, _vp, _sz, _vp, _sz],
     "mxq_kv_read": [_vp, _vp, _vp, _sz, _i, _vp, _vp],
     "mxq_kv_attention": [_vp, _vp, _i, _vp, _sz, _sz, _sz, _vp, _sz, _vp, _vp, _sz, _sz, _f, _vp, _vp],
     "mxq_token_logprobs": [_vp, _i, _vp, _sz, _sz, _sz, _vp, _sz, _vp, _vp, _vp, _vp, _vp],

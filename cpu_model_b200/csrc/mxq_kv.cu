@@ -322,7 +322,7 @@ struct Runs {
 // fp32 rows of 32 heads in 5.2 us, a launch and two dependent reads.
 template <typename T, int D>
 __global__ void __launch_bounds__(kCopyWarps * 32)
-    kv_append_kernel(KvView c, const T* __restrict__ k, const T* __restrict__ v, long stride,
+    kv_append_kernel(KvView c, const T* __restrict__ k, long k_stride, const T* __restrict__ v, long v_stride,
                      const int32_t* __restrict__ slot, int n, int chunk) {
   constexpr int V = D / 32;        // dimensions a lane
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -330,6 +330,7 @@ __global__ void __launch_bounds__(kCopyWarps * 32)
   if (base >= n) return;
   const bool is_v = blockIdx.z != 0;
   const T* src = (is_v ? v : k) + (long)head * D + lane * V;
+  const long stride = is_v ? v_stride : k_stride;
   int8_t* data = is_v ? c.v : c.k;
   uint8_t* scales = is_v ? c.vs : c.ks;
   const Runs runs(slot, n, c.n_pages * c.page, base, chunk);
@@ -546,16 +547,16 @@ int rows_a_warp(const KvView& c, int n) {
 }
 
 template <typename T>
-cudaError_t launch_append(const KvView& c, const void* k, const void* v, long stride, const int32_t* slot, int n,
-                          cudaStream_t st) {
+cudaError_t launch_append(const KvView& c, const void* k, long k_stride, const void* v, long v_stride,
+                          const int32_t* slot, int n, cudaStream_t st) {
   const int chunk = rows_a_warp(c, n), per = chunk * kCopyWarps;
   const dim3 grid((unsigned)((n + per - 1) / per), (unsigned)c.heads, 2);
   if (c.dim == 64)
-    kv_append_kernel<T, 64><<<grid, kCopyWarps * 32, 0, st>>>(c, static_cast<const T*>(k), static_cast<const T*>(v),
-                                                              stride, slot, n, chunk);
+    kv_append_kernel<T, 64><<<grid, kCopyWarps * 32, 0, st>>>(c, static_cast<const T*>(k), k_stride,
+                                                              static_cast<const T*>(v), v_stride, slot, n, chunk);
   else
-    kv_append_kernel<T, 128><<<grid, kCopyWarps * 32, 0, st>>>(c, static_cast<const T*>(k), static_cast<const T*>(v),
-                                                               stride, slot, n, chunk);
+    kv_append_kernel<T, 128><<<grid, kCopyWarps * 32, 0, st>>>(c, static_cast<const T*>(k), k_stride,
+                                                               static_cast<const T*>(v), v_stride, slot, n, chunk);
   return cudaGetLastError();
 }
 
@@ -637,6 +638,11 @@ int mxq_kv_release(mxq_ctx c, const uint8_t* done, int32_t* len, size_t n_req, s
 
 int mxq_kv_append(mxq_ctx c, const mxq_kv_cache* cache, int dtype, const void* k, const void* v, size_t row_stride,
                   const int32_t* slot, size_t n) {
+  return mxq_kv_append_strided(c, cache, dtype, k, row_stride, v, row_stride, slot, n);
+}
+
+int mxq_kv_append_strided(mxq_ctx c, const mxq_kv_cache* cache, int dtype, const void* k, size_t k_stride, const void* v,
+                          size_t v_stride, const int32_t* slot, size_t n) {
   if (!c) return bad(nullptr, "null context");
   KvView kv;
   if (const char* msg = kv_view(cache, &kv)) return bad(c, msg);
@@ -645,15 +651,16 @@ int mxq_kv_append(mxq_ctx c, const mxq_kv_cache* cache, int dtype, const void* k
   if (n == 0) return MXQ_OK;
   if (!k || !v || !slot) return bad(c, "kv append: null pointer");
   if (n > (1u << 30)) return bad(c, "kv append: too many rows");
-  if (row_stride < (size_t)kv.heads * kv.dim) return bad(c, "kv append: rows overlap");
-  if (!aligned16(k) || !aligned16(v) || row_stride * es % 16)
+  const size_t row = (size_t)kv.heads * kv.dim;
+  if (k_stride < row || v_stride < row) return bad(c, "kv append: rows overlap");
+  if (!aligned16(k) || !aligned16(v) || k_stride * es % 16 || v_stride * es % 16)
     return bad(c, "kv append: rows must start on 16-byte boundaries");
   ServeDevice g(ctx_device(c));
   const cudaStream_t st = ctx_stream(c);
   const cudaError_t e =
-      dtype == MXQ_DT_F32 ? launch_append<float>(kv, k, v, (long)row_stride, slot, (int)n, st)
-      : dtype == MXQ_DT_BF16 ? launch_append<__nv_bfloat16>(kv, k, v, (long)row_stride, slot, (int)n, st)
-                             : launch_append<__half>(kv, k, v, (long)row_stride, slot, (int)n, st);
+      dtype == MXQ_DT_F32 ? launch_append<float>(kv, k, (long)k_stride, v, (long)v_stride, slot, (int)n, st)
+      : dtype == MXQ_DT_BF16 ? launch_append<__nv_bfloat16>(kv, k, (long)k_stride, v, (long)v_stride, slot, (int)n, st)
+                             : launch_append<__half>(kv, k, (long)k_stride, v, (long)v_stride, slot, (int)n, st);
   return serve_launched(c, e, "kv append");
 }
 

@@ -183,11 +183,11 @@ void kv_append(uintptr_t ctx, const KVCache& cache, const Tensor& k, const Tenso
   const int64_t n = slots.numel();
   if (k.sizes() != at::IntArrayRef({n, cache.c.n_kv_heads, cache.c.head_dim}))
     refuse("kv_append: k and v must be [n][heads][head_dim] of the cache with one slot a row");
-  const int64_t stride = row_stride(k, "k");
-  if (row_stride(v, "v") != stride) refuse("kv_append: k and v must have the same row stride");
   same_device(cache.k, {&cache.v, &cache.k_scale, &cache.v_scale, &k, &v, &slots});
   const mxq_kv_cache c = cache.now();
-  check(mxq_kv_append(bind(ctx, k), &c, dt, k.data_ptr(), v.data_ptr(), stride, ptr<int32_t>(slots), n), ctx);
+  check(mxq_kv_append_strided(bind(ctx, k), &c, dt, k.data_ptr(), row_stride(k, "k"), v.data_ptr(), row_stride(v, "v"),
+                              ptr<int32_t>(slots), n),
+        ctx);
   written({&cache.k, &cache.v, &cache.k_scale, &cache.v_scale});
 }
 

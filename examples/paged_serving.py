@@ -76,7 +76,7 @@ class PagedDecoder:
         for w in self.layers:
             qkv = mx.mx_linear(self._norm(x), w["qkv"])
             q, k, v = (t.unflatten(1, (-1, c.head_dim)) for t in qkv.split([q_dim, kv_dim, kv_dim], 1))
-            mx.kv_append(w["cache"], self._rotate(k, plan.positions), v.contiguous(), plan.slots)
+            mx.kv_append(w["cache"], self._rotate(k, plan.positions), v, plan.slots)
             att, _ = mx.kv_attention(self._rotate(q, plan.positions), w["cache"], self.table, plan.ctx_len, plan.cu, max_new=max_new,
                                      want_lse=False)
             x = x + mx.mx_linear(att.flatten(1), w["out"])

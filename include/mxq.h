@@ -662,6 +662,12 @@ MXQ_API int mxq_kv_release(mxq_ctx ctx, const uint8_t* done, int32_t* len,
 MXQ_API int mxq_kv_append(mxq_ctx ctx, const mxq_kv_cache* cache, int dtype,
                           const void* k, const void* v, size_t row_stride,
                           const int32_t* slot, size_t n);
+/* The same with a row stride of its own for K and for V: K after a rotary
+ * embedding beside V in the fused rows. */
+MXQ_API int mxq_kv_append_strided(mxq_ctx ctx, const mxq_kv_cache* cache,
+                                  int dtype, const void* k, size_t k_stride,
+                                  const void* v, size_t v_stride,
+                                  const int32_t* slot, size_t n);
 /* Cached tokens back as values: k_out, v_out [n][n_kv_heads][head_dim] of type
  * dtype (exact in fp32 and bf16; a slot outside the pool gives zeros). */
 MXQ_API int mxq_kv_read(mxq_ctx ctx, const mxq_kv_cache* cache,

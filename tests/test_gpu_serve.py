@@ -572,3 +572,25 @@ def test_a_cache_follows_its_tensors(ctx):
               lambda: mx.kv_attention(x, cache, slots[None, :1].contiguous(), slots[:1], slots[:2])):
         with pytest.raises(ValueError):
             f()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n", [1, 3, 40])
+def test_append_k_of_its_own_and_v_as_a_slice(ctx, n, dtype):
+    """What a rotary embedding leaves: K rows of their own beside V rows inside the fused ones, and the other way round."""
+    P, H, D = 32, 2, 64
+    fused = torch.randn((n, 6 * H * D), device="cuda").to(dtype)
+    v = fused[:, 5 * H * D:].unflatten(1, (H, D))
+    k = torch.randn((n, H, D), device="cuda").to(dtype)
+    slots = torch.arange(5, 5 + n, dtype=torch.int32, device="cuda")
+    for a, b in ((k, v), (v, k)):
+        caches = [mx.KVCache.empty(2, P, H, D) for _ in range(2)]
+        mx.kv_append(caches[0], a, b, slots, ctx=ctx)
+        mx.kv_append(caches[1], a.contiguous(), b.contiguous(), slots, ctx=ctx)
+        for name in ("k", "v", "k_scale", "v_scale"):
+            assert torch.equal(getattr(caches[0], name), getattr(caches[1], name))
+    odd = torch.zeros((n, 6 * H * D + 1), device="cuda").to(dtype)[:, :H * D].unflatten(1, (H, D))
+    if n > 1:
+        for a, b in ((k, odd), (odd, k), (k, k[:1].expand(n, H, D))):
+            with pytest.raises(ValueError):
+                mx.kv_append(caches[0], a, b, slots, ctx=ctx)
